@@ -21,6 +21,7 @@ LIB_PATH = os.path.join(HERE, "libgpt2amd.so")
 N_LAYER, N_HEAD, N_EMBD, VOCAB, N_CTX = 12, 12, 768, 50257, 1024
 HEAD_DIM, FFN, QKV = 64, 3072, 2304
 TOTAL_PARAMS = 124439808
+PAGE_TOKENS, PAGE_TILE, BEAM_MAX = 32, 2048, 16           # include/gpt2_pagedkv.h
 DECODE_AUTO, DECODE_MULTI, DECODE_PERSISTENT = -1, 0, 1   # gpt2_decode_graph_create_mode modes
 N_QTENSORS = 1 + 4 * N_LAYER
 
@@ -84,6 +85,11 @@ class GPT2KVCache(C.Structure):
                 ("nHead", C.c_int), ("headDim", C.c_int), ("len", C.c_int)]
 
 
+class GPT2PagedKV(C.Structure):
+    _fields_ = [(n, _vp) for n in ("codes", "scales", "open", "table", "len", "start", "slot", "refs", "status", "plan")] + \
+               [(n, C.c_int) for n in ("nLayer", "nHead", "headDim", "nPages", "nSeq", "maxPages")] + [("arena", _vp)]
+
+
 class GPT2Backend(C.Structure):
     _fields_ = [("name", C.c_char_p)] + [(n, _vp) for n in (
         "embed", "layernorm", "matmul", "attention", "gelu", "add", "matmul_q", "gemv", "gemv_q")]
@@ -92,6 +98,7 @@ class GPT2Backend(C.Structure):
 # (name, restype, argtypes) for every symbol declared in include/*.h plus the test/tuning hooks.
 _i, _u, _sz, _d = C.c_int, C.c_uint, C.c_size_t, C.c_double
 _BE = C.POINTER(GPT2Backend)
+_PKV = C.POINTER(GPT2PagedKV)
 SIGNATURES = {
     # include/gpt2_kernels.h
     "gpt2_load_weights": (_i, [C.c_char_p, C.POINTER(GPT2Weights)]),
@@ -164,6 +171,21 @@ SIGNATURES = {
     "gpt2_decode_graph_sync": (_i, [_vp, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "gpt2_decode_graph_destroy": (None, [_vp]),
     "gpt2_decode_graph_time": (_i, [_vp, _i, _fp]),
+    # include/gpt2_pagedkv.h
+    "gpt2_pkv_alloc": (_i, [_PKV, _i, _i, _i, _i, _i]),
+    "gpt2_pkv_free": (None, [_PKV]),
+    "gpt2_pkv_reset": (None, [_PKV]),
+    "gpt2_pkv_status": (_i, [_PKV]),
+    "gpt2_pkv_grow": (None, [_PKV, _vp, _i]),
+    "gpt2_pkv_embed": (None, [_vp, _vp, _vp, _vp, _PKV, _vp, _i]),
+    "gpt2_pkv_append": (None, [_PKV, _i, _vp, _vp, _i]),
+    "gpt2_pkv_attn_ws": (_sz, [_PKV, _i]),
+    "gpt2_pkv_attn": (None, [_vp, _vp, _PKV, _i, _vp, _i, _i, _vp, _sz]),
+    "gpt2_pkv_read": (None, [_vp, _PKV, _i, _vp, _vp, _i]),
+    "gpt2_pkv_fork": (None, [_PKV, _vp]),
+    "gpt2_pkv_compact": (None, [_PKV]),
+    "gpt2_beam_select_ws": (_sz, [_i, _i, _i]),
+    "gpt2_beam_select": (None, [_vp, _vp, _vp, _vp, _vp, C.c_long, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
     # bench / tuning hooks (not part of the reference interface)
     "gpt2_tune_gemm_count": (_i, []),
     "gpt2_tune_gemm_name": (C.c_char_p, [_i]),
@@ -337,6 +359,24 @@ class KVCache:
 
     def free(self) -> None:
         lib().gpt2_kv_free(C.byref(self.kv))
+
+
+def pkv_plan_ints(n_seq: int, max_pages: int, n_pages: int) -> int:
+    """GPT2_PKV_PLAN_INTS: the words of a paged cache's plan buffer."""
+    return n_seq * max_pages + 4 * n_seq + 3 * n_pages + 16
+
+
+class PagedKV:
+    """A paged INT8 K/V cache for several sequences (gpt2_pkv_alloc)."""
+
+    def __init__(self, n_pages: int, n_seq: int, max_len: int = N_CTX, n_layer: int = N_LAYER, n_head: int = N_HEAD):
+        self.c = GPT2PagedKV()
+        if lib().gpt2_pkv_alloc(C.byref(self.c), n_layer, n_head, n_pages, n_seq, max_len):
+            check("gpt2_pkv_alloc")
+            raise GPUError("gpt2_pkv_alloc failed")
+
+    def free(self) -> None:
+        lib().gpt2_pkv_free(C.byref(self.c))
 
 
 def half_bits_to_f32(h: np.ndarray) -> np.ndarray:

@@ -1,0 +1,610 @@
+// pagedkv.hip -- the paged K/V cache (gpt2_pagedkv.h): bookkeeping of its pages (growing, forking, compacting), the
+// append that quantises complete pages, and reading rows back.  Its attention is attn_paged.hip.
+//
+// All of it is bound by memory or, at the sizes of a decode step, by launch latency: the kernels are few, take what
+// depends on the sequences' lengths from device memory, and never come back to the host.
+#include <cmath>
+#include <cstring>
+
+#include "pagedkv.h"
+
+namespace g2 {
+
+// The plan buffer: staged page tables | per-sequence words | per-page words | a few words.
+struct PkvPlan {
+    int *tables;                   // [nSeq][maxPages]
+    int *len, *slot, *from;        // [nSeq] after a fork; from: the open page copied, or -1
+    int *map, *hole, *mover;       // [nPages] of a compaction; a grow's free pages are in map
+    int *word;                     // [0] moves of a compaction, [1] a fork's parents are in range
+};
+__host__ __device__ __forceinline__ PkvPlan pkv_plan(const GPT2PagedKV &c) {
+    PkvPlan p;
+    p.tables = c.plan;
+    p.len = p.tables + (size_t)c.nSeq * c.maxPages;
+    p.slot = p.len + c.nSeq;
+    p.from = p.slot + c.nSeq;
+    p.map = p.len + 4 * (size_t)c.nSeq;
+    p.hole = p.map + c.nPages;
+    p.mover = p.hole + c.nPages;
+    p.word = p.mover + c.nPages;
+    return p;
+}
+
+// Exclusive sum over a work-group of 64 NW threads; `total` for all.  Ends with a barrier, so `lds` can be used again.
+template <int NW>
+__device__ __forceinline__ int block_scan(int v, int *lds, int &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += u;
+    }
+    if (lane == 63) lds[w] = sum;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const int x = lds[i];
+        if (i < w) before += x;
+        total += x;
+    }
+    __syncthreads();
+    return before + sum - v;
+}
+
+__global__ void k_pkv_reset(GPT2PagedKV c) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < c.nSeq) {
+        c.len[i] = 0;
+        c.start[i] = 0;
+        c.slot[i] = i;
+    }
+    if (i < c.nPages) c.refs[i] = 0;
+    if (i < 4) c.status[i] = 0;
+}
+
+// ------------------------------------------------------------------ grow
+// One work-group: needs and their sums over the sequences, then a walk over refs that hands the lowest free pages out in
+// order, which stops when enough are found.  Table entries past the complete pages mean nothing, so they are written as
+// pages are found; refs and lengths follow once all are.
+__global__ __launch_bounds__(1024) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
+    __shared__ int off[GPT2_PKV_MAX_SEQ], lds[16];
+    constexpr int PER = GPT2_PKV_MAX_SEQ / 1024;
+    const int tid = threadIdx.x;
+    const PkvPlan plan = pkv_plan(c);
+    int len[PER], need[PER], sum = 0;
+    bool bad_arg = false, bad_len = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int s = tid * PER + j;
+        len[j] = need[j] = 0;
+        if (s < c.nSeq) {
+            const int a = rows[s], b = rows[s + 1];
+            len[j] = c.len[s];
+            bad_arg |= a < 0 || b < a || b > nRows || len[j] < 0;
+            const long after = (long)len[j] + (b - a);
+            bad_len |= after > (long)c.maxPages * PKV_P;
+            need[j] = (bad_arg || bad_len) ? 0 : (int)(after / PKV_P) - len[j] / PKV_P;
+        }
+        sum += need[j];
+    }
+    const bool arg = __syncthreads_or(bad_arg), cap = __syncthreads_or(bad_len);
+    int total;
+    int at = block_scan<16>(sum, lds, total);
+    bool full = cap;
+    if (!arg && !cap && total > 0) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            off[tid * PER + j] = at;
+            at += need[j];
+        }
+        __syncthreads();
+        int found = 0;
+        for (int base = 0; base < c.nPages && found < total; base += 4 * 1024) {
+            const int p0 = base + 4 * tid;
+            bool is_free[4];
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                is_free[j] = p0 + j < c.nPages && c.refs[p0 + j] == 0;
+                n += is_free[j];
+            }
+            int here, k = found + block_scan<16>(n, lds, here);
+            found += here;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (is_free[j]) {
+                    if (k < total) {
+                        // the last sequence whose pages begin at or before the k-th; it needs one
+                        int lo = 0, hi = c.nSeq;
+                        while (hi - lo > 1) {
+                            const int mid = (lo + hi) >> 1;
+                            if (off[mid] <= k) lo = mid;
+                            else hi = mid;
+                        }
+                        c.table[(size_t)lo * c.maxPages + c.len[lo] / PKV_P + (k - off[lo])] = p0 + j;
+                        plan.map[k] = p0 + j;
+                    }
+                    ++k;
+                }
+        }
+        full = found < total;   // the same in every thread
+        __syncthreads();
+        if (!full)
+            for (int k = tid; k < total; k += 1024) c.refs[plan.map[k]] = 1;
+    }
+    const bool refuse = arg || full;
+    if (refuse && tid == 0) atomicCAS(c.status, 0, arg ? E_ARG : E_CAPACITY);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int s = tid * PER + j;
+        if (s < c.nSeq) {
+            c.start[s] = len[j];
+            if (!refuse) c.len[s] = len[j] + (rows[s + 1] - rows[s]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ embed
+__global__ __launch_bounds__(256) void k_pkv_embed(uint16_t *__restrict__ x, const uint16_t *__restrict__ wte,
+                                                   const uint16_t *__restrict__ wpe, const int *__restrict__ ids, GPT2PagedKV c,
+                                                   const int *__restrict__ rows, int nRows) {
+    constexpr int E = GPT2_N_EMBD;
+    const int row = blockIdx.x;
+    const int s = pkv_seq_of_row(rows, c.nSeq, row);
+    if (s < 0) return;
+    const PkvSeq q = pkv_seq(c, rows, nRows, s);
+    if (q.n == 0) return;
+    const int pos = q.start + row - q.row0, id = ids[row];
+    for (int e = threadIdx.x; e < E; e += 256) {
+        const float te = (unsigned)id < (unsigned)GPT2_VOCAB ? h2f(wte[(size_t)id * E + e]) : 0.f;
+        const float pe = (unsigned)pos < (unsigned)GPT2_N_CTX ? h2f(wpe[(size_t)pos * E + e]) : 0.f;
+        x[(size_t)row * E + e] = f2h(te + pe);
+    }
+}
+
+// ------------------------------------------------------------------ append
+// What the cache can hold of a value: codes stand for finite numbers only.
+__device__ __forceinline__ f16 pkv_finite(f16 v) {
+    const float f = (float)v;
+    return f != f ? (f16)0.f : (f16)fminf(fmaxf(f, -65504.f), 65504.f);
+}
+
+// A sequence's units: the pages that its new rows complete, one at least.  Unit 0 also writes the open page, whose rows
+// before the call it reads, so no other work-group touches it.
+__device__ __forceinline__ int pkv_append_units(const PkvSeq &q) {
+    return q.n ? max(1, q.len / PKV_P - q.start / PKV_P) : 0;
+}
+
+// One wave per unit, K|V and head.  Lane l holds dims 8 (l & 7) .. + 7 of tokens 8 i + l / 8 (i < 4), 16-byte loads of
+// whole row pieces; the block's maximum is the wave's.  A V tile's order (8 tokens of a dim together) is reached through
+// a tile of bytes in LDS.
+__device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, const uint16_t *__restrict__ qkv, const PkvSeq &q,
+                                                int seq, int u, int kv, int h, uint8_t *lds) {
+    const int lane = threadIdx.x & 63, t = lane >> 3, d0 = (lane & 7) * 8;
+    const int E = c.nHead * PKV_D;
+    const int had = q.start / PKV_P, full = q.len / PKV_P;
+    const uint16_t *src = qkv + (size_t)q.row0 * 3 * E + (1 + kv) * E + h * PKV_D;   // row of position start
+    uint16_t *open = c.open + pkv_tile(c, c.nSeq, L, q.slot, kv, h) * PKV_TILE;
+    if (had + u < full) {
+        const int page = c.table[(size_t)seq * c.maxPages + had + u];
+        f16 x[4][8];
+        float peak = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tok = 8 * i + t, pos = (had + u) * PKV_P + tok;
+            if (pos >= q.start) {
+                const f16x8 v = *reinterpret_cast<const f16x8 *>(src + (size_t)(pos - q.start) * 3 * E + d0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = pkv_finite(v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[i][e] = __builtin_bit_cast(f16, open[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) peak = fmaxf(peak, fabsf((float)x[i][e]));
+        }
+        peak = wave_max_u(peak);
+        const float scale = peak == 0.f ? 1.0f : peak / 127.0f;
+        if (pkv_page_ok(c, page)) {
+            const size_t at = pkv_tile(c, c.nPages, L, page, kv, h);
+            int8_t *tile = c.codes + at * PKV_TILE;
+            if (lane == 0) c.scales[at] = scale;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float r = fminf(fmaxf(rintf((float)x[i][e] / scale), -127.f), 127.f);
+                    const uint32_t b = (uint32_t)(int)r & 255u;
+                    if (kv) lds[pkv_v_at(8 * i + t, d0 + e)] = (uint8_t)b;
+                    else w[e >> 2] |= b << (8 * (e & 3));
+                }
+                if (!kv) *reinterpret_cast<uint2 *>(tile + pkv_k_at(8 * i + t, d0)) = uint2{w[0], w[1]};
+            }
+            if (kv) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is this wave's own
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<i32x4 *>(tile + 1024 * i + 16 * lane) = *reinterpret_cast<const i32x4 *>(lds + 1024 * i + 16 * lane);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        }
+    }
+    if (u == 0) {
+        for (int pos = max(q.start, full * PKV_P); pos < q.len; ++pos) {
+            const int tok = pos % PKV_P;
+            const f16 v = pkv_finite(__builtin_bit_cast(f16, src[(size_t)(pos - q.start) * 3 * E + lane]));
+            open[kv ? pkv_v_at(tok, lane) : pkv_k_at(tok, lane)] = __builtin_bit_cast(uint16_t, v);
+        }
+    }
+}
+
+// BY_SEQ: a work-group per sequence that does all of its units (no more rows than sequences: nearly always one unit each);
+// else one per unit.
+template <bool BY_SEQ>
+__global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const uint16_t *__restrict__ qkv,
+                                                    const int *__restrict__ rows, int nRows) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4][PKV_TILE];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kh = blockIdx.y * 4 + w;
+    if (kh >= 2 * c.nHead) return;   // wave-uniform; no barrier follows
+    int u = BY_SEQ ? 0 : blockIdx.x;
+    const int seq = BY_SEQ ? (int)blockIdx.x : pkv_seq_of_unit(u, c.nSeq, [&](int s) { return pkv_append_units(pkv_seq(c, rows, nRows, s)); });
+    if (seq < 0) return;
+    const PkvSeq q = pkv_seq(c, rows, nRows, seq);
+    const int kv = kh >= c.nHead, h = kh - kv * c.nHead;
+    if constexpr (BY_SEQ) {
+        const int n = pkv_append_units(q);
+        for (u = 0; u < n; ++u) pkv_append_unit(c, L, qkv, q, seq, u, kv, h, lds[w]);
+    } else {
+        pkv_append_unit(c, L, qkv, q, seq, u, kv, h, lds[w]);
+    }
+}
+
+// ------------------------------------------------------------------ read
+__global__ __launch_bounds__(256) void k_pkv_read(uint16_t *__restrict__ out, GPT2PagedKV c, int L, const int *__restrict__ rows,
+                                                  const int *__restrict__ pos0, int nRows) {
+    const int row = blockIdx.x;
+    const int s = pkv_seq_of_row(rows, c.nSeq, row);
+    if (s < 0) return;
+    const int len = min(c.len[s], c.maxPages * PKV_P), slot = c.slot[s];
+    const long pos = (long)pos0[s] + (row - rows[s]);
+    const bool there = pos >= 0 && pos < len;
+    const int p = there ? (int)(pos / PKV_P) : 0, tok = there ? (int)(pos % PKV_P) : 0;
+    const bool opened = p >= len / PKV_P;
+    const int page = there && !opened ? c.table[(size_t)s * c.maxPages + p] : -1;
+    for (int i = threadIdx.x; i < 2 * c.nHead * (PKV_D / 8); i += 256) {
+        const int d0 = (i & 7) * 8, kh = i >> 3, kv = kh >= c.nHead, h = kh - kv * c.nHead;
+        f16x8 v = {};
+        if (there && opened && (unsigned)slot < (unsigned)c.nSeq) {
+            const uint16_t *t = c.open + pkv_tile(c, c.nSeq, L, slot, kv, h) * PKV_TILE;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(f16, t[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)]);
+        } else if (pkv_page_ok(c, page)) {
+            const size_t at = pkv_tile(c, c.nPages, L, page, kv, h);
+            const int8_t *t = c.codes + at * PKV_TILE;
+            const float scale = c.scales[at];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (f16)((float)t[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)] * scale);
+        }
+        *reinterpret_cast<f16x8 *>(out + (size_t)row * 2 * c.nHead * PKV_D + (size_t)kh * PKV_D + d0) = v;
+    }
+}
+
+// ------------------------------------------------------------------ fork
+// First launch: work-group s < nSeq stages sequence s's page table and settles its pages' counts by its children; the last
+// one settles the open pages: a parent's first child keeps its slot, the others (and empty ones) take, in order, the slots of the
+// sequences without a child, of which there are as many.
+__global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int *__restrict__ parent) {
+    __shared__ int lds[4], children[GPT2_PKV_MAX_SEQ], first[GPT2_PKV_MAX_SEQ], spare[GPT2_PKV_MAX_SEQ];
+    const int tid = threadIdx.x, me = blockIdx.x;
+    const PkvPlan plan = pkv_plan(c);
+    bool bad = false;
+    if (me < c.nSeq) {
+        int mine = 0;
+        for (int i = tid; i < c.nSeq; i += 256) {
+            const int p = parent[i];
+            bad |= p < -1 || p >= c.nSeq;
+            mine += p == me;
+        }
+        if (__syncthreads_or(bad)) return;
+        int n;
+        block_scan<4>(mine, lds, n);
+        const int full = min(c.len[me] / PKV_P, c.maxPages);
+        for (int t = tid; t < full; t += 256) {
+            const int page = c.table[(size_t)me * c.maxPages + t];
+            plan.tables[(size_t)me * c.maxPages + t] = page;
+            if (n != 1 && pkv_page_ok(c, page)) atomicAdd(c.refs + page, n - 1);
+        }
+        return;
+    }
+    for (int i = tid; i < c.nSeq; i += 256) {
+        children[i] = 0;
+        first[i] = c.nSeq;
+    }
+    __syncthreads();
+    for (int i = tid; i < c.nSeq; i += 256) {
+        const int p = parent[i];
+        if (p < -1 || p >= c.nSeq) bad = true;
+        else if (p >= 0) {
+            atomicAdd(children + p, 1);
+            atomicMin(first + p, i);
+        }
+    }
+    bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        plan.word[1] = !bad;
+        if (bad) atomicCAS(c.status, 0, E_ARG);
+    }
+    if (bad) return;
+    const int per = (c.nSeq + 255) / 256, i0 = min(tid * per, c.nSeq), i1 = min(i0 + per, c.nSeq);
+    int n = 0, total;
+    for (int i = i0; i < i1; ++i) n += children[i] == 0;
+    int k = block_scan<4>(n, lds, total);
+    for (int i = i0; i < i1; ++i)
+        if (children[i] == 0) spare[k++] = c.slot[i];
+    n = 0;
+    for (int i = i0; i < i1; ++i) n += parent[i] < 0 || first[parent[i]] != i;
+    k = block_scan<4>(n, lds, total);   // its barriers order spare's writes before the reads below
+    for (int i = i0; i < i1; ++i) {
+        const int p = parent[i];
+        const bool heir = p >= 0 && first[p] == i;
+        plan.len[i] = p >= 0 ? c.len[p] : 0;
+        plan.slot[i] = heir ? c.slot[p] : spare[k++];
+        plan.from[i] = heir || p < 0 ? -1 : c.slot[p];
+    }
+}
+
+// Second launch: blockIdx.y 0 the books, y > 0 layer y - 1's open page of sequence blockIdx.x, only the tokens in it.
+__global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__restrict__ parent) {
+    const int me = blockIdx.x, tid = threadIdx.x;
+    const PkvPlan plan = pkv_plan(c);
+    if (!plan.word[1]) {
+        if (blockIdx.y == 0 && tid == 0) c.start[me] = c.len[me];
+        return;
+    }
+    const int p = parent[me], len = plan.len[me];
+    if (blockIdx.y == 0) {
+        if (tid == 0) {
+            c.len[me] = c.start[me] = len;
+            c.slot[me] = plan.slot[me];
+        }
+        if (p < 0 || p == me) return;
+        for (int t = tid; t < min(len / PKV_P, c.maxPages); t += 256)
+            c.table[(size_t)me * c.maxPages + t] = plan.tables[(size_t)p * c.maxPages + t];
+        return;
+    }
+    const int from = plan.from[me], to = plan.slot[me], used = len % PKV_P;
+    if (used <= 0 || (unsigned)from >= (unsigned)c.nSeq || (unsigned)to >= (unsigned)c.nSeq) return;
+    const int L = blockIdx.y - 1, H = c.nHead;
+    const uint16_t *src = c.open + pkv_tile(c, c.nSeq, L, from, 0, 0) * PKV_TILE;
+    uint16_t *dst = c.open + pkv_tile(c, c.nSeq, L, to, 0, 0) * PKV_TILE;
+    const int kc = used * PKV_D / 8, vc = (used >> 3) * PKV_D;   // 16-byte pieces of a K tile, of a V tile's whole octets
+    for (int i = tid; i < H * kc; i += 256) {
+        const size_t at = (size_t)(i / kc) * PKV_TILE + 8 * (i % kc);
+        *reinterpret_cast<i32x4 *>(dst + at) = *reinterpret_cast<const i32x4 *>(src + at);
+    }
+    src += (size_t)H * PKV_TILE;
+    dst += (size_t)H * PKV_TILE;
+    for (int i = tid; i < H * vc; i += 256) {
+        const size_t at = (size_t)(i / vc) * PKV_TILE + 8 * (i % vc);
+        *reinterpret_cast<i32x4 *>(dst + at) = *reinterpret_cast<const i32x4 *>(src + at);
+    }
+    if (used & 7)
+        for (int i = tid; i < H * PKV_D; i += 256)
+            for (int t = used & ~7; t < used; ++t) {
+                const size_t at = (size_t)(i / PKV_D) * PKV_TILE + pkv_v_at(t, i % PKV_D);
+                dst[at] = src[at];
+            }
+}
+
+// ------------------------------------------------------------------ compact
+// First launch, one work-group: live pages counted, then ranked: holes below the count, movers at or past it (as many).
+__global__ __launch_bounds__(1024) void k_pkv_compact_plan(GPT2PagedKV c) {
+    __shared__ int lds[16];
+    const int tid = threadIdx.x;
+    const PkvPlan plan = pkv_plan(c);
+    int n = 0, live;
+    for (int p = tid; p < c.nPages; p += 1024) n += c.refs[p] != 0;
+    block_scan<16>(n, lds, live);
+    int holes = 0, movers = 0;
+    for (int base = 0; base < c.nPages; base += 4 * 1024) {
+        const int p0 = base + 4 * tid;
+        bool hole[4], mover[4];
+        int mine = 0;   // holes in the upper half, movers in the lower: at most 4096 of a step
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + j;
+            const bool in = p < c.nPages, used = in && c.refs[p] != 0;
+            hole[j] = in && !used && p < live;
+            mover[j] = used && p >= live;
+            mine += (hole[j] << 16) + mover[j];
+            if (in) plan.map[p] = p;
+        }
+        int total;
+        const int before = block_scan<16>(mine, lds, total);
+        int kh = holes + (before >> 16), km = movers + (before & 0xffff);
+        holes += total >> 16;
+        movers += total & 0xffff;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (hole[j]) plan.hole[kh++] = p0 + j;
+            if (mover[j]) plan.mover[km++] = p0 + j;
+        }
+    }
+    __syncthreads();
+    for (int k = tid; k < movers; k += 1024) {
+        const int to = plan.hole[k], from = plan.mover[k];
+        plan.map[from] = to;
+        c.refs[to] = c.refs[from];
+        c.refs[from] = 0;
+    }
+    if (tid == 0) {
+        plan.word[0] = movers;
+        c.status[1] = live;
+    }
+}
+
+// Second launch: the first `copiers` work-groups move pages (a unit is a page's codes and scales of one layer), the
+// others renumber the page tables.
+__global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers) {
+    const int tid = threadIdx.x;
+    const PkvPlan plan = pkv_plan(c);
+    if ((int)blockIdx.x >= copiers) {
+        const size_t i = (size_t)(blockIdx.x - copiers) * 256 + tid;
+        if (i >= (size_t)c.nSeq * c.maxPages) return;
+        const int s = (int)(i / c.maxPages), t = (int)(i % c.maxPages);
+        if (t >= c.len[s] / PKV_P) return;
+        const int page = c.table[i];
+        if (pkv_page_ok(c, page)) c.table[i] = plan.map[page];
+        return;
+    }
+    const long units = (long)plan.word[0] * c.nLayer;
+    const int pieces = 2 * c.nHead * (PKV_TILE / 16);
+    for (long u = blockIdx.x; u < units; u += copiers) {
+        const int k = (int)(u / c.nLayer), L = (int)(u % c.nLayer);
+        const size_t from = pkv_tile(c, c.nPages, L, plan.mover[k], 0, 0), to = pkv_tile(c, c.nPages, L, plan.hole[k], 0, 0);
+        const i32x4 *src = reinterpret_cast<const i32x4 *>(c.codes + from * PKV_TILE);
+        i32x4 *dst = reinterpret_cast<i32x4 *>(c.codes + to * PKV_TILE);
+        for (int i = tid; i < pieces; i += 256) dst[i] = src[i];
+        for (int i = tid; i < 2 * c.nHead; i += 256) c.scales[to + i] = c.scales[from + i];
+    }
+}
+
+// ------------------------------------------------------------------ host
+bool pkv_refused(const GPT2PagedKV *c, const char *what) {
+    if (!c) return arg_fail(what);
+    const void *p[] = {c->scales, c->table, c->len, c->start, c->slot, c->refs, c->status, c->plan};
+    for (const void *q : p)
+        if (!q || ((uintptr_t)q & 3)) return arg_fail(what);
+    if (!c->codes || !c->open || !aligned16(c->codes) || !aligned16(c->open)) return arg_fail(what);
+    if (c->headDim != PKV_D || c->nLayer < 1 || c->nLayer > 65000 || c->nHead < 1 || c->nHead > 4096 || c->nPages < 1 || c->nPages > (1 << 26) ||
+        c->nSeq < 1 || c->nSeq > GPT2_PKV_MAX_SEQ || c->maxPages < 1 || c->maxPages > (1 << 25) ||
+        (long)c->nSeq * c->maxPages > (1L << 30))
+        return arg_fail(what);
+    return false;
+}
+
+bool pkv_refused_batch(const GPT2PagedKV *c, int L, const int *rows, int nRows, const char *what) {
+    if (pkv_refused(c, what)) return true;
+    if (L < 0 || L >= c->nLayer || !rows || ((uintptr_t)rows & 3) || nRows < 0 || nRows > (1 << 24)) return arg_fail(what);
+    return false;
+}
+
+}  // namespace g2
+
+using namespace g2;
+
+static size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+extern "C" int gpt2_pkv_alloc(GPT2PagedKV *c, int nLayer, int nHead, int nPages, int nSeq, int maxLen) {
+    if (!c) return arg_fail("gpt2_pkv_alloc: null cache"), 1;
+    memset(c, 0, sizeof(*c));
+    if (nLayer < 1 || nLayer > 65000 || nHead < 1 || nHead > 4096 || nPages < 1 || nPages > (1 << 26) || nSeq < 1 || nSeq > GPT2_PKV_MAX_SEQ || maxLen < 1 ||
+        maxLen > (1 << 30) || (long)nSeq * cdiv(maxLen, PKV_P) > (1L << 30))
+        return arg_fail("gpt2_pkv_alloc: sizes out of range"), 1;
+    const size_t maxPages = cdiv(maxLen, PKV_P), tiles = (size_t)nLayer * nPages * 2 * nHead, opens = (size_t)nLayer * nSeq * 2 * nHead;
+    const size_t sizes[] = {tiles * PKV_TILE, tiles * 4, opens * PKV_TILE * 2, (size_t)nSeq * maxPages * 4, (size_t)nSeq * 4, (size_t)nSeq * 4,
+                            (size_t)nSeq * 4, (size_t)nPages * 4, 16, GPT2_PKV_PLAN_INTS(nSeq, maxPages, nPages) * 4};
+    size_t total = 0;
+    for (size_t n : sizes) total += align16(n);
+    size_t freeB = 0, totB = 0;
+    if (hipMemGetInfo(&freeB, &totB) != hipSuccess || total + ((size_t)64 << 20) > freeB) return set_error(E_CAPACITY, "gpt2_pkv_alloc: not enough memory"), 1;
+    char *p = (char *)gpt2_dmalloc(total);
+    if (!p) return 1;
+    void **field[] = {(void **)&c->codes, (void **)&c->scales, (void **)&c->open, (void **)&c->table, (void **)&c->len,
+                      (void **)&c->start, (void **)&c->slot, (void **)&c->refs, (void **)&c->status, (void **)&c->plan};
+    c->arena = p;
+    for (size_t i = 0; i < sizeof sizes / sizeof *sizes; ++i) {
+        *field[i] = p;
+        p += align16(sizes[i]);
+    }
+    c->nLayer = nLayer;
+    c->nHead = nHead;
+    c->headDim = PKV_D;
+    c->nPages = nPages;
+    c->nSeq = nSeq;
+    c->maxPages = (int)maxPages;
+    gpt2_pkv_reset(c);
+    return 0;
+}
+
+extern "C" void gpt2_pkv_free(GPT2PagedKV *c) {
+    if (c && c->arena) {
+        gpt2_dfree(c->arena);
+        memset(c, 0, sizeof(*c));
+    }
+}
+
+extern "C" void gpt2_pkv_reset(GPT2PagedKV *c) {
+    if (pkv_refused(c, "gpt2_pkv_reset: bad cache")) return;
+    const int n = c->nPages > c->nSeq ? c->nPages : c->nSeq;
+    hipLaunchKernelGGL(k_pkv_reset, dim3(cdiv(n, 256)), dim3(256), 0, stream(), *c);
+    check_launch("k_pkv_reset");
+}
+
+extern "C" int gpt2_pkv_status(GPT2PagedKV *c) {
+    if (pkv_refused(c, "gpt2_pkv_status: bad cache")) return E_ARG;
+    int code = 0;
+    const int none = 0;
+    if (int e = gpt2_d2h(&code, c->status, sizeof code)) return e;
+    if (code) {
+        gpt2_h2d(c->status, &none, sizeof none);
+        set_error(code, code == E_CAPACITY ? "paged K/V cache: no free page, or a sequence longer than its table" : "paged K/V cache: offsets or parents out of range");
+    }
+    return code;
+}
+
+extern "C" void gpt2_pkv_grow(GPT2PagedKV *c, const int *rows, int nRows) {
+    if (pkv_refused_batch(c, 0, rows, nRows, "gpt2_pkv_grow: bad cache or rows")) return;
+    hipLaunchKernelGGL(k_pkv_grow, dim3(1), dim3(1024), 0, stream(), *c, rows, nRows);
+    check_launch("k_pkv_grow");
+}
+
+extern "C" void gpt2_pkv_embed(gpt2_half *x, const gpt2_half *wte, const gpt2_half *wpe, const int *ids, const GPT2PagedKV *c,
+                               const int *rows, int nRows) {
+    if (pkv_refused_batch(c, 0, rows, nRows, "gpt2_pkv_embed: bad cache or rows")) return;
+    if (nRows == 0) return;
+    if (!x || !wte || !wpe || !ids) { arg_fail("gpt2_pkv_embed: null pointer"); return; }
+    hipLaunchKernelGGL(k_pkv_embed, dim3(nRows), dim3(256), 0, stream(), x, wte, wpe, ids, *c, rows, nRows);
+    check_launch("k_pkv_embed");
+}
+
+extern "C" void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, const int *rows, int nRows) {
+    if (pkv_refused_batch(c, L, rows, nRows, "gpt2_pkv_append: bad cache, layer or rows")) return;
+    if (nRows == 0) return;
+    if (!qkv || !aligned16(qkv)) { arg_fail("gpt2_pkv_append: null/unaligned"); return; }
+    const bool by_seq = nRows <= c->nSeq;
+    const dim3 grid(by_seq ? c->nSeq : nRows / PKV_P + c->nSeq, cdiv(2 * c->nHead, 4));
+    const auto fn = by_seq ? k_pkv_append<true> : k_pkv_append<false>;
+    hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream(), *c, L, qkv, rows, nRows);
+    check_launch("k_pkv_append");
+}
+
+extern "C" void gpt2_pkv_read(gpt2_half *kv, const GPT2PagedKV *c, int L, const int *rows, const int *pos, int nRows) {
+    if (pkv_refused_batch(c, L, rows, nRows, "gpt2_pkv_read: bad cache, layer or rows")) return;
+    if (nRows == 0) return;
+    if (!kv || !aligned16(kv) || !pos || ((uintptr_t)pos & 3)) { arg_fail("gpt2_pkv_read: null/unaligned"); return; }
+    hipLaunchKernelGGL(k_pkv_read, dim3(nRows), dim3(256), 0, stream(), kv, *c, L, rows, pos, nRows);
+    check_launch("k_pkv_read");
+}
+
+extern "C" void gpt2_pkv_fork(GPT2PagedKV *c, const int *parent) {
+    if (pkv_refused(c, "gpt2_pkv_fork: bad cache")) return;
+    if (!parent || ((uintptr_t)parent & 3)) { arg_fail("gpt2_pkv_fork: null/unaligned"); return; }
+    hipLaunchKernelGGL(k_pkv_fork_plan, dim3(c->nSeq + 1), dim3(256), 0, stream(), *c, parent);
+    hipLaunchKernelGGL(k_pkv_fork, dim3(c->nSeq, 1 + c->nLayer), dim3(256), 0, stream(), *c, parent);
+    check_launch("k_pkv_fork");
+}
+
+extern "C" void gpt2_pkv_compact(GPT2PagedKV *c) {
+    if (pkv_refused(c, "gpt2_pkv_compact: bad cache")) return;
+    const int copiers = 2048;
+    hipLaunchKernelGGL(k_pkv_compact_plan, dim3(1), dim3(1024), 0, stream(), *c);
+    hipLaunchKernelGGL(k_pkv_compact, dim3(copiers + cdiv((long)c->nSeq * c->maxPages, 256)), dim3(256), 0, stream(), *c, copiers);
+    check_launch("k_pkv_compact");
+}
