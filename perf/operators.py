@@ -324,7 +324,7 @@ def _bind(s):
     c.nSeq, c.maxPages = s["table"].shape
     s["plan"] = torch.zeros(pkg.pkv_plan_ints(c.nSeq, c.maxPages, c.nPages), dtype=torch.int32, device="cuda")
     for name in ("codes", "scales", "open", "table", "len", "start", "slot", "refs", "status", "plan"):
-        setattr(c, name, s[name].data_ptr())
+        setattr(c, name, s[name].data_ptr() or s["codes"].data_ptr())   # a compaction's state has no open pages, and touches none
     s["cache"], ref = c, C.byref(c)
     if op == "attn":
         s["ws"] = torch.empty(lib.gpt2_pkv_attn_ws(ref, s["total"]), dtype=torch.uint8, device="cuda")
