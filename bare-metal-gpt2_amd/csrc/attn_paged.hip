@@ -22,10 +22,11 @@ struct PagedAttn {
     uint16_t *att;
     const uint16_t *qkv;
     const int *rows;
-    int L, nRows, splits;
+    int L, nRows, group, splits, per;
     float *po;      // [splits][nRows][nHead][64] unscaled sums of a split
-    float2 *pml;    // [splits][nRows][nHead] their maximum and weight
+    float4 *pml;    // [splits][nRows][nHead] their maximum and weight, and how many splits there are
 };
+constexpr int ATTN_SPLITS = 64;   // at most
 
 // A page in flight: its K rows and V octets as they lie.
 struct PageRaw {
@@ -33,18 +34,33 @@ struct PageRaw {
 };
 
 // Attention of 16 rows as it accumulates: column jq is a row; o[2 i + b] element r is dim 32 i + 8 g + 2 r + b.
+// m: the running maximum of x; l: the sum of the weights; o: the weighted sum of the values in units of 2^lv.
 struct AttnAcc {
-    float m, l;
+    float m, l, lv;
     f32x4 o[4];
 };
 
-__device__ __forceinline__ void page_load(const int8_t *__restrict__ k, const int8_t *__restrict__ v, PageRaw &R) {
+// A page (K tile, V tile) on its way to a 4 KB stage in LDS: four instructions of 1 KB, whole rows.  The 16-byte pieces of a
+// K row are swizzled by the row (by choosing what each lane fetches), so that the reads below meet no bank conflict.
+__device__ __forceinline__ void page_issue(const int8_t *__restrict__ k, const int8_t *__restrict__ v, char *stage) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int key = 16 * i + (lane >> 2);
+        __builtin_amdgcn_global_load_lds(k + key * PKV_D + 16 * ((lane & 3) ^ (key >> 3)), G2_LDS(stage + 1024 * i), 16, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) __builtin_amdgcn_global_load_lds(v + 1024 * i + 16 * lane, G2_LDS(stage + PKV_TILE + 1024 * i), 16, 0, 0);
+#endif
+}
+__device__ __forceinline__ void page_take(const char *__restrict__ stage, PageRaw &R) {
     const int lane = threadIdx.x & 63, jq = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
-        R.k[t] = *reinterpret_cast<const i32x4 *>(k + (8 * (jq >> 2) + 4 * t + (jq & 3)) * PKV_D + 16 * g);
+        R.k[t] = *reinterpret_cast<const i32x4 *>(stage + (8 * (jq >> 2) + 4 * t + (jq & 3)) * PKV_D + 16 * (g ^ (jq >> 2)));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) R.v[i] = *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * i + 2 * jq) * 8);
+    for (int i = 0; i < 2; ++i) R.v[i] = *reinterpret_cast<const i32x4 *>(stage + PKV_TILE + (g * PKV_D + 32 * i + 2 * jq) * 8);
 }
 
 // 32 tokens from `key0` on against the columns: fragments of K (kf[t]: dims 16 g .. + 7 and + 8 .. + 15 of the lane's key
@@ -52,41 +68,52 @@ __device__ __forceinline__ void page_load(const int8_t *__restrict__ k, const in
 __device__ __forceinline__ void attn_page(AttnAcc &A, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const f16x8 (&q)[2], float sk,
                                           float sv, int key0, int lim, bool masked) {
     const int g = (threadIdx.x & 63) >> 4;
-    float x[8];
+    float s[8];
     const float scale = sk * (0.125f * 1.4426950408889634f);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        f32x4 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][0], q[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][1], q[1], s, 0, 0, 0);
+        f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][0], q[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][1], q[1], y, 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r] * scale;
+        for (int r = 0; r < 4; ++r) s[4 * t + r] = y[r];
     }
     if (masked) {
+        const int n = lim - key0 - 8 * g;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (key0 + 8 * g + e >= lim) x[e] = -INFINITY;
+        for (int e = 0; e < 8; ++e) s[e] = e < n ? s[e] : -INFINITY;
     }
-    float mx = x[0];
+    float mx = s[0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-    const float mn = fmaxf(A.m, group_max(mx));
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
+    const float mn = fmaxf(A.m, group_max(mx) * scale);
     const float base = mn == -INFINITY ? 0.f : mn;   // a column that sees none of these keys
-    const float corr = __builtin_amdgcn_exp2f(A.m - base);
-    A.m = mn;
+    // The maximum moves rarely after the first pages; s_v is a factor of the weights (as an addend of their exponent), so
+    // that P.V adds to o as it is: relative to 2^lv, which follows s_v where that is far from it (fp16 weights).
+    if (__ballot(mn > A.m)) {
+        const float corr = __builtin_amdgcn_exp2f(A.m - base);
+        A.m = mn;
+        A.l *= corr;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A.o[i] *= corr;
+    }
+    const float lsv = __builtin_amdgcn_logf(sv);
+    if (fabsf(lsv - A.lv) > 4.f) {   // the same in every lane
+        const float f = __builtin_amdgcn_exp2f(A.lv - lsv);
+        A.lv = lsv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A.o[i] *= f;
+    }
+    const float add = lsv - A.lv - base;
     f16x8 p;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = (f16)__builtin_amdgcn_exp2f(x[e] - base);
+    for (int e = 0; e < 8; ++e) p[e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[e], scale, add));
     // the weights' sum is that of the fp16 values that the matrix units multiply
     float ps = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) ps = __builtin_amdgcn_fdot2(f16x2{p[e], p[e + 1]}, f16x2{1, 1}, ps, false);
-    A.l = fmaf(A.l, corr, ps);
+    A.l = fmaf(ps, __builtin_amdgcn_exp2f(A.lv - lsv), A.l);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], p, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) A.o[i][r] = fmaf(A.o[i][r], corr, y[r] * sv);
-    }
+    for (int i = 0; i < 4; ++i) A.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], p, A.o[i], 0, 0, 0);
 }
 
 __device__ __forceinline__ void attn_codes(AttnAcc &A, const PageRaw &R, const f16x8 (&q)[2], float sk, float sv, int key0, int lim,
@@ -113,154 +140,288 @@ __device__ __forceinline__ void attn_open(AttnAcc &A, const uint16_t *__restrict
         kf[t][0] = *reinterpret_cast<const f16x8 *>(row);
         kf[t][1] = *reinterpret_cast<const f16x8 *>(row + 8);
     }
+    const int n = used - 8 * g;   // of the lane's 8 tokens, those that are there
+    i32x4 keep;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        vf[i] = *reinterpret_cast<const f16x8 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8);
+    for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (8 * g + e >= used) vf[i][e] = (f16)0.f;
-    }
+    for (int i = 0; i < 4; ++i)
+        vf[i] = __builtin_bit_cast(f16x8, *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8) & keep);
     attn_page(A, kf, vf, q, 1.f, 1.f, key0, lim, true);
 }
 
-// Rows 16 rb .. + 15 of a sequence, one head, one split of the pages; W waves take the pages in turn and join in LDS.
+// What a pass goes over, as steps of a page each: the first `shared` pages of sequence seq0, for every column, then the
+// pages from there on of each of `beams` sequences (lane b holds beam b's), for that beam's column alone.
+struct AttnSteps {
+    int seq0, len0, slot0, shared, total;
+    int beams, seq, len, slot, off;   // off: own pages of the beams before
+};
+
+// One pass: 16 columns (column jq: row `row` of the activations, -1 for none, which sees the keys below `lim`; every
+// column sees those below `first`), one head, split z of the steps.  The W waves take steps in turn and join in LDS.
+constexpr int ATTN_STAGES = 2;
 template <int W>
-__device__ __forceinline__ void attn_rows(const PagedAttn &a, const PkvSeq &s, int seq, int h, int rb, int split) {
-    __shared__ float lds_m[W][16], lds_l[W][16];
-    __shared__ f32x4 lds_o[W][4][64];
+struct AttnLds {
+    char ring[W][ATTN_STAGES * 2 * PKV_TILE];
+    float m[W][16], l[W][16];
+};
+template <int W>
+__device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &st, int h, int z, int row, int lim, int first, AttnLds<W> &lds) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
     const int E = c.nHead * PKV_D;
-    const int i0 = 16 * rb, i = i0 + jq, first = s.start + i0 + 1, lim = s.start + i + 1;   // keys that rows i0 and i see
-    const int end = s.start + min(s.n, i0 + 16), pages = (end + PKV_P - 1) / PKV_P, full = s.len / PKV_P;
-    const int per = (pages + a.splits - 1) / a.splits, p0 = min(pages, split * per), p1 = min(pages, p0 + per);
-    const uint16_t *qrow = a.qkv + (size_t)(s.row0 + min(i, s.n - 1)) * 3 * E + h * PKV_D + 16 * g;
-    const f16x8 q[2] = {*reinterpret_cast<const f16x8 *>(qrow), *reinterpret_cast<const f16x8 *>(qrow + 8)};
+    const int splits = min(a.splits, max(1, (st.total + a.per - 1) / a.per)), stride = splits * W;
+    if (z >= splits) return;   // the whole work-group
+    const uint16_t *qrow = a.qkv + (size_t)max(row, 0) * 3 * E + h * PKV_D + 16 * g;
+    f16x8 q[2] = {};
+    if (row >= 0) {
+        q[0] = *reinterpret_cast<const f16x8 *>(qrow);
+        q[1] = *reinterpret_cast<const f16x8 *>(qrow + 8);
+    }
     AttnAcc A;
     A.m = -INFINITY;
-    A.l = 0.f;
+    A.l = A.lv = 0.f;
 #pragma unroll
     for (int d = 0; d < 4; ++d) A.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int pc = p0 + w; pc < p1; pc += 64 * W) {
-        // the wave's next 64 pages: lane l holds the number and the scales of page pc + W l
-        const int mine = pc + W * lane;
-        int page = mine < min(p1, full) ? c.table[(size_t)seq * c.maxPages + mine] : -1;
-        if (!pkv_page_ok(c, page)) page = -1;
+    const size_t vstep = (size_t)c.nHead * PKV_TILE;   // from a page's K tile to its V tile
+    for (int t0 = z * W + w; t0 < st.total; t0 += 64 * stride) {
+        // the wave's next 64 steps, a lane each: the page's number in its sequence, whose it is, the pool's page, scales
+        const int t = t0 + stride * lane;
+        int b = -1, p = t, seq = st.seq0, len = st.len0;
+        if (st.beams) {   // wave-uniform
+            const int u = t - st.shared;
+            for (int k = 0; k < st.beams; ++k)
+                if (u >= __builtin_amdgcn_readlane(st.off, k)) b = k;
+            const int from = max(b, 0), off = __shfl(st.off, from, 64), s1 = __shfl(st.seq, from, 64), n1 = __shfl(st.len, from, 64);
+            if (b >= 0) {
+                p = st.shared + u - off;
+                seq = s1;
+                len = n1;
+            }
+        }
+        const int full = len / PKV_P;
+        int page = t < st.total && p < full ? c.table[(size_t)seq * c.maxPages + p] : -1;
+        const bool there = pkv_page_ok(c, page);
+        const uint64_t opened = __ballot(t < st.total && p == full);
         float sk = 0.f, sv = 0.f;
-        if (page >= 0) {
+        if (there) {
             const size_t at = pkv_tile(c, c.nPages, a.L, page, 0, h);
             sk = c.scales[at];
             sv = c.scales[at + c.nHead];
         }
-        const int n = min(64, (p1 - pc + W - 1) / W);
-        for (int j = 0; j < n; ++j) {
-            const int p = pc + W * j, key0 = p * PKV_P, pg = __builtin_amdgcn_readlane(page, j);
-            if (p == full) {
-                const uint16_t *k = c.open + pkv_tile(c, c.nSeq, a.L, s.slot, 0, h) * PKV_TILE;
-                attn_open(A, k, k + (size_t)c.nHead * PKV_TILE, s.len - key0, q, key0, lim);
-            } else if (pg >= 0) {
-                const int8_t *k = c.codes + pkv_tile(c, c.nPages, a.L, pg, 0, h) * PKV_TILE;
-                PageRaw R;
-                page_load(k, k + (size_t)c.nHead * PKV_TILE, R);
-                attn_codes(A, R, q, lane_f(sk, j), lane_f(sv, j), key0, lim, key0 + PKV_P > first);
-            }
+        const int who = p << 5 | (b + 1);   // p < 2^25 (maxPages)
+        // complete pages through the wave's own ring of stages: all but one ahead of the one in use
+        uint64_t left = __ballot(there), todo = left;
+        int stage = 0, ahead = 0;   // pages under way
+        char *const ring = lds.ring[w];
+        auto issue = [&](int s) {
+            const int8_t *k = c.codes + pkv_tile(c, c.nPages, a.L, __builtin_amdgcn_readlane(page, __builtin_ctzll(todo)), 0, h) * PKV_TILE;
+            page_issue(k, k + vstep, ring + 2 * PKV_TILE * s);
+            todo &= todo - 1;
+            ++ahead;
+        };
+#pragma unroll
+        for (int s = 0; s < ATTN_STAGES; ++s)
+            if (todo) issue(s);
+        asm volatile("" : "+v"(sk), "+v"(sv));   // waited for here, once, and not with every page under way in the loop
+        while (left) {
+            const int j = __builtin_ctzll(left);
+            left &= left - 1;
+            --ahead;
+            wait_tiles<4, ATTN_STAGES - 1>(ahead);
+            asm volatile("" ::: "memory");
+            PageRaw R;
+            page_take(ring + 2 * PKV_TILE * stage, R);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the stage is filled again
+            if (todo) issue(stage);
+            stage = stage + 1 == ATTN_STAGES ? 0 : stage + 1;
+            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1, key0 = (x >> 5) * PKV_P;
+            attn_codes(A, R, q, lane_f(sk, j), lane_f(sv, j), key0, bj < 0 || bj == jq ? lim : 0, bj >= 0 || key0 + PKV_P > first);
+        }
+        for (uint64_t o = opened; o; o &= o - 1) {
+            const int j = __builtin_ctzll(o);
+            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1, key0 = (x >> 5) * PKV_P;
+            const int slot = bj < 0 ? st.slot0 : __builtin_amdgcn_readlane(st.slot, max(bj, 0));
+            const uint16_t *k = c.open + pkv_tile(c, c.nSeq, a.L, slot, 0, h) * PKV_TILE;
+            attn_open(A, k, k + vstep, __builtin_amdgcn_readlane(len, j) - key0, q, key0, bj < 0 || bj == jq ? lim : 0);
         }
     }
-    const float l = group_sum(A.l);
-    if (g == 0) {
-        lds_m[w][jq] = A.m;
-        lds_l[w][jq] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < 4; ++d) lds_o[w][d][lane] = A.o[d];
+    // the waves' sums to one maximum, then together
+    A.l = group_sum(A.l);
+    if (g == 0) lds.m[w][jq] = A.l != 0.f ? A.m : -INFINITY;
     __syncthreads();
-    if (w < 2) {   // dims 32 w + 8 g .. + 7 of row i
-        float mx = -INFINITY, L = 0.f, f[W];
+    float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < W; ++u) mx = lds_l[u][jq] != 0.f ? fmaxf(mx, lds_m[u][jq]) : mx;
+    for (int u = 0; u < W; ++u) mx = fmaxf(mx, lds.m[u][jq]);
+    const float f = A.l != 0.f ? __builtin_amdgcn_exp2f(A.m - mx) : 0.f;
+    if (row >= 0) {
+        if (g == 0) lds.l[w][jq] = A.l * f;
 #pragma unroll
-        for (int u = 0; u < W; ++u) {
-            f[u] = lds_l[u][jq] != 0.f ? __builtin_amdgcn_exp2f(lds_m[u][jq] - mx) : 0.f;
-            L += lds_l[u][jq] * f[u];
-        }
+        for (int d = 0; d < 4; ++d) reinterpret_cast<f32x4 *>(lds.ring[w])[64 * d + lane] = A.o[d] * (f * __builtin_amdgcn_exp2f(A.lv));   // the ring is idle
+    }
+    __syncthreads();
+    if (w < 2 && row >= 0) {   // dims 32 w + 8 g .. + 7 of the column's row
+        float L = 0.f;
         f32x4 y[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int u = 0; u < W; ++u)
+        for (int u = 0; u < W; ++u) {
+            const f32x4 *o = reinterpret_cast<const f32x4 *>(lds.ring[u]);
+            L += lds.l[u][jq];
+            y[0] += o[128 * w + lane];
+            y[1] += o[128 * w + 64 + lane];
+        }
+        if (a.splits == 1) {
+            const float inv = L != 0.f ? 1.f / L : 0.f;   // no key: 0
+            f16x8 o;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[b][r] = fmaf(lds_o[u][2 * w + b][lane][r], f[u], y[b][r]);
-        if (i < s.n) {
-            const size_t row = s.row0 + i;
-            if (a.splits == 1) {
-                const float inv = L != 0.f ? 1.f / L : 0.f;   // no key: 0
-                f16x8 o;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = (f16)(y[e & 1][e >> 1] * inv);
-                *reinterpret_cast<f16x8 *>(a.att + row * E + h * PKV_D + 32 * w + 8 * g) = o;
-            } else {
-                const size_t at = ((size_t)split * a.nRows + row) * c.nHead + h;
-                float *o = a.po + at * PKV_D + 32 * w + 8 * g;
-                *reinterpret_cast<f32x4 *>(o) = f32x4{y[0][0], y[1][0], y[0][1], y[1][1]};
-                *reinterpret_cast<f32x4 *>(o + 4) = f32x4{y[0][2], y[1][2], y[0][3], y[1][3]};
-                if (w == 0 && g == 0) a.pml[at] = float2{mx, L};
-            }
+            for (int e = 0; e < 8; ++e) o[e] = (f16)(y[e & 1][e >> 1] * inv);
+            *reinterpret_cast<f16x8 *>(a.att + (size_t)row * E + h * PKV_D + 32 * w + 8 * g) = o;
+        } else {
+            const size_t at = ((size_t)z * a.nRows + row) * c.nHead + h;
+            float *o = a.po + at * PKV_D + 32 * w + 8 * g;
+            *reinterpret_cast<f32x4 *>(o) = f32x4{y[0][0], y[1][0], y[0][1], y[1][1]};
+            *reinterpret_cast<f32x4 *>(o + 4) = f32x4{y[0][2], y[1][2], y[0][3], y[1][3]};
+            if (w == 0 && g == 0) a.pml[at] = float4{mx, L, __int_as_float(splits), 0.f};
         }
     }
 }
 
-// BY_SEQ: a work-group takes all row blocks of a sequence (no more rows than sequences: nearly always one block).
-template <int W, bool BY_SEQ>
-__global__ __launch_bounds__(64 * W) void k_pkv_attn(PagedAttn a) {
-    const int h = blockIdx.x % a.c.nHead, split = blockIdx.y;
+// Rows 16 rb .. + 15 of one sequence, as a pass.
+struct AttnCols {
+    int row, lim, first;
+};
+__device__ __forceinline__ AttnSteps attn_rows(const PkvSeq &s, int seq, int rb, AttnCols &col) {
+    const int i0 = 16 * rb, i = i0 + (threadIdx.x & 15), pages = (s.start + min(s.n, i0 + 16) + PKV_P - 1) / PKV_P;
+    col = {i < s.n ? s.row0 + i : -1, i < s.n ? s.start + i + 1 : 0, s.start + i0 + 1};
+    return {seq, s.len, s.slot, pages, pages, 0, 0, 0, 0, 0};
+}
+
+// The beams of a group, one row each at most, as a pass.  Lane b holds beam b's sequence; `on`: those with a row.
+__device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq &s, int seq0, uint64_t on, AttnCols &col) {
+    const GPT2PagedKV &c = a.c;
+    const int lane = threadIdx.x & 63, jq = lane & 15, one = __builtin_ctzll(on);
+    // the leading pages that all share, complete in each
+    int least = s.n ? s.len / PKV_P : 0x7fffffff;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));   // beams are lanes 0 .. 15
+    least = __builtin_amdgcn_readfirstlane(least);
+    int shared = 0;
+    for (; shared < least; shared += 64) {
+        const int p = shared + lane;
+        bool same = p < least;
+        if (same) {
+            const int page = c.table[(size_t)(seq0 + one) * c.maxPages + p];
+            for (int b = one + 1; b < a.group; ++b)
+                if (on >> b & 1) same &= c.table[(size_t)(seq0 + b) * c.maxPages + p] == page;
+        }
+        const uint64_t differ = __ballot(!same);
+        if (differ) {
+            shared += __builtin_ctzll(differ);
+            break;
+        }
+    }
+    const int own = s.n ? (s.len + PKV_P - 1) / PKV_P - shared : 0;
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const int v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+    }
+    const int total = shared + __builtin_amdgcn_readlane(sum, 15);
+    const int n = __shfl(s.n, jq, 64), row = __shfl(s.row0, jq, 64), len = __shfl(s.len, jq, 64);
+    col = {n ? row : -1, n ? len : 0, shared * PKV_P};
+    return {seq0 + one, __builtin_amdgcn_readlane(s.len, one), 0, shared, total, a.group, seq0 + min(lane, a.group - 1), s.len, s.slot, sum - own};
+}
+
+// One row a sequence, nearly always (no more rows than sequences): a work-group per group of beams, head and split.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
+    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+    const int h = blockIdx.x % a.c.nHead, lane = threadIdx.x & 63;
+    const int seq0 = blockIdx.x / a.c.nHead * a.group;
+    PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq0 + min(lane, a.group - 1));
+    if (lane >= a.group) s.n = 0;
+    const uint64_t on = __ballot(s.n > 0);
+    if (!on) return;
+    const bool together = (on & (on - 1)) && !__ballot(s.n > 1);   // else one sequence after another
+    int b = __builtin_ctzll(on), rb = 0;
+    for (;;) {
+        AttnSteps st;
+        AttnCols col;
+        PkvSeq u;
+        u.n = 0;
+        if (together) {
+            st = attn_beams(a, s, seq0, on, col);
+        } else {
+            u.start = __builtin_amdgcn_readlane(s.start, b);
+            u.len = __builtin_amdgcn_readlane(s.len, b);
+            u.row0 = __builtin_amdgcn_readlane(s.row0, b);
+            u.n = __builtin_amdgcn_readlane(s.n, b);
+            u.slot = __builtin_amdgcn_readlane(s.slot, b);
+            st = attn_rows(u, seq0 + b, rb, col);
+        }
+        attn_pass<W>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+        if (together) break;
+        if (16 * ++rb >= u.n) {
+            const uint64_t more = on & ~((2ull << b) - 1);   // b < 16
+            if (!more) break;
+            b = __builtin_ctzll(more);
+            rb = 0;
+        }
+        __syncthreads();
+    }
+}
+
+// Any number of rows a sequence: a work-group per 16 of them, head and split.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_pkv_attn_rows(PagedAttn a) {
+    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+    const int h = blockIdx.x % a.c.nHead;
     int rb = blockIdx.x / a.c.nHead;
-    if constexpr (BY_SEQ) {
-        const int seq = rb;
-        const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
-        for (rb = 0; 16 * rb < s.n; ++rb) {
-            if (rb) __syncthreads();
-            attn_rows<W>(a, s, seq, h, rb, split);
-        }
-    } else {
-        const int seq = pkv_seq_of_unit(rb, a.c.nSeq, [&](int s) { return (pkv_seq(a.c, a.rows, a.nRows, s).n + 15) / 16; });
-        if (seq < 0) return;
-        attn_rows<W>(a, pkv_seq(a.c, a.rows, a.nRows, seq), seq, h, rb, split);
-    }
+    const int seq = pkv_seq_of_unit(rb, a.c.nSeq, [&](int s) { return (pkv_seq(a.c, a.rows, a.nRows, s).n + 15) / 16; });
+    if (seq < 0) return;
+    AttnCols col;
+    const AttnSteps st = attn_rows(pkv_seq(a.c, a.rows, a.nRows, seq), seq, rb, col);
+    attn_pass<W>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
 }
 
-// Joins the splits: a wave per row and head, a lane per dim.
+// Joins the splits: a wave per row and head; lane z holds split z's maximum and weight, then lane d dim d.
 __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
     const int lane = threadIdx.x & 63, h = blockIdx.y * 4 + (threadIdx.x >> 6), row = blockIdx.x;
     if (h >= a.c.nHead) return;
     const int seq = pkv_seq_of_row(a.rows, a.c.nSeq, row);
     if (seq < 0 || pkv_seq(a.c, a.rows, a.nRows, seq).n == 0) return;
-    float mx = -INFINITY, L = 0.f, o = 0.f;
-    for (int z = 0; z < a.splits; ++z) {
-        const float2 ml = a.pml[((size_t)z * a.nRows + row) * a.c.nHead + h];
-        if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
+    const size_t at = (size_t)row * a.c.nHead + h, per = (size_t)a.nRows * a.c.nHead;
+    const int splits = max(1, min(__builtin_amdgcn_readfirstlane(__float_as_int(a.pml[at].z)), a.splits));
+    static_assert(ATTN_SPLITS <= 64, "a lane a split");
+    const float4 ml = a.pml[at + per * min(lane, splits - 1)];
+    const bool on = lane < splits && ml.y != 0.f;
+    const float mx = wave_max_u(on ? ml.x : -INFINITY), f = on ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
+    const float L = wave_sum_u(on ? ml.y * f : 0.f);
+    float o = 0.f;
+    for (int z = 0; z < splits; z += 8) {   // eight loads under way; f is 0 past the last split
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = a.po[(at + per * min(z + i, splits - 1)) * PKV_D + lane];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o = fmaf(v[i], lane_f(f, z + i), o);
     }
-    for (int z = 0; z < a.splits; ++z) {
-        const size_t at = ((size_t)z * a.nRows + row) * a.c.nHead + h;
-        const float2 ml = a.pml[at];
-        if (ml.y == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(ml.x - mx);
-        L = fmaf(ml.y, f, L);
-        o = fmaf(a.po[at * PKV_D + lane], f, o);
-    }
-    a.att[(size_t)row * a.c.nHead * PKV_D + h * PKV_D + lane] = f2h(L != 0.f ? o / L : 0.f);
+    a.att[at * PKV_D + lane] = f2h(L != 0.f ? o / L : 0.f);
 }
 
-// Work-groups of one split, and into how many splits the pages go.
-static long attn_groups(const GPT2PagedKV *c, int nRows) {
-    return (long)(nRows <= c->nSeq ? c->nSeq : nRows / 16 + c->nSeq) * c->nHead;
-}
-static int attn_splits(const GPT2PagedKV *c, int nRows) {
-    const long groups = attn_groups(c, nRows);
-    int n = (int)((1024 + groups - 1) / groups);
-    const int most = cdiv(c->maxPages, 16);
-    if (n > most) n = most;
-    return n < 1 ? 1 : n > 32 ? 32 : n;
+// How the steps are split over work-groups: at least `per` of them each, into `splits` at most.  None for caches whose
+// sequences a work-group's waves get through in the time of a second launch, nor where the rows alone make enough
+// work-groups.  Where splits of 64 pages fill the card they stream best (16 contexts up to 16384 tokens: 51 us, 59 with 16 pages
+// each); fewer sequences need smaller ones (one of 16384: 8.6 us, 14).
+struct AttnSplit {
+    int splits, per;
+};
+static AttnSplit attn_split(const GPT2PagedKV *c, int nRows) {
+    if (c->maxPages <= 64 || (nRows > c->nSeq && (long)(nRows / 16) * c->nHead >= 512)) return {1, 64};
+    const long groups = (long)(nRows > c->nSeq ? nRows / 16 + 1 : c->nSeq) * c->nHead;
+    const int per = groups * (c->maxPages / 64) >= 512 ? 64 : 16, n = cdiv(c->maxPages, per);
+    return {n > ATTN_SPLITS ? ATTN_SPLITS : n, per};
 }
 
 }  // namespace g2
@@ -268,9 +429,9 @@ static int attn_splits(const GPT2PagedKV *c, int nRows) {
 using namespace g2;
 
 extern "C" size_t gpt2_pkv_attn_ws(const GPT2PagedKV *c, int nRows) {
-    if (!c || nRows < 1 || c->nSeq < 1 || c->nHead < 1 || c->maxPages < 1) return 16;
-    const int n = attn_splits(c, nRows);
-    return n == 1 ? 16 : (size_t)n * nRows * c->nHead * (PKV_D + 2) * 4;
+    if (!c || nRows < 1 || c->nHead < 1 || c->maxPages < 1) return 16;
+    const int n = attn_split(c, nRows).splits;
+    return n == 1 ? 16 : (size_t)n * nRows * c->nHead * (PKV_D + 4) * 4;
 }
 
 extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2PagedKV *c, int L, const int *rows, int nRows,
@@ -287,12 +448,19 @@ extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2Pa
     a.rows = rows;
     a.L = L;
     a.nRows = nRows;
-    a.splits = attn_splits(c, nRows);
+    a.group = group;
+    const AttnSplit sp = attn_split(c, nRows);
+    a.splits = sp.splits;
+    a.per = sp.per;
     a.po = (float *)ws;
-    a.pml = (float2 *)(a.po + (size_t)a.splits * nRows * c->nHead * PKV_D);
-    const dim3 grid((unsigned)attn_groups(c, nRows), a.splits);
-    const auto fn = nRows <= c->nSeq ? k_pkv_attn<4, true> : k_pkv_attn<4, false>;
-    hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream(), a);
+    a.pml = (float4 *)(a.po + (size_t)a.splits * nRows * c->nHead * PKV_D);
+    if (nRows > c->nSeq) {
+        hipLaunchKernelGGL(k_pkv_attn_rows<4>, dim3((nRows / 16 + c->nSeq) * c->nHead, a.splits), dim3(256), 0, stream(), a);
+    } else {
+        const int groups = c->nSeq / group * c->nHead;
+        if (a.splits == 1 && groups < 256) hipLaunchKernelGGL(k_pkv_attn_one<8>, dim3(groups), dim3(512), 0, stream(), a);
+        else hipLaunchKernelGGL(k_pkv_attn_one<4>, dim3(groups, a.splits), dim3(256), 0, stream(), a);
+    }
     if (a.splits > 1) hipLaunchKernelGGL(k_pkv_attn_join, dim3(nRows, cdiv(c->nHead, 4)), dim3(256), 0, stream(), a);
     check_launch("k_pkv_attn");
 }

@@ -16,27 +16,35 @@ namespace g2 {
 
 constexpr int BEAM_NV = 4;                              // 16-byte pieces a thread
 constexpr int BEAM_PART = 256 * BEAM_NV;                // pieces a work-group: 8192 logits
+constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / BEAM_PART;
 struct BeamPart {
     double sum;                                         // of exp(x - m)
     float m;
-    uint32_t key[GPT2_BEAM_MAX];
+    uint32_t key[GPT2_BEAM_MAX];                        // the best, in order
 };
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
 
+// Maximum over the wave, the same scalar for all: rows of 16 lanes by DPP, then the four rows.
 __device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
+    const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16), c = __builtin_amdgcn_readlane((int)v, 32),
+                   d = __builtin_amdgcn_readlane((int)v, 48);
+    return max(max(a, b), max(c, d));
 }
 
-// NaN counts as -inf, +inf as 65504, -0 as +0.
-__device__ __forceinline__ f16 beam_logit(f16 x) {
-    const float f = (float)x + 0.f;
-    return f != f ? (f16)-INFINITY : (f16)fminf(f, 65504.f);
+// Two logits as they count: NaN as -inf, +inf as 65504, -0 as +0; and their bits in order.
+__device__ __forceinline__ f16x2 beam_logits(f16x2 x) {
+    x = x + f16x2{(f16)0.f, (f16)0.f};
+    x = __builtin_elementwise_max(x, f16x2{(f16)-INFINITY, (f16)-INFINITY});
+    return __builtin_elementwise_min(x, f16x2{(f16)65504.f, (f16)65504.f});
 }
-__device__ __forceinline__ uint32_t beam_key(f16 x, int token) {
-    const uint32_t b = __builtin_bit_cast(uint16_t, x);
-    const uint32_t o = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
-    return o << 16 | (uint32_t)(65535 - token);
+__device__ __forceinline__ uint32_t beam_order(f16x2 x) {
+    const i16x2 b = __builtin_bit_cast(i16x2, x);
+    return __builtin_bit_cast(uint32_t, b ^ ((b >> 15) | (short)0x8000));
 }
 __device__ __forceinline__ float beam_key_logit(uint32_t key) {
     const uint32_t o = key >> 16;
@@ -45,130 +53,157 @@ __device__ __forceinline__ float beam_key_logit(uint32_t key) {
 
 // One part of a row: its 16-byte pieces [part * BEAM_PART, ...), the first part also the logits before the first whole
 // piece and after the last.
+//
+// A thread's logits stay in registers as keys of their own, order << 16 | (63 - i) for its i-th; the tokens of a thread
+// ascend with i, so its largest is its best.  A wave's `beams`-th best thread is a lower bound for the part's result, and the
+// keys at or above the waves' best bound (those of 4 beams - 3 threads at most) are ranked by counting.
 __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, const uint16_t *__restrict__ logits, long ld, int V,
                                                    int beams, int parts) {
+    constexpr int N = 8 * BEAM_NV;
     __shared__ float lds_m[4];
     __shared__ double lds_s[4];
-    __shared__ uint32_t lds_k[4 * GPT2_BEAM_MAX];
+    __shared__ uint32_t lds_t[4], lds_k[(4 * GPT2_BEAM_MAX - 3) * (N + 1)];
+    __shared__ int lds_n;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, part = blockIdx.x;
     const uint16_t *x = logits + (size_t)blockIdx.y * ld;
     const int head = min(V, (int)(((16 - ((uintptr_t)x & 15)) & 15) >> 1)), pieces = (V - head) >> 3;
-    f16 v[BEAM_NV * 8 + 1];
-    uint32_t key[BEAM_NV * 8 + 1];
+    const int first = part * BEAM_PART + tid, left = V - 8 * pieces, odd = tid < head ? tid : 8 * pieces + tid;
+    if (tid == 0) lds_n = 0;
+    f16x2 v[N / 2], vodd;
+    uint32_t key[N], kodd;
 #pragma unroll
     for (int j = 0; j < BEAM_NV; ++j) {
-        const int p = part * BEAM_PART + j * 256 + tid;
-        f16x8 h = {};
-        if (p < pieces) h = *reinterpret_cast<const f16x8 *>(x + head + 8 * p);
+        i32x4 h = {(int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00};
+        if (first + 256 * j < pieces) h = *reinterpret_cast<const i32x4 *>(x + head + 8 * (first + 256 * j));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[8 * j + e] = p < pieces ? beam_logit(h[e]) : (f16)-INFINITY;
-            key[8 * j + e] = p < pieces ? beam_key(v[8 * j + e], head + 8 * p + e) : 0u;
-        }
+        for (int d = 0; d < 4; ++d) v[4 * j + d] = __builtin_bit_cast(f16x2, (int)h[d]);
     }
-    {
-        const int left = V - 8 * pieces, t = tid < head ? tid : 8 * pieces + tid;
-        const bool on = part == 0 && tid < left;
-        v[8 * BEAM_NV] = on ? beam_logit(__builtin_bit_cast(f16, x[t])) : (f16)-INFINITY;
-        key[8 * BEAM_NV] = on ? beam_key(v[8 * BEAM_NV], t) : 0u;
-    }
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i <= 8 * BEAM_NV; ++i) m = fmaxf(m, (float)v[i]);
-    m = wave_max_u(m);
-    if (lane == 0) lds_m[w] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
-    const float base = m == -INFINITY ? 0.f : m;
-    float s32 = 0.f;
-#pragma unroll
-    for (int i = 0; i <= 8 * BEAM_NV; ++i) s32 += __builtin_amdgcn_exp2f(((float)v[i] - base) * 1.4426950408889634f);
-    double sum = s32;   // at most 33 terms in fp32, the rest in fp64
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) lds_s[w] = sum;
-    // the wave's best keys
+    const bool has_odd = part == 0 && tid < left;
+    vodd = f16x2{(f16)-INFINITY, (f16)-INFINITY};
+    if (has_odd) vodd[0] = __builtin_bit_cast(f16, x[odd]);
     uint32_t best = 0;
 #pragma unroll
-    for (int i = 0; i <= 8 * BEAM_NV; ++i) best = max(best, key[i]);
-    for (int k = 0; k < beams; ++k) {
-        const uint32_t top = wave_max_key(best);
-        if (lane == 0) lds_k[w * GPT2_BEAM_MAX + k] = top;
-        if (best == top) {
-            best = 0;
+    for (int i = 0; i < N / 2; ++i) {
+        v[i] = beam_logits(v[i]);
+        const uint32_t o = first + 256 * (i / 4) < pieces ? beam_order(v[i]) : 0u;
+        key[2 * i] = o << 16 | (uint32_t)(63 - 2 * i);
+        key[2 * i + 1] = (o & 0xffff0000u) | (uint32_t)(63 - 2 * i - 1);
+        best = max(best, max(key[2 * i], key[2 * i + 1]));
+    }
+    vodd = beam_logits(vodd);
+    const int token0 = head + 8 * first;
+    auto token = [&](uint32_t k) {   // of one of the thread's own keys
+        const int i = 63 - (int)(k & 63u);
+        return token0 + 2048 * (i >> 3) + (i & 7);
+    };
+    best = best >> 16 ? (best & 0xffff0000u) | (uint32_t)(65535 - token(best)) : 0u;
+    kodd = has_odd ? beam_order(vodd) << 16 | (uint32_t)(65535 - odd) : 0u;
+    best = max(best, kodd);
+
+    // the wave's maximum, and the bound
+    uint32_t top = wave_max_key(best), bound = top, rest = best;
+    const float m = top ? beam_key_logit(top) : -INFINITY;
+    for (int k = 1; k < beams; ++k) {
+        rest = rest == bound ? 0u : rest;
+        bound = wave_max_key(rest);
+    }
+    // exp(x - m) as 2^(x l - c), l = log2 e in fp32, c = m l rounded; what the rounding takes is put back in fp64
+    constexpr float l2e = 1.4426950408889634f;
+    const float c = m == -INFINITY ? 0.f : m * l2e;
+    float s32 = 0.f;
 #pragma unroll
-            for (int i = 0; i <= 8 * BEAM_NV; ++i) best = key[i] < top ? max(best, key[i]) : best;
-        }
+    for (int i = 0; i < N / 2; ++i) {
+        s32 += __builtin_amdgcn_exp2f(fmaf((float)v[i][0], l2e, -c));
+        s32 += __builtin_amdgcn_exp2f(fmaf((float)v[i][1], l2e, -c));
+    }
+    s32 += __builtin_amdgcn_exp2f(fmaf((float)vodd[0], l2e, -c));
+    double sum = s32;   // 33 terms at most in fp32, the rest in fp64
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+        lds_t[w] = bound;
+        lds_m[w] = m;
+        lds_s[w] = m == -INFINITY ? 0.0 : sum * (1.0 + 0.6931471805599453 * ((double)c - (double)m * (double)l2e));
     }
     __syncthreads();
-    if (w == 0) {   // of the four waves': a lane's key has the rank of how many are larger
-        BeamPart *o = out + (size_t)blockIdx.y * parts + part;
-        const uint32_t mine = (lane & 15) < beams ? lds_k[lane] : 0u;
-        int rank = 0;
+    bound = max(max(lds_t[0], lds_t[1]), max(lds_t[2], lds_t[3]));
+    if (__ballot(best >= bound)) {   // wave-uniform; a bound of 0: every key is wanted
+        // the thread's keys with the bound's order count up to the bound's token
+        const int d = 65535 - (int)(bound & 0xffffu) - token0, n = d < 0 ? 0 : min(N, 8 * (d >> 11) + min((d & 2047) + 1, 8));
+        const uint32_t own = bound ? (bound & 0xffff0000u) + (uint32_t)(64 - n) : 0x10000u;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-            rank += other > mine || (other == mine && i < lane);
-        }
+        for (int i = 0; i < N; ++i)
+            if (key[i] >= own) lds_k[atomicAdd(&lds_n, 1)] = (key[i] & 0xffff0000u) | (uint32_t)(65535 - token(key[i]));
+        if (kodd && kodd >= bound) lds_k[atomicAdd(&lds_n, 1)] = kodd;
+    }
+    __syncthreads();
+    const int n = lds_n;
+    BeamPart *o = out + (size_t)blockIdx.y * parts + part;
+    if (tid < beams && tid >= n) o->key[tid] = 0u;
+    for (int i = tid; i < n; i += 256) {
+        const uint32_t mine = lds_k[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += lds_k[j] > mine;
         if (rank < beams) o->key[rank] = mine;
-        if (lane == 0) {
-            o->m = m;
-            o->sum = (lds_s[0] + lds_s[1]) + (lds_s[2] + lds_s[3]);
-        }
+    }
+    if (tid == 0) {
+        const float mx = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+        double all = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lds_m[i] != -INFINITY) all += lds_m[i] == mx ? lds_s[i] : lds_s[i] * exp((double)lds_m[i] - (double)mx);
+        o->m = mx;
+        o->sum = all;
     }
 }
 
-// A work-group per group: a wave joins a row's parts, then a thread per candidate counts those ahead of it.
-__global__ __launch_bounds__(256) void k_beam_join(int *__restrict__ token, int *__restrict__ parent, float *score_out, int *done_out,
-                                                   const BeamPart *__restrict__ part, const float *score, const int *done, int beams,
-                                                   int V, int eos, int parts) {
+// A work-group per group, a wave per row: the row's parts are joined, then a thread per candidate counts those ahead of it.
+__global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restrict__ token, int *__restrict__ parent, float *score_out, int *done_out,
+                                                                  const BeamPart *__restrict__ part, const float *score, const int *done,
+                                                                  int beams, int V, int eos, int parts) {
     __shared__ double cand[GPT2_BEAM_MAX * GPT2_BEAM_MAX];
-    __shared__ int tok[GPT2_BEAM_MAX * GPT2_BEAM_MAX];   // -1: no candidate
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int row0 = blockIdx.x * beams;
-    for (int i = tid; i < GPT2_BEAM_MAX * GPT2_BEAM_MAX; i += 256) tok[i] = -1;
-    __syncthreads();
-    for (int b = w; b < beams; b += 4) {
-        const BeamPart *p = part + (size_t)(row0 + b) * parts;
-        const double from = (double)score[row0 + b];
-        if (eos >= 0 && done[row0 + b]) {
-            if (lane == 0) {
-                tok[b * GPT2_BEAM_MAX] = eos;
-                cand[b * GPT2_BEAM_MAX] = from != from ? -INFINITY : from;
-            }
-            continue;
-        }
-        float m = -INFINITY;
-        for (int i = 0; i < parts; ++i) m = fmaxf(m, p[i].m);
-        double sum = 0.0;
-        for (int i = 0; i < parts; ++i) sum += p[i].m == -INFINITY ? 0.0 : p[i].sum * exp((double)p[i].m - (double)m);
-        const double lse = log(sum);
-        // the best of the parts' keys, a part's own in order: 16 parts at most a lane's share is 4 keys
-        const int n = parts * beams;
-        for (int k = lane; k < n; k += 64) {
-            const uint32_t mine = p[k / beams].key[k % beams];
-            if (!mine) continue;
-            int rank = 0;
-            for (int i = 0; i < n; ++i) rank += p[i / beams].key[i % beams] > mine;
-            if (rank < beams) {
-                const double s = from + ((double)beam_key_logit(mine) - (double)m) - lse;
-                tok[b * GPT2_BEAM_MAX + rank] = 65535 - (int)(mine & 0xffffu);
-                cand[b * GPT2_BEAM_MAX + rank] = s != s ? -INFINITY : s;
-            }
-        }
+    __shared__ int tok[GPT2_BEAM_MAX * GPT2_BEAM_MAX];   // beam b's at b * beams; -1: no candidate
+    const int tid = threadIdx.x, lane = tid & 63, b = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.x * beams + b;
+    const BeamPart *p = part + (size_t)row * parts;
+    const double from = (double)score[row];
+    const bool ended = eos >= 0 && done[row];
+    static_assert(BEAM_PARTS * GPT2_BEAM_MAX <= 128 && BEAM_PARTS <= 64, "two keys a lane, a part a lane");
+    const int n = parts * beams;
+    uint32_t k0 = lane < n ? p[lane / beams].key[lane % beams] : 0u, k1 = lane + 64 < n ? p[(lane + 64) / beams].key[(lane + 64) % beams] : 0u;
+    const float mp = lane < parts ? p[lane].m : -INFINITY;
+    const double sp = lane < parts ? p[lane].sum : 0.0;
+    const float m = wave_max_u(mp);
+    const double term = mp == -INFINITY ? 0.0 : mp == m ? sp : sp * exp((double)mp - (double)m);
+    double sum = 0.0;
+    for (int i = 0; i < parts; ++i) sum += __shfl(term, i, 64);
+    const double lse = log(sum);
+    uint32_t mine = 0;   // lane k: the row's k-th best
+    for (int k = 0; k < beams; ++k) {
+        const uint32_t top = wave_max_key(max(k0, k1));
+        if (lane == k) mine = top;
+        k0 = k0 == top ? 0u : k0;
+        k1 = k1 == top ? 0u : k1;
+    }
+    if (lane < beams) {
+        double s = ended ? from : from + ((double)beam_key_logit(mine) - (double)m) - lse;
+        if (s != s) s = -INFINITY;
+        cand[b * beams + lane] = s;
+        tok[b * beams + lane] = ended ? (lane == 0 ? eos : -1) : mine ? 65535 - (int)(mine & 0xffffu) : -1;
     }
     __syncthreads();
-    const int b = tid / GPT2_BEAM_MAX;
-    if (tok[tid] < 0) return;
-    const double mine = cand[tid];
+    const int all = beams * beams;
+    if (tid >= all || tok[tid] < 0) return;
+    const double s = cand[tid];
     int rank = 0;
-    for (int i = 0; i < beams * GPT2_BEAM_MAX; ++i)
-        if (tok[i] >= 0) rank += cand[i] > mine || (cand[i] == mine && i < tid);
+    for (int i = 0; i < all; ++i)
+        if (tok[i] >= 0) rank += cand[i] > s || (cand[i] == s && i < tid);
     if (rank < beams) {
-        token[row0 + rank] = tok[tid];
-        parent[row0 + rank] = row0 + b;
-        score_out[row0 + rank] = (float)mine;
-        done_out[row0 + rank] = eos >= 0 && tok[tid] == eos;
+        const int at = blockIdx.x * beams + rank;
+        token[at] = tok[tid];
+        parent[at] = blockIdx.x * beams + tid / beams;
+        score_out[at] = (float)s;
+        done_out[at] = eos >= 0 && tok[tid] == eos;
     }
 }
 
@@ -201,7 +236,7 @@ extern "C" void gpt2_beam_select(int *token, int *parent, float *score_out, int 
     const int parts = beam_parts(V);
     BeamPart *part = (BeamPart *)ws;
     hipLaunchKernelGGL(k_beam_part, dim3(parts, groups * beams), dim3(256), 0, stream(), part, logits, ld, V, beams, parts);
-    hipLaunchKernelGGL(k_beam_join, dim3(groups), dim3(256), 0, stream(), token, parent, score_out, done_out, part, score, done,
+    hipLaunchKernelGGL(k_beam_join, dim3(groups), dim3(64 * beams), 0, stream(), token, parent, score_out, done_out, part, score, done,
                        beams, V, eos, parts);
     check_launch("k_beam_select");
 }

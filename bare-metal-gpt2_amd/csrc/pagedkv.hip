@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "attn_prefill.h"   // tr_read
 #include "pagedkv.h"
 
 namespace g2 {
@@ -29,6 +30,9 @@ __host__ __device__ __forceinline__ PkvPlan pkv_plan(const GPT2PagedKV &c) {
     p.word = p.mover + c.nPages;
     return p;
 }
+
+// A wave's own LDS accesses happen in order; this keeps the compiler from reordering them.
+__device__ __forceinline__ void pkv_lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // Exclusive sum over a work-group of 64 NW threads; `total` for all.  Ends with a barrier, so `lds` can be used again.
 template <int NW>
@@ -166,10 +170,90 @@ __global__ __launch_bounds__(256) void k_pkv_embed(uint16_t *__restrict__ x, con
 }
 
 // ------------------------------------------------------------------ append
+// A tile on its way: 16 pairs of a lane.  By rows, pair 4 i + j is dims 8 (lane & 7) + 2 j, + 1 of token 8 i + lane / 8; by
+// dims, tokens 8 i + 2 j, + 1 of dim `lane` (both in the order of the tile that they go to).
+constexpr int PKV_ROW = 160;   // bytes of a token's row in LDS: neither its writes nor the transposing reads meet a bank conflict
+
 // What the cache can hold of a value: codes stand for finite numbers only.
-__device__ __forceinline__ f16 pkv_finite(f16 v) {
-    const float f = (float)v;
-    return f != f ? (f16)0.f : (f16)fminf(fmaxf(f, -65504.f), 65504.f);
+__device__ __forceinline__ uint16_t pkv_finite(uint16_t v) {
+    const float f = h2f(v);
+    return f != f ? (uint16_t)0 : f2h(fminf(fmaxf(f, -65504.f), 65504.f));
+}
+__device__ __forceinline__ bool pkv_is_finite(const uint32_t (&d)[16]) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, d[i] & 0x7fff7fffu));
+    return max((int)m[0], (int)m[1]) < 0x7c00;
+}
+__device__ __forceinline__ void pkv_make_finite(uint32_t (&d)[16]) {
+    if (__ballot(!pkv_is_finite(d)))   // hardly ever
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = pkv_finite((uint16_t)d[i]) | (uint32_t)pkv_finite((uint16_t)(d[i] >> 16)) << 16;
+}
+
+// By rows: the page's tokens that are new rows (`src`: the row of position `start`), zeros elsewhere.
+__device__ __forceinline__ void pkv_load_rows(const uint16_t *__restrict__ src, size_t ld, int pos0, const PkvSeq &q, uint32_t (&d)[16]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pos = pos0 + 8 * i + (lane >> 3);
+        i32x4 v = {0, 0, 0, 0};
+        if (pos >= q.start && pos < q.len) v = *reinterpret_cast<const i32x4 *>(src + (size_t)(pos - q.start) * ld + 8 * (lane & 7));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[4 * i + j] = (uint32_t)v[j];
+    }
+}
+
+// Rows to dims, through the wave's own LDS and the transposing reads (lane 16 G + j: dim 16 G + j of four tokens each).
+__device__ __forceinline__ void pkv_by_dims(uint32_t (&d)[16], char *lds) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<i32x4 *>(lds + (8 * i + (lane >> 3)) * PKV_ROW + 16 * (lane & 7)) = i32x4{(int)d[4 * i], (int)d[4 * i + 1], (int)d[4 * i + 2], (int)d[4 * i + 3]};
+    pkv_lds_order();
+    const char *col = lds + ((lane & 15) >> 2) * PKV_ROW + 2 * (16 * (lane >> 4) + 4 * (lane & 3));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint2 v = __builtin_bit_cast(uint2, tr_read(col + 4 * i * PKV_ROW));
+        d[2 * i] = v.x;
+        d[2 * i + 1] = v.y;
+    }
+    pkv_lds_order();
+}
+
+// Codes of a whole tile and its scale: q = rint(fl(x / s)), |x / s| <= 127 (1 + 2^-24).  x / s is y = x (1 / s) to within
+// 2^-16; only where that lies that near to the middle between two whole numbers (a tile in some twenty has such a value)
+// are the quotients formed.  y + 1.5 2^23 is the nearest whole number in its low byte.
+__device__ __forceinline__ float pkv_quantize(const uint32_t (&d)[16], uint32_t (&out)[8]) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, d[i] & 0x7fff7fffu));
+    const float peak = wave_max_u(fmaxf(h2f(m[0]), h2f(m[1])));
+    const float s = peak == 0.f ? 1.0f : peak / 127.0f, inv = 1.0f / s;
+    constexpr float magic = 12582912.f;
+    float far = 0.f;
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float x = h2f((uint16_t)(d[i / 2] >> (16 * (i & 1))));
+        const float y = fmaf(x, inv, magic);
+        w[i] = __float_as_uint(y);
+        far = fmaxf(far, fabsf(fmaf(x, inv, magic - y)));
+    }
+    if (__ballot(far > 0.5f - 1.f / 32768)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float x = h2f((uint16_t)(d[i / 2] >> (16 * (i & 1))));
+            w[i] = (uint32_t)(int)fminf(fmaxf(rintf(x / s), -127.f), 127.f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        out[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[4 * i + 3], w[4 * i + 2], 0x0c0c0400u),
+                                       __builtin_amdgcn_perm(w[4 * i + 1], w[4 * i], 0x0c0c0400u), 0x05040100u);
+    return s;
 }
 
 // A sequence's units: the pages that its new rows complete, one at least.  Unit 0 also writes the open page, whose rows
@@ -178,68 +262,65 @@ __device__ __forceinline__ int pkv_append_units(const PkvSeq &q) {
     return q.n ? max(1, q.len / PKV_P - q.start / PKV_P) : 0;
 }
 
-// One wave per unit, K|V and head.  Lane l holds dims 8 (l & 7) .. + 7 of tokens 8 i + l / 8 (i < 4), 16-byte loads of
-// whole row pieces; the block's maximum is the wave's.  A V tile's order (8 tokens of a dim together) is reached through
-// a tile of bytes in LDS.
+// One wave per unit, K|V and head: whole row pieces in, 16 bytes a lane, the tile's maximum over the wave, 8 bytes of codes a
+// lane and store, 512 contiguous.
 __device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, const uint16_t *__restrict__ qkv, const PkvSeq &q,
-                                                int seq, int u, int kv, int h, uint8_t *lds) {
-    const int lane = threadIdx.x & 63, t = lane >> 3, d0 = (lane & 7) * 8;
+                                                int seq, int u, int kv, int h, char *lds) {
+    const int lane = threadIdx.x & 63;
     const int E = c.nHead * PKV_D;
     const int had = q.start / PKV_P, full = q.len / PKV_P;
     const uint16_t *src = qkv + (size_t)q.row0 * 3 * E + (1 + kv) * E + h * PKV_D;   // row of position start
     uint16_t *open = c.open + pkv_tile(c, c.nSeq, L, q.slot, kv, h) * PKV_TILE;
+    uint32_t d[16];
     if (had + u < full) {
-        const int page = c.table[(size_t)seq * c.maxPages + had + u];
-        f16 x[4][8];
-        float peak = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int tok = 8 * i + t, pos = (had + u) * PKV_P + tok;
-            if (pos >= q.start) {
-                const f16x8 v = *reinterpret_cast<const f16x8 *>(src + (size_t)(pos - q.start) * 3 * E + d0);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = pkv_finite(v[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[i][e] = __builtin_bit_cast(f16, open[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) peak = fmaxf(peak, fabsf((float)x[i][e]));
-        }
-        peak = wave_max_u(peak);
-        const float scale = peak == 0.f ? 1.0f : peak / 127.0f;
-        if (pkv_page_ok(c, page)) {
-            const size_t at = pkv_tile(c, c.nPages, L, page, kv, h);
-            int8_t *tile = c.codes + at * PKV_TILE;
-            if (lane == 0) c.scales[at] = scale;
+        const int page = c.table[(size_t)seq * c.maxPages + had + u], kept = u ? 0 : q.start % PKV_P;
+        pkv_load_rows(src, 3 * (size_t)E, (had + u) * PKV_P, q, d);
+        if (kv) pkv_by_dims(d, lds);
+        if (kept) {   // the open page's tokens from before the call
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint32_t w[2] = {0, 0};
+                const i32x4 v = *reinterpret_cast<const i32x4 *>(open + 8 * (64 * i + lane));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float r = fminf(fmaxf(rintf((float)x[i][e] / scale), -127.f), 127.f);
-                    const uint32_t b = (uint32_t)(int)r & 255u;
-                    if (kv) lds[pkv_v_at(8 * i + t, d0 + e)] = (uint8_t)b;
-                    else w[e >> 2] |= b << (8 * (e & 3));
+                for (int j = 0; j < 4; ++j) {
+                    const int n = kv ? kept - (8 * i + 2 * j) : kept > 8 * i + (lane >> 3) ? 2 : 0;   // of the pair, how many
+                    const uint32_t keep = n >= 2 ? ~0u : n == 1 ? 0xffffu : 0u;
+                    d[4 * i + j] = ((uint32_t)v[j] & keep) | (d[4 * i + j] & ~keep);
                 }
-                if (!kv) *reinterpret_cast<uint2 *>(tile + pkv_k_at(8 * i + t, d0)) = uint2{w[0], w[1]};
             }
-            if (kv) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile is this wave's own
+        }
+        pkv_make_finite(d);
+        uint32_t w[8];
+        const float scale = pkv_quantize(d, w);
+        if (pkv_page_ok(c, page)) {
+            const size_t at = pkv_tile(c, c.nPages, L, page, kv, h);
+            if (lane == 0) c.scales[at] = scale;
+            uint2 *tile = reinterpret_cast<uint2 *>(c.codes + at * PKV_TILE);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    *reinterpret_cast<i32x4 *>(tile + 1024 * i + 16 * lane) = *reinterpret_cast<const i32x4 *>(lds + 1024 * i + 16 * lane);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            }
+            for (int i = 0; i < 4; ++i) tile[64 * i + lane] = uint2{w[2 * i], w[2 * i + 1]};
         }
     }
-    if (u == 0) {
-        for (int pos = max(q.start, full * PKV_P); pos < q.len; ++pos) {
+    const int first = max(q.start, full * PKV_P);
+    if (u || first >= q.len) return;
+    if (q.len - first <= 2) {
+        for (int pos = first; pos < q.len; ++pos) {
             const int tok = pos % PKV_P;
-            const f16 v = pkv_finite(__builtin_bit_cast(f16, src[(size_t)(pos - q.start) * 3 * E + lane]));
-            open[kv ? pkv_v_at(tok, lane) : pkv_k_at(tok, lane)] = __builtin_bit_cast(uint16_t, v);
+            open[kv ? pkv_v_at(tok, lane) : pkv_k_at(tok, lane)] = pkv_finite(src[(size_t)(pos - q.start) * 3 * E + lane]);
         }
+        return;
+    }
+    pkv_load_rows(src, 3 * (size_t)E, full * PKV_P, q, d);
+    pkv_make_finite(d);
+    const int t0 = first % PKV_P, t1 = q.len % PKV_P;   // tokens [t0, t1) are written, no others
+    if (kv) pkv_by_dims(d, lds);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int tok = 8 * i + (lane >> 3);
+        if (kv ? t0 <= 8 * i && 8 * i + 8 <= t1 : t0 <= tok && tok < t1)
+            *reinterpret_cast<i32x4 *>(open + 8 * (64 * i + lane)) = i32x4{(int)d[4 * i], (int)d[4 * i + 1], (int)d[4 * i + 2], (int)d[4 * i + 3]};
+        else if (kv)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (t0 <= 8 * i + e && 8 * i + e < t1) open[8 * (64 * i + lane) + e] = (uint16_t)(d[4 * i + e / 2] >> (16 * (e & 1)));
     }
 }
 
@@ -248,7 +329,7 @@ __device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, con
 template <bool BY_SEQ>
 __global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const uint16_t *__restrict__ qkv,
                                                     const int *__restrict__ rows, int nRows) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4][PKV_TILE];
+    __shared__ __attribute__((aligned(16))) char lds[4][PKV_P * PKV_ROW];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.y * 4 + w;
     if (kh >= 2 * c.nHead) return;   // wave-uniform; no barrier follows
@@ -266,32 +347,74 @@ __global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const 
 }
 
 // ------------------------------------------------------------------ read
+// A unit is a page that the rows of a sequence touch; a wave takes one K|V and head of it: the tile in its own order,
+// 8 values a lane and piece, V through LDS to rows, 16-byte stores.
+struct PkvRead {
+    long pos;        // of the sequence's first row
+    int row0, n;
+};
+__device__ __forceinline__ PkvRead pkv_read_rows(const int *__restrict__ rows, const int *__restrict__ pos, int nRows, int s) {
+    PkvRead r;
+    r.pos = pos[s];
+    r.row0 = rows[s];
+    r.n = rows[s + 1] - r.row0;
+    if (r.row0 < 0 || r.n < 0 || r.n > nRows || r.row0 > nRows - r.n) r.n = 0;
+    return r;
+}
 __global__ __launch_bounds__(256) void k_pkv_read(uint16_t *__restrict__ out, GPT2PagedKV c, int L, const int *__restrict__ rows,
-                                                  const int *__restrict__ pos0, int nRows) {
-    const int row = blockIdx.x;
-    const int s = pkv_seq_of_row(rows, c.nSeq, row);
+                                                  const int *__restrict__ pos, int nRows) {
+    __shared__ __attribute__((aligned(16))) uint16_t lds[4][PKV_P][PKV_D];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane >> 3, d0 = (lane & 7) * 8;
+    const int kh = blockIdx.y * 4 + w;
+    if (kh >= 2 * c.nHead) return;   // wave-uniform; no barrier follows
+    int u = blockIdx.x;
+    const int s = pkv_seq_of_unit(u, c.nSeq, [&](int s) {
+        const PkvRead r = pkv_read_rows(rows, pos, nRows, s);
+        return r.n ? (int)(((r.pos + r.n - 1) >> 5) - (r.pos >> 5)) + 1 : 0;
+    });
     if (s < 0) return;
-    const int len = min(c.len[s], c.maxPages * PKV_P), slot = c.slot[s];
-    const long pos = (long)pos0[s] + (row - rows[s]);
-    const bool there = pos >= 0 && pos < len;
-    const int p = there ? (int)(pos / PKV_P) : 0, tok = there ? (int)(pos % PKV_P) : 0;
-    const bool opened = p >= len / PKV_P;
-    const int page = there && !opened ? c.table[(size_t)s * c.maxPages + p] : -1;
-    for (int i = threadIdx.x; i < 2 * c.nHead * (PKV_D / 8); i += 256) {
-        const int d0 = (i & 7) * 8, kh = i >> 3, kv = kh >= c.nHead, h = kh - kv * c.nHead;
-        f16x8 v = {};
-        if (there && opened && (unsigned)slot < (unsigned)c.nSeq) {
-            const uint16_t *t = c.open + pkv_tile(c, c.nSeq, L, slot, kv, h) * PKV_TILE;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(f16, t[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)]);
-        } else if (pkv_page_ok(c, page)) {
+    const PkvRead r = pkv_read_rows(rows, pos, nRows, s);
+    const long p = (r.pos >> 5) + u;   // the page's number; its first row is that of position 32 p
+    const int kv = kh >= c.nHead, h = kh - kv * c.nHead, len = (int)min((long)c.len[s], (long)c.maxPages * PKV_P), slot = c.slot[s];
+    f16x8 v[4] = {};
+    if (p >= 0 && p < len / PKV_P) {
+        const int page = c.table[(size_t)s * c.maxPages + p];
+        if (pkv_page_ok(c, page)) {
             const size_t at = pkv_tile(c, c.nPages, L, page, kv, h);
-            const int8_t *t = c.codes + at * PKV_TILE;
             const float scale = c.scales[at];
+            const uint2 *tile = reinterpret_cast<const uint2 *>(c.codes + at * PKV_TILE);
+            uint2 q[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (f16)((float)t[kv ? pkv_v_at(tok, d0 + e) : pkv_k_at(tok, d0 + e)] * scale);
+            for (int i = 0; i < 4; ++i) q[i] = tile[64 * i + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f16x8 x = i8x8_to_f16x8(q[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = (f16)((float)x[e] * scale);
+            }
         }
-        *reinterpret_cast<f16x8 *>(out + (size_t)row * 2 * c.nHead * PKV_D + (size_t)kh * PKV_D + d0) = v;
+    } else if (p >= 0 && p * PKV_P < len && (unsigned)slot < (unsigned)c.nSeq) {
+        const uint16_t *tile = c.open + pkv_tile(c, c.nSeq, L, slot, kv, h) * PKV_TILE;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f16x8 *>(tile + 8 * (64 * i + lane));
+    }
+    if (kv) {   // lane: 8 tokens of its dim; rows from the wave's own LDS
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const f16 x = v[i][e];   // a copy: a bit cast of the element itself takes the vector's first
+                lds[w][8 * i + e][lane] = __builtin_bit_cast(uint16_t, x);
+            }
+        pkv_lds_order();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f16x8 *>(&lds[w][8 * i + t][d0]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long at = p * PKV_P + 8 * i + t, j = at - r.pos;
+        if (j >= 0 && j < r.n)
+            *reinterpret_cast<f16x8 *>(out + (size_t)(r.row0 + j) * 2 * c.nHead * PKV_D + (size_t)kh * PKV_D + d0) = at < len ? v[i] : f16x8{};
     }
 }
 
@@ -359,7 +482,9 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
     }
 }
 
-// Second launch: blockIdx.y 0 the books, y > 0 layer y - 1's open page of sequence blockIdx.x, only the tokens in it.
+// Second launch: blockIdx.y 0 the books, then the open page of sequence blockIdx.x, a layer's K or V each, only the tokens in
+// it.  A thread copies piece `tid` (16 bytes) of every head's tile, four heads under way; of a V tile's octet that the tokens end
+// in, it puts those that are there among what was.
 __global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__restrict__ parent) {
     const int me = blockIdx.x, tid = threadIdx.x;
     const PkvPlan plan = pkv_plan(c);
@@ -380,26 +505,25 @@ __global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__re
     }
     const int from = plan.from[me], to = plan.slot[me], used = len % PKV_P;
     if (used <= 0 || (unsigned)from >= (unsigned)c.nSeq || (unsigned)to >= (unsigned)c.nSeq) return;
-    const int L = blockIdx.y - 1, H = c.nHead;
-    const uint16_t *src = c.open + pkv_tile(c, c.nSeq, L, from, 0, 0) * PKV_TILE;
-    uint16_t *dst = c.open + pkv_tile(c, c.nSeq, L, to, 0, 0) * PKV_TILE;
-    const int kc = used * PKV_D / 8, vc = (used >> 3) * PKV_D;   // 16-byte pieces of a K tile, of a V tile's whole octets
-    for (int i = tid; i < H * kc; i += 256) {
-        const size_t at = (size_t)(i / kc) * PKV_TILE + 8 * (i % kc);
-        *reinterpret_cast<i32x4 *>(dst + at) = *reinterpret_cast<const i32x4 *>(src + at);
+    const int L = (blockIdx.y - 1) >> 1, kv = (blockIdx.y - 1) & 1;
+    const int n = kv ? used - 8 * (tid >> 6) : 8 * (used > tid >> 3);   // the piece's values that are there
+    if (n <= 0) return;
+    i32x4 keep = {-1, -1, -1, -1};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
+    const i32x4 *src = reinterpret_cast<const i32x4 *>(c.open + pkv_tile(c, c.nSeq, L, from, kv, 0) * PKV_TILE) + tid;
+    i32x4 *dst = reinterpret_cast<i32x4 *>(c.open + pkv_tile(c, c.nSeq, L, to, kv, 0) * PKV_TILE) + tid;
+    for (int h = 0; h < c.nHead; h += 4) {
+        i32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = src[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)];
+        if (n < 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (v[i] & keep) | (dst[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)] & ~keep);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (h + i < c.nHead) dst[(size_t)(h + i) * (PKV_TILE / 8)] = v[i];
     }
-    src += (size_t)H * PKV_TILE;
-    dst += (size_t)H * PKV_TILE;
-    for (int i = tid; i < H * vc; i += 256) {
-        const size_t at = (size_t)(i / vc) * PKV_TILE + 8 * (i % vc);
-        *reinterpret_cast<i32x4 *>(dst + at) = *reinterpret_cast<const i32x4 *>(src + at);
-    }
-    if (used & 7)
-        for (int i = tid; i < H * PKV_D; i += 256)
-            for (int t = used & ~7; t < used; ++t) {
-                const size_t at = (size_t)(i / PKV_D) * PKV_TILE + pkv_v_at(t, i % PKV_D);
-                dst[at] = src[at];
-            }
 }
 
 // ------------------------------------------------------------------ compact
@@ -482,7 +606,7 @@ bool pkv_refused(const GPT2PagedKV *c, const char *what) {
     for (const void *q : p)
         if (!q || ((uintptr_t)q & 3)) return arg_fail(what);
     if (!c->codes || !c->open || !aligned16(c->codes) || !aligned16(c->open)) return arg_fail(what);
-    if (c->headDim != PKV_D || c->nLayer < 1 || c->nLayer > 65000 || c->nHead < 1 || c->nHead > 4096 || c->nPages < 1 || c->nPages > (1 << 26) ||
+    if (c->headDim != PKV_D || c->nLayer < 1 || c->nLayer > 32000 || c->nHead < 1 || c->nHead > 4096 || c->nPages < 1 || c->nPages > (1 << 26) ||
         c->nSeq < 1 || c->nSeq > GPT2_PKV_MAX_SEQ || c->maxPages < 1 || c->maxPages > (1 << 25) ||
         (long)c->nSeq * c->maxPages > (1L << 30))
         return arg_fail(what);
@@ -504,7 +628,7 @@ static size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 extern "C" int gpt2_pkv_alloc(GPT2PagedKV *c, int nLayer, int nHead, int nPages, int nSeq, int maxLen) {
     if (!c) return arg_fail("gpt2_pkv_alloc: null cache"), 1;
     memset(c, 0, sizeof(*c));
-    if (nLayer < 1 || nLayer > 65000 || nHead < 1 || nHead > 4096 || nPages < 1 || nPages > (1 << 26) || nSeq < 1 || nSeq > GPT2_PKV_MAX_SEQ || maxLen < 1 ||
+    if (nLayer < 1 || nLayer > 32000 || nHead < 1 || nHead > 4096 || nPages < 1 || nPages > (1 << 26) || nSeq < 1 || nSeq > GPT2_PKV_MAX_SEQ || maxLen < 1 ||
         maxLen > (1 << 30) || (long)nSeq * cdiv(maxLen, PKV_P) > (1L << 30))
         return arg_fail("gpt2_pkv_alloc: sizes out of range"), 1;
     const size_t maxPages = cdiv(maxLen, PKV_P), tiles = (size_t)nLayer * nPages * 2 * nHead, opens = (size_t)nLayer * nSeq * 2 * nHead;
@@ -589,7 +713,7 @@ extern "C" void gpt2_pkv_read(gpt2_half *kv, const GPT2PagedKV *c, int L, const 
     if (pkv_refused_batch(c, L, rows, nRows, "gpt2_pkv_read: bad cache, layer or rows")) return;
     if (nRows == 0) return;
     if (!kv || !aligned16(kv) || !pos || ((uintptr_t)pos & 3)) { arg_fail("gpt2_pkv_read: null/unaligned"); return; }
-    hipLaunchKernelGGL(k_pkv_read, dim3(nRows), dim3(256), 0, stream(), kv, *c, L, rows, pos, nRows);
+    hipLaunchKernelGGL(k_pkv_read, dim3(nRows / PKV_P + 2 * c->nSeq, cdiv(2 * c->nHead, 4)), dim3(256), 0, stream(), kv, *c, L, rows, pos, nRows);
     check_launch("k_pkv_read");
 }
 
@@ -597,7 +721,7 @@ extern "C" void gpt2_pkv_fork(GPT2PagedKV *c, const int *parent) {
     if (pkv_refused(c, "gpt2_pkv_fork: bad cache")) return;
     if (!parent || ((uintptr_t)parent & 3)) { arg_fail("gpt2_pkv_fork: null/unaligned"); return; }
     hipLaunchKernelGGL(k_pkv_fork_plan, dim3(c->nSeq + 1), dim3(256), 0, stream(), *c, parent);
-    hipLaunchKernelGGL(k_pkv_fork, dim3(c->nSeq, 1 + c->nLayer), dim3(256), 0, stream(), *c, parent);
+    hipLaunchKernelGGL(k_pkv_fork, dim3(c->nSeq, 1 + 2 * c->nLayer), dim3(256), 0, stream(), *c, parent);
     check_launch("k_pkv_fork");
 }
 
