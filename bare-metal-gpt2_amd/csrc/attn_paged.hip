@@ -34,11 +34,17 @@ struct PageRaw {
 };
 
 // Attention of 16 rows as it accumulates: column jq is a row; o[2 i + b] element r is dim 32 i + 8 g + 2 r + b.
-// m: the running maximum of x; l: the sum of the weights; o: the weighted sum of the values in units of 2^lv.
+// m: the running maximum of x; l: the sum of the weights (in every element); o: the weighted sum of the values.
 struct AttnAcc {
-    float m, l, lv;
-    f32x4 o[4];
+    float m;
+    f32x4 l, o[4];
 };
+__device__ __forceinline__ void attn_clear(AttnAcc &A) {
+    A.m = -INFINITY;
+    A.l = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < 4; ++d) A.o[d] = A.l;
+}
 
 // A page (K tile, V tile) on its way to a 4 KB stage in LDS: four instructions of 1 KB, whole rows.  The 16-byte pieces of a
 // K row are swizzled by the row (by choosing what each lane fetches), so that the reads below meet no bank conflict.
@@ -63,82 +69,102 @@ __device__ __forceinline__ void page_take(const char *__restrict__ stage, PageRa
     for (int i = 0; i < 2; ++i) R.v[i] = *reinterpret_cast<const i32x4 *>(stage + PKV_TILE + (g * PKV_D + 32 * i + 2 * jq) * 8);
 }
 
-// 32 tokens from `key0` on against the columns: fragments of K (kf[t]: dims 16 g .. + 7 and + 8 .. + 15 of the lane's key
-// of tile t) and of V (vf[2 i + b]: tokens 8 g .. + 7 of dim 32 i + 2 jq + b); column jq sees keys below `lim`.
-__device__ __forceinline__ void attn_page(AttnAcc &A, const f16x8 (&kf)[2][2], const f16x8 (&vf)[4], const f16x8 (&q)[2], float sk,
-                                          float sv, int key0, int lim, bool masked) {
+// A page as the products take it: fragments of K (k[t]: dims 16 g .. + 7 and + 8 .. + 15 of the lane's key of tile t) and of V
+// (v[2 i + b]: tokens 8 g .. + 7 of dim 32 i + 2 jq + b), its scales and first token; column jq sees keys below `lim`, which
+// `masked` says matters (the same in every lane).
+struct PageFrag {
+    f16x8 k[2][2], v[4];
+    float sk, sv;
+    int key0, lim;
+    bool masked;
+};
+
+// Maximum of three as the hardware has it (fmaxf of products would first make each operand canonical).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// N pages against the columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it where few
+// waves share a SIMD, and two pages go down it in little more than the time of one.
+template <int N>
+__device__ __forceinline__ void attn_pages(AttnAcc &A, const PageFrag (&P)[N], const f16x8 (&q)[2]) {
     const int g = (threadIdx.x & 63) >> 4;
-    float s[8];
-    const float scale = sk * (0.125f * 1.4426950408889634f);
+    float s[N][8], scale[N], mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][0], q[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][1], q[1], y, 0, 0, 0);
+    for (int n = 0; n < N; ++n) {
+        scale[n] = P[n].sk * (0.125f * 1.4426950408889634f);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * t + r] = y[r];
+        for (int t = 0; t < 2; ++t) {
+            f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][0], q[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][1], q[1], y, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][4 * t + r] = y[r];
+        }
     }
-    if (masked) {
-        const int n = lim - key0 - 8 * g;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = e < n ? s[e] : -INFINITY;
+    for (int n = 0; n < N; ++n) {
+        if (P[n].masked) {
+            const int left = P[n].lim - P[n].key0 - 8 * g;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[n][e] = e < left ? s[n][e] : -INFINITY;
+        }
+        const float m = max3(max3(max3(s[n][0], s[n][1], s[n][2]), s[n][3], s[n][4]), max3(s[n][5], s[n][6], s[n][7]), -INFINITY);
+        mx = fmaxf(mx, m * scale[n]);
     }
-    float mx = s[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
-    const float mn = fmaxf(A.m, group_max(mx) * scale);
+    const float mn = fmaxf(A.m, group_max(mx));
     const float base = mn == -INFINITY ? 0.f : mn;   // a column that sees none of these keys
-    // The maximum moves rarely after the first pages; s_v is a factor of the weights (as an addend of their exponent), so
-    // that P.V adds to o as it is: relative to 2^lv, which follows s_v where that is far from it (fp16 weights).
-    if (__ballot(mn > A.m)) {
+    if (__ballot(mn > A.m)) {   // the maximum moves rarely after the first pages
         const float corr = __builtin_amdgcn_exp2f(A.m - base);
         A.m = mn;
         A.l *= corr;
 #pragma unroll
         for (int i = 0; i < 4; ++i) A.o[i] *= corr;
     }
-    const float lsv = __builtin_amdgcn_logf(sv);
-    if (fabsf(lsv - A.lv) > 4.f) {   // the same in every lane
-        const float f = __builtin_amdgcn_exp2f(A.lv - lsv);
-        A.lv = lsv;
+    // The weights are rounded to fp16, which costs an output about as much as its own rounding (1.2e-4 of it against
+    // 2.1e-4; with s_v in them, so that P.V could add to o in the product, 2e-4: the largest weight is then no longer 1 exactly,
+    // and it was no faster).
+    f16x8 p[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) A.o[i] *= f;
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[n][e], scale[n], -base));
     }
-    const float add = lsv - A.lv - base;
-    f16x8 p;
+    // their sum, of the fp16 values as they are multiplied, on the matrix units too: a row of ones
+    const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[e], scale, add));
-    // the weights' sum is that of the fp16 values that the matrix units multiply
-    float ps = 0.f;
+    for (int n = 0; n < N; ++n) A.l = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, p[n], A.l, 0, 0, 0);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) ps = __builtin_amdgcn_fdot2(f16x2{p[e], p[e + 1]}, f16x2{1, 1}, ps, false);
-    A.l = fmaf(ps, __builtin_amdgcn_exp2f(A.lv - lsv), A.l);
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A.o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], p, A.o[i], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].v[i], p[n], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) A.o[i][r] = fmaf(y[r], P[n].sv, A.o[i][r]);
+        }
 }
 
-__device__ __forceinline__ void attn_codes(AttnAcc &A, const PageRaw &R, const f16x8 (&q)[2], float sk, float sv, int key0, int lim,
-                                           bool masked) {
-    f16x8 kf[2][2], vf[4];
+__device__ __forceinline__ void page_widen(const PageRaw &R, PageFrag &P) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        kf[t][0] = i8x8_to_f16x8(uint2{(uint32_t)R.k[t][0], (uint32_t)R.k[t][1]});
-        kf[t][1] = i8x8_to_f16x8(uint2{(uint32_t)R.k[t][2], (uint32_t)R.k[t][3]});
-        vf[2 * t] = i8x8_to_f16x8(uint2{(uint32_t)R.v[t][0], (uint32_t)R.v[t][1]});
-        vf[2 * t + 1] = i8x8_to_f16x8(uint2{(uint32_t)R.v[t][2], (uint32_t)R.v[t][3]});
+        P.k[t][0] = i8x8_to_f16x8(uint2{(uint32_t)R.k[t][0], (uint32_t)R.k[t][1]});
+        P.k[t][1] = i8x8_to_f16x8(uint2{(uint32_t)R.k[t][2], (uint32_t)R.k[t][3]});
+        P.v[2 * t] = i8x8_to_f16x8(uint2{(uint32_t)R.v[t][0], (uint32_t)R.v[t][1]});
+        P.v[2 * t + 1] = i8x8_to_f16x8(uint2{(uint32_t)R.v[t][2], (uint32_t)R.v[t][3]});
     }
-    attn_page(A, kf, vf, q, sk, sv, key0, lim, masked);
 }
 
 // The open page: fp16 in the same order; tokens at or past `used` are whatever was there, so their values are cleared.
 __device__ __forceinline__ void attn_open(AttnAcc &A, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, int used,
                                           const f16x8 (&q)[2], int key0, int lim) {
     const int lane = threadIdx.x & 63, jq = lane & 15, g = lane >> 4;
-    f16x8 kf[2][2], vf[4];
+    PageFrag P[1];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const uint16_t *row = k + (8 * (jq >> 2) + 4 * t + (jq & 3)) * PKV_D + 16 * g;
-        kf[t][0] = *reinterpret_cast<const f16x8 *>(row);
-        kf[t][1] = *reinterpret_cast<const f16x8 *>(row + 8);
+        P[0].k[t][0] = *reinterpret_cast<const f16x8 *>(row);
+        P[0].k[t][1] = *reinterpret_cast<const f16x8 *>(row + 8);
     }
     const int n = used - 8 * g;   // of the lane's 8 tokens, those that are there
     i32x4 keep;
@@ -146,8 +172,12 @@ __device__ __forceinline__ void attn_open(AttnAcc &A, const uint16_t *__restrict
     for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        vf[i] = __builtin_bit_cast(f16x8, *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8) & keep);
-    attn_page(A, kf, vf, q, 1.f, 1.f, key0, lim, true);
+        P[0].v[i] = __builtin_bit_cast(f16x8, *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8) & keep);
+    P[0].sk = P[0].sv = 1.f;
+    P[0].key0 = key0;
+    P[0].lim = lim;
+    P[0].masked = true;
+    attn_pages<1>(A, P, q);
 }
 
 // What a pass goes over, as steps of a page each: the first `shared` pages of sequence seq0, for every column, then the
@@ -159,7 +189,7 @@ struct AttnSteps {
 
 // One pass: 16 columns (column jq: row `row` of the activations, -1 for none, which sees the keys below `lim`; every
 // column sees those below `first`), one head, split z of the steps.  The W waves take steps in turn and join in LDS.
-constexpr int ATTN_STAGES = 2;
+constexpr int ATTN_STAGES = 4;
 template <int W>
 struct AttnLds {
     char ring[W][ATTN_STAGES * 2 * PKV_TILE];
@@ -179,10 +209,7 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
         q[1] = *reinterpret_cast<const f16x8 *>(qrow + 8);
     }
     AttnAcc A;
-    A.m = -INFINITY;
-    A.l = A.lv = 0.f;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) A.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    attn_clear(A);
 
     const size_t vstep = (size_t)c.nHead * PKV_TILE;   // from a page's K tile to its V tile
     for (int t0 = z * W + w; t0 < st.total; t0 += 64 * stride) {
@@ -225,19 +252,39 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
         for (int s = 0; s < ATTN_STAGES; ++s)
             if (todo) issue(s);
         asm volatile("" : "+v"(sk), "+v"(sv));   // waited for here, once, and not with every page under way in the loop
-        while (left) {
+        auto take = [&](int at, PageFrag &P) {   // from a stage, which is filled again
             const int j = __builtin_ctzll(left);
             left &= left - 1;
-            --ahead;
-            wait_tiles<4, ATTN_STAGES - 1>(ahead);
-            asm volatile("" ::: "memory");
             PageRaw R;
-            page_take(ring + 2 * PKV_TILE * stage, R);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the stage is filled again
+            page_take(ring + 2 * PKV_TILE * at, R);
+            page_widen(R, P);
+            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1;
+            P.sk = lane_f(sk, j);
+            P.sv = lane_f(sv, j);
+            P.key0 = (x >> 5) * PKV_P;
+            P.lim = bj < 0 || bj == jq ? lim : 0;
+            P.masked = bj >= 0 || P.key0 + PKV_P > first;
+        };
+        while (left & (left - 1)) {
+            ahead -= 2;
+            wait_tiles<4, ATTN_STAGES - 2>(ahead);
+            asm volatile("" ::: "memory");
+            PageFrag P[2];
+            take(stage, P[0]);
+            take(stage + 1, P[1]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the stages are filled again
             if (todo) issue(stage);
-            stage = stage + 1 == ATTN_STAGES ? 0 : stage + 1;
-            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1, key0 = (x >> 5) * PKV_P;
-            attn_codes(A, R, q, lane_f(sk, j), lane_f(sv, j), key0, bj < 0 || bj == jq ? lim : 0, bj >= 0 || key0 + PKV_P > first);
+            if (todo) issue(stage + 1);
+            stage = (stage + 2) % ATTN_STAGES;
+            attn_pages<2>(A, P, q);
+        }
+        if (left) {
+            wait_vm<0>();
+            asm volatile("" ::: "memory");
+            PageFrag P[1];
+            take(stage, P[0]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            attn_pages<1>(A, P, q);
         }
         for (uint64_t o = opened; o; o &= o - 1) {
             const int j = __builtin_ctzll(o);
@@ -248,17 +295,17 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
         }
     }
     // the waves' sums to one maximum, then together
-    A.l = group_sum(A.l);
-    if (g == 0) lds.m[w][jq] = A.l != 0.f ? A.m : -INFINITY;
+    const float l = A.l[0];
+    if (g == 0) lds.m[w][jq] = l != 0.f ? A.m : -INFINITY;
     __syncthreads();
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < W; ++u) mx = fmaxf(mx, lds.m[u][jq]);
-    const float f = A.l != 0.f ? __builtin_amdgcn_exp2f(A.m - mx) : 0.f;
+    const float f = l != 0.f ? __builtin_amdgcn_exp2f(A.m - mx) : 0.f;
     if (row >= 0) {
-        if (g == 0) lds.l[w][jq] = A.l * f;
+        if (g == 0) lds.l[w][jq] = l * f;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) reinterpret_cast<f32x4 *>(lds.ring[w])[64 * d + lane] = A.o[d] * (f * __builtin_amdgcn_exp2f(A.lv));   // the ring is idle
+        for (int d = 0; d < 4; ++d) reinterpret_cast<f32x4 *>(lds.ring[w])[64 * d + lane] = A.o[d] * f;   // the ring is idle
     }
     __syncthreads();
     if (w < 2 && row >= 0) {   // dims 32 w + 8 g .. + 7 of the column's row
@@ -386,6 +433,148 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_rows(PagedAttn a) {
     attn_pass<W>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
 }
 
+// Many rows a sequence: a work-group per 64 of them and head, a wave per 16, every wave over all pages.  The four waves share
+// the work of turning a page into fragments: a wave takes a quarter (a K tile's half, or 16 of V's 32 pairs of dims) from memory to
+// registers, 16 bytes a lane, ATTN_AHEAD pairs of pages ahead, to fp16, and to LDS in the order in which all four read it.  16 rows a
+// work-group would read each page from L2 four times as often, which bounds that form (61 us for 8 prompts of up to 600 rows over
+// up to 2000 tokens).
+constexpr int ATTN_AHEAD = 2;   // pairs of pages
+__global__ __launch_bounds__(256) void k_pkv_attn_block(PagedAttn a) {
+    __shared__ __attribute__((aligned(1024))) f16x8 lds[2][2][8][64];   // two pages at a time: K (2 t + half), then V (4 + 2 i + b)
+    const GPT2PagedKV &c = a.c;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
+    const int h = blockIdx.x % c.nHead, E = c.nHead * PKV_D;
+    int rb = blockIdx.x / c.nHead;
+    const int seq = pkv_seq_of_unit(rb, c.nSeq, [&](int s) { return (pkv_seq(c, a.rows, a.nRows, s).n + 63) / 64; });
+    if (seq < 0) return;
+    const PkvSeq s = pkv_seq(c, a.rows, a.nRows, seq);
+    rb = (s.n + 63) / 64 - 1 - rb;   // the longest first
+    const int i0 = 64 * rb + 16 * w, i = i0 + jq, full = s.len / PKV_P;
+    const int last = s.start + min(s.n, 64 * rb + 64), pages = (last + PKV_P - 1) / PKV_P;   // of the work-group's rows
+    const int first = s.start + i0 + 1, lim = i < s.n ? s.start + i + 1 : 0;                 // keys that the wave's rows, and row i, see
+    const int end = i0 < s.n ? s.start + min(s.n, i0 + 16) : 0;                               // ... and any of the wave's
+    const uint16_t *qrow = a.qkv + (size_t)(s.row0 + min(i, s.n - 1)) * 3 * E + h * PKV_D + 16 * g;
+    const f16x8 q[2] = {*reinterpret_cast<const f16x8 *>(qrow), *reinterpret_cast<const f16x8 *>(qrow + 8)};
+    AttnAcc A;
+    attn_clear(A);
+
+    // The wave's quarter of a page: where its 16 bytes a lane lie in the tile, and the fragments' slots that they fill.  K: wave
+    // t takes keys 8 x + 4 t + y, lane 16 x + 4 y + z dims 16 z .. + 15 of one, for lane 16 z + 4 x + y of the product.
+    const int from = w < 2 ? (8 * (lane >> 4) + 4 * w + ((lane >> 2) & 3)) * PKV_D + 16 * (lane & 3) : (g * PKV_D + 32 * (w - 2) + 2 * jq) * 8;
+    // (swizzled: 16 lanes that write, or read, together meet no bank conflict)
+    auto swizzle = [](int l) { return l ^ (l >> 4) << 2; };
+    const int slot = swizzle(w < 2 ? 16 * (lane & 3) + 4 * (lane >> 4) + ((lane >> 2) & 3) : lane), mine = swizzle(lane);
+    const int8_t *const quarter = c.codes + pkv_tile(c, c.nPages, a.L, 0, w >> 1, h) * PKV_TILE + from;
+    uint32_t off_lo = 0, off_hi = 0;   // of the lane's page in the layer, in bytes
+    int page = -1;
+    float sk = 0.f, sv = 0.f;
+    auto fetch = [&](int base) {   // numbers and scales of the 64 pages from `base` on, a lane each
+        const int p = base + lane;
+        page = p < min(pages, full) ? c.table[(size_t)seq * c.maxPages + p] : -1;
+        if (!pkv_page_ok(c, page)) page = -1;
+        const size_t off = (size_t)max(page, 0) * 2 * c.nHead * PKV_TILE;   // pages that are none read page 0, and are skipped below
+        off_lo = (uint32_t)off;
+        off_hi = (uint32_t)(off >> 32);
+        sk = sv = 0.f;
+        if (page >= 0) {
+            const size_t at = pkv_tile(c, c.nPages, a.L, page, 0, h);
+            sk = c.scales[at];
+            sv = c.scales[at + c.nHead];
+        }
+    };
+    auto part = [&](int p) {
+        const uint32_t lo = __builtin_amdgcn_readlane((int)off_lo, p), hi = __builtin_amdgcn_readlane((int)off_hi, p);
+        return *reinterpret_cast<const i32x4 *>(quarter + ((size_t)hi << 32 | lo));
+    };
+    auto put = [&](const i32x4 v, int buf, int n) {
+        lds[buf][n][2 * w][slot] = i8x8_to_f16x8(uint2{(uint32_t)v[0], (uint32_t)v[1]});
+        lds[buf][n][2 * w + 1][slot] = i8x8_to_f16x8(uint2{(uint32_t)v[2], (uint32_t)v[3]});
+    };
+    auto get = [&](int buf, int n, int p, float k, float v, PageFrag &P) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            P.k[t][0] = lds[buf][n][2 * t][mine];
+            P.k[t][1] = lds[buf][n][2 * t + 1][mine];
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) P.v[d] = lds[buf][n][4 + d][mine];
+        P.sk = k;
+        P.sv = v;
+        P.key0 = p * PKV_P;
+        P.lim = lim;
+        P.masked = P.key0 + PKV_P > first;
+    };
+    const int whole = min(pages, full);
+    for (int base = 0; base < whole; base += 64) {
+        fetch(base);
+        const int n = min(64, whole - base);
+        // pairs of pages; one that is none, or past the last, takes part with no key to see (and a scale that is a number)
+        i32x4 raw[ATTN_AHEAD][2];
+#pragma unroll
+        for (int j = 0; j < ATTN_AHEAD; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) raw[j][k] = part(min(2 * j + k, n - 1));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) put(raw[0][k], 0, k);
+        lds_barrier();
+        for (int p0 = 0; p0 < n; p0 += 2 * ATTN_AHEAD) {
+#pragma unroll
+            for (int j = 0; j < ATTN_AHEAD; ++j) {
+                const int p = p0 + 2 * j;
+                if (p < n) {   // the same for all waves
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) raw[j][k] = part(min(p + 2 * ATTN_AHEAD + k, n - 1));
+                    if (p + 2 < n)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) put(raw[(j + 1) % ATTN_AHEAD][k], (j + 1) & 1, k);
+                    if ((base + p) * PKV_P < end) {
+                        PageFrag P[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int pk = p + k, at = min(pk, 63);
+                            get(j & 1, k, base + pk, lane_f(sk, at), lane_f(sv, at), P[k]);
+                            if (pk >= n || __builtin_amdgcn_readlane(page, at) < 0) {
+                                P[k].sk = P[k].sv = 1.f;
+                                P[k].lim = 0;
+                                P[k].masked = true;
+                            }
+                        }
+                        attn_pages<2>(A, P, q);
+                    }
+                    lds_barrier();
+                }
+            }
+        }
+    }
+    if (pages > full) {   // the open page: fp16 as it lies, tokens that are not there cleared
+        const uint16_t *tile = c.open + pkv_tile(c, c.nSeq, a.L, s.slot, w >> 1, h) * PKV_TILE + from;
+        const i32x4 x = *reinterpret_cast<const i32x4 *>(tile), y = *reinterpret_cast<const i32x4 *>(tile + 8);
+        const int n = w < 2 ? 8 : s.len - full * PKV_P - 8 * g;
+        i32x4 keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
+        lds[0][0][2 * w][slot] = __builtin_bit_cast(f16x8, x & keep);
+        lds[0][0][2 * w + 1][slot] = __builtin_bit_cast(f16x8, y & keep);
+        lds_barrier();
+        if (full * PKV_P < end) {
+            PageFrag P[1];
+            get(0, 0, full, 1.f, 1.f, P[0]);
+            attn_pages<1>(A, P, q);
+        }
+    }
+    const float inv = A.l[0] != 0.f ? 1.f / A.l[0] : 0.f;
+    if (i < s.n) {
+        uint16_t *out = a.att + (size_t)(s.row0 + i) * E + h * PKV_D + 8 * g;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            f16x8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = (f16)(A.o[2 * d + (e & 1)][e >> 1] * inv);
+            *reinterpret_cast<f16x8 *>(out + 32 * d) = o;
+        }
+    }
+}
+
 // Joins the splits: a wave per row and head; lane z holds split z's maximum and weight, then lane d dim d.
 __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
     const int lane = threadIdx.x & 63, h = blockIdx.y * 4 + (threadIdx.x >> 6), row = blockIdx.x;
@@ -417,7 +606,9 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
 struct AttnSplit {
     int splits, per;
 };
+static bool attn_by_block(const GPT2PagedKV *c, int nRows) { return nRows / 32 >= c->nSeq && (long)(nRows / 64) * c->nHead >= 128; }
 static AttnSplit attn_split(const GPT2PagedKV *c, int nRows) {
+    if (attn_by_block(c, nRows)) return {1, 64};
     if (c->maxPages <= 64 || (nRows > c->nSeq && (long)(nRows / 16) * c->nHead >= 512)) return {1, 64};
     const long groups = (long)(nRows > c->nSeq ? nRows / 16 + 1 : c->nSeq) * c->nHead;
     const int per = groups * (c->maxPages / 64) >= 512 ? 64 : 16, n = cdiv(c->maxPages, per);
@@ -454,7 +645,9 @@ extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2Pa
     a.per = sp.per;
     a.po = (float *)ws;
     a.pml = (float4 *)(a.po + (size_t)a.splits * nRows * c->nHead * PKV_D);
-    if (nRows > c->nSeq) {
+    if (attn_by_block(c, nRows)) {
+        hipLaunchKernelGGL(k_pkv_attn_block, dim3((nRows / 64 + c->nSeq) * c->nHead), dim3(256), 0, stream(), a);
+    } else if (nRows > c->nSeq) {
         hipLaunchKernelGGL(k_pkv_attn_rows<4>, dim3((nRows / 16 + c->nSeq) * c->nHead, a.splits), dim3(256), 0, stream(), a);
     } else {
         const int groups = c->nSeq / group * c->nHead;

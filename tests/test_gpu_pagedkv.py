@@ -179,6 +179,48 @@ def test_attention_many_sequences(pkg, L):
     p.check_attention(0, x[0])
 
 
+@pytest.mark.parametrize("heads,before,counts", [
+    (12, [40, 500, 7], [300, 401, 64]),
+    (12, [0, 0, 0], [704, 0, 33]),
+    (16, [31, 32], [1, 640]),
+    (12, [2100], [770]),
+])
+def test_attention_blocks(pkg, L, heads, before, counts):
+    """Batches of enough rows for work-groups of 64: prompts from nothing, prompts on top of cached ones, ragged."""
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=100, seqs=len(counts), max_len=3000), np.random.default_rng(20)
+    p.step(rng, before)
+    x = p.step(rng, counts)
+    p.same()
+    p.check_attention(0, x[0], extra=3)
+    r = p.r   # a page that is none
+    r.table[0, 0] = r.pages
+    r.upload(pkg, p.c)
+    p.check_attention(0, x[0])
+
+
+@pytest.mark.parametrize("max_len", [320, 4000])
+@pytest.mark.parametrize("group", [2, 3, 8, 16])
+def test_attention_beams(pkg, L, group, max_len):
+    """Beams that share a prompt's pages: the same as without the hint, to the order of sums; with beams that have no row, that
+    share nothing, that have several rows."""
+    seqs = 2 * group
+    p, rng = Pair(pkg, L, layers=1, heads=2, pages=40 * group, seqs=seqs, max_len=max_len), np.random.default_rng(group)
+    r = p.r
+    p.step(rng, [200 if s == 0 else 65 if s == group else 0 for s in range(seqs)])
+    p.fork([s // group * group for s in range(seqs)])
+    some = np.ones(seqs, int)
+    for counts in (some, some * 30, some, np.arange(seqs) % 2, np.where(np.arange(seqs) == 1, 1, 0), some):
+        x = p.step(rng, counts)
+        p.check_attention(0, x[0], group=group)
+        plain, hinted = p.attend(0, x[0]), p.attend(0, x[0], group=group)
+        assert np.abs(plain.astype(np.float32) - hinted).max(initial=0) <= 2 * p.r.attend(0, x[0], p.rows)[1].max(initial=0)
+    p.fork(np.concatenate([rng.integers(0, group, group), group + rng.integers(0, group, group)]))
+    r.table[0, 1] = -1   # differs from the others' from its second page on, and is none
+    r.upload(pkg, p.c)
+    x = p.step(rng, some)
+    p.check_attention(0, x[0], group=group)
+
+
 def test_stale_and_foreign_values_do_not_reach_a_row(pkg, L):
     """NaN in unused tokens of the open pages, in free pages' scales, and in other sequences' query rows."""
     rng = np.random.default_rng(12)
