@@ -79,19 +79,17 @@ struct PageFrag {
     bool masked;
 };
 
-// Maximum of three as the hardware has it (fmaxf of products would first make each operand canonical).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// Maximum of products, as the median with infinity: fmaxf would first make each of them canonical, an instruction more.  The
+// compiler does not see what `inf` is, or it would make a maximum of it.
+__device__ __forceinline__ float max_by(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
 // N pages against the columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it where few
 // waves share a SIMD, and two pages go down it in little more than the time of one.
 template <int N>
 __device__ __forceinline__ void attn_pages(AttnAcc &A, const PageFrag (&P)[N], const f16x8 (&q)[2]) {
     const int g = (threadIdx.x & 63) >> 4;
-    float s[N][8], scale[N], mx = -INFINITY;
+    float s[N][8], scale[N], mx = -INFINITY, inf = INFINITY;
+    asm("" : "+s"(inf));
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         scale[n] = P[n].sk * (0.125f * 1.4426950408889634f);
@@ -110,7 +108,8 @@ __device__ __forceinline__ void attn_pages(AttnAcc &A, const PageFrag (&P)[N], c
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[n][e] = e < left ? s[n][e] : -INFINITY;
         }
-        const float m = max3(max3(max3(s[n][0], s[n][1], s[n][2]), s[n][3], s[n][4]), max3(s[n][5], s[n][6], s[n][7]), -INFINITY);
+        const float m = max_by(max_by(max_by(s[n][0], s[n][1], inf), max_by(s[n][2], s[n][3], inf), inf),
+                               max_by(max_by(s[n][4], s[n][5], inf), max_by(s[n][6], s[n][7], inf), inf), inf);
         mx = fmaxf(mx, m * scale[n]);
     }
     const float mn = fmaxf(A.m, group_max(mx));
@@ -156,15 +155,13 @@ __device__ __forceinline__ void page_widen(const PageRaw &R, PageFrag &P) {
 }
 
 // The open page: fp16 in the same order; tokens at or past `used` are whatever was there, so their values are cleared.
-__device__ __forceinline__ void attn_open(AttnAcc &A, const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, int used,
-                                          const f16x8 (&q)[2], int key0, int lim) {
+__device__ __forceinline__ void open_take(const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, int used, PageFrag &P) {
     const int lane = threadIdx.x & 63, jq = lane & 15, g = lane >> 4;
-    PageFrag P[1];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const uint16_t *row = k + (8 * (jq >> 2) + 4 * t + (jq & 3)) * PKV_D + 16 * g;
-        P[0].k[t][0] = *reinterpret_cast<const f16x8 *>(row);
-        P[0].k[t][1] = *reinterpret_cast<const f16x8 *>(row + 8);
+        P.k[t][0] = *reinterpret_cast<const f16x8 *>(row);
+        P.k[t][1] = *reinterpret_cast<const f16x8 *>(row + 8);
     }
     const int n = used - 8 * g;   // of the lane's 8 tokens, those that are there
     i32x4 keep;
@@ -172,12 +169,8 @@ __device__ __forceinline__ void attn_open(AttnAcc &A, const uint16_t *__restrict
     for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        P[0].v[i] = __builtin_bit_cast(f16x8, *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8) & keep);
-    P[0].sk = P[0].sv = 1.f;
-    P[0].key0 = key0;
-    P[0].lim = lim;
-    P[0].masked = true;
-    attn_pages<1>(A, P, q);
+        P.v[i] = __builtin_bit_cast(f16x8, *reinterpret_cast<const i32x4 *>(v + (g * PKV_D + 32 * (i >> 1) + 2 * jq + (i & 1)) * 8) & keep);
+    P.sk = P.sv = 1.f;
 }
 
 // What a pass goes over, as steps of a page each: the first `shared` pages of sequence seq0, for every column, then the
@@ -189,13 +182,16 @@ struct AttnSteps {
 
 // One pass: 16 columns (column jq: row `row` of the activations, -1 for none, which sees the keys below `lim`; every
 // column sees those below `first`), one head, split z of the steps.  The W waves take steps in turn and join in LDS.
-constexpr int ATTN_STAGES = 4;
+// One loop, two steps at a time, and little code around it: the instructions of a short call come from L2 (the call with one
+// token took 4.4 us with 8.5 KB of code and 5.4 with 11.6).
+template <int W>
+constexpr int ATTN_STAGES = W > 4 ? 4 : 2;   // of 4 KB
 template <int W>
 struct AttnLds {
-    char ring[W][ATTN_STAGES * 2 * PKV_TILE];
+    char ring[W][ATTN_STAGES<W> * 2 * PKV_TILE];
     float m[W][16], l[W][16];
 };
-template <int W>
+template <int W, bool BEAMS>
 __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &st, int h, int z, int row, int lim, int first, AttnLds<W> &lds) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
@@ -212,11 +208,12 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
     attn_clear(A);
 
     const size_t vstep = (size_t)c.nHead * PKV_TILE;   // from a page's K tile to its V tile
+    const int8_t *const layer = c.codes + pkv_tile(c, c.nPages, a.L, 0, 0, h) * PKV_TILE;
     for (int t0 = z * W + w; t0 < st.total; t0 += 64 * stride) {
         // the wave's next 64 steps, a lane each: the page's number in its sequence, whose it is, the pool's page, scales
         const int t = t0 + stride * lane;
         int b = -1, p = t, seq = st.seq0, len = st.len0;
-        if (st.beams) {   // wave-uniform
+        if constexpr (BEAMS) {
             const int u = t - st.shared;
             for (int k = 0; k < st.beams; ++k)
                 if (u >= __builtin_amdgcn_readlane(st.off, k)) b = k;
@@ -230,7 +227,7 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
         const int full = len / PKV_P;
         int page = t < st.total && p < full ? c.table[(size_t)seq * c.maxPages + p] : -1;
         const bool there = pkv_page_ok(c, page);
-        const uint64_t opened = __ballot(t < st.total && p == full);
+        uint64_t opened = __ballot(t < st.total && p == full);
         float sk = 0.f, sv = 0.f;
         if (there) {
             const size_t at = pkv_tile(c, c.nPages, a.L, page, 0, h);
@@ -238,60 +235,56 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
             sv = c.scales[at + c.nHead];
         }
         const int who = p << 5 | (b + 1);   // p < 2^25 (maxPages)
-        // complete pages through the wave's own ring of stages: all but one ahead of the one in use
+        const size_t off = (size_t)max(page, 0) * 2 * c.nHead * PKV_TILE;   // of the page in the layer, in bytes
+        // complete pages through the wave's own ring of stages
         uint64_t left = __ballot(there), todo = left;
         int stage = 0, ahead = 0;   // pages under way
         char *const ring = lds.ring[w];
         auto issue = [&](int s) {
-            const int8_t *k = c.codes + pkv_tile(c, c.nPages, a.L, __builtin_amdgcn_readlane(page, __builtin_ctzll(todo)), 0, h) * PKV_TILE;
+            const int j = __builtin_ctzll(todo);
+            const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)off, j), hi = __builtin_amdgcn_readlane((int)(uint32_t)(off >> 32), j);
+            const int8_t *k = layer + ((size_t)hi << 32 | lo);
             page_issue(k, k + vstep, ring + 2 * PKV_TILE * s);
             todo &= todo - 1;
             ++ahead;
         };
-#pragma unroll
-        for (int s = 0; s < ATTN_STAGES; ++s)
-            if (todo) issue(s);
+#pragma nounroll
+        for (int s = 0; s < ATTN_STAGES<W> && todo; ++s) issue(s);
         asm volatile("" : "+v"(sk), "+v"(sv));   // waited for here, once, and not with every page under way in the loop
-        auto take = [&](int at, PageFrag &P) {   // from a stage, which is filled again
-            const int j = __builtin_ctzll(left);
-            left &= left - 1;
-            PageRaw R;
-            page_take(ring + 2 * PKV_TILE * at, R);
-            page_widen(R, P);
-            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1;
-            P.sk = lane_f(sk, j);
-            P.sv = lane_f(sv, j);
-            P.key0 = (x >> 5) * PKV_P;
-            P.lim = bj < 0 || bj == jq ? lim : 0;
-            P.masked = bj >= 0 || P.key0 + PKV_P > first;
-        };
-        while (left & (left - 1)) {
-            ahead -= 2;
-            wait_tiles<4, ATTN_STAGES - 2>(ahead);
+        // Two steps at a time: two complete pages, or one and an open one, or an open one; a place without a step takes
+        // part with whatever the stage holds (codes are finite) and no column sees it.
+        while (left | opened) {
+            ahead = max(ahead - 2, 0);
+            wait_tiles<4, ATTN_STAGES<W> - 2>(ahead);
             asm volatile("" ::: "memory");
             PageFrag P[2];
-            take(stage, P[0]);
-            take(stage + 1, P[1]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const bool open = n == 1 && !left && opened, none = !open && !left;
+                const int j = open ? __builtin_ctzll(opened) : none ? 0 : __builtin_ctzll(left);
+                const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1;
+                P[n].key0 = (x >> 5) * PKV_P;
+                P[n].lim = none || (BEAMS && bj >= 0 && bj != jq) ? 0 : lim;
+                P[n].masked = none || open || (BEAMS && bj >= 0) || P[n].key0 + PKV_P > first;
+                if (open) {
+                    const int slot = BEAMS && bj >= 0 ? __builtin_amdgcn_readlane(st.slot, max(bj, 0)) : st.slot0;
+                    const uint16_t *k = c.open + pkv_tile(c, c.nSeq, a.L, slot, 0, h) * PKV_TILE;
+                    open_take(k, k + vstep, __builtin_amdgcn_readlane(len, j) - P[n].key0, P[n]);
+                    opened &= opened - 1;
+                } else {
+                    PageRaw R;
+                    page_take(ring + 2 * PKV_TILE * (stage + n), R);
+                    page_widen(R, P[n]);
+                    P[n].sk = none ? 1.f : lane_f(sk, j);
+                    P[n].sv = none ? 1.f : lane_f(sv, j);
+                    left &= left - 1;
+                }
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the stages are filled again
             if (todo) issue(stage);
             if (todo) issue(stage + 1);
-            stage = (stage + 2) % ATTN_STAGES;
+            stage = (stage + 2) % ATTN_STAGES<W>;
             attn_pages<2>(A, P, q);
-        }
-        if (left) {
-            wait_vm<0>();
-            asm volatile("" ::: "memory");
-            PageFrag P[1];
-            take(stage, P[0]);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            attn_pages<1>(A, P, q);
-        }
-        for (uint64_t o = opened; o; o &= o - 1) {
-            const int j = __builtin_ctzll(o);
-            const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1, key0 = (x >> 5) * PKV_P;
-            const int slot = bj < 0 ? st.slot0 : __builtin_amdgcn_readlane(st.slot, max(bj, 0));
-            const uint16_t *k = c.open + pkv_tile(c, c.nSeq, a.L, slot, 0, h) * PKV_TILE;
-            attn_open(A, k, k + vstep, __builtin_amdgcn_readlane(len, j) - key0, q, key0, bj < 0 || bj == jq ? lim : 0);
         }
     }
     // the waves' sums to one maximum, then together
@@ -357,11 +350,11 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
     for (; shared < least; shared += 64) {
         const int p = shared + lane;
         bool same = p < least;
-        if (same) {
-            const int page = c.table[(size_t)(seq0 + one) * c.maxPages + p];
-            for (int b = one + 1; b < a.group; ++b)
-                if (on >> b & 1) same &= c.table[(size_t)(seq0 + b) * c.maxPages + p] == page;
-        }
+        int page[16];   // all loads under way before the first comparison
+#pragma unroll
+        for (int b = 0; b < 16; ++b) page[b] = c.table[(size_t)(seq0 + (on >> b & 1 ? b : one)) * c.maxPages + min(p, c.maxPages - 1)];
+#pragma unroll
+        for (int b = 1; b < 16; ++b) same &= page[b] == page[0];
         const uint64_t differ = __ballot(!same);
         if (differ) {
             shared += __builtin_ctzll(differ);
@@ -381,9 +374,24 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
     return {seq0 + one, __builtin_amdgcn_readlane(s.len, one), 0, shared, total, a.group, seq0 + min(lane, a.group - 1), s.len, s.slot, sum - own};
 }
 
-// One row a sequence, nearly always (no more rows than sequences): a work-group per group of beams, head and split.
+// One row a sequence, nearly always (no more rows than sequences): a work-group per sequence, head and split ...
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
+    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+    const int h = blockIdx.x % a.c.nHead, seq = blockIdx.x / a.c.nHead;
+    const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
+#pragma nounroll
+    for (int rb = 0; 16 * rb < s.n; ++rb) {
+        if (rb) __syncthreads();
+        AttnCols col;
+        const AttnSteps st = attn_rows(s, seq, rb, col);
+        attn_pass<W, false>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+    }
+}
+
+// ... or per group of beams, together where they have a row each at most and there are two.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
     const int h = blockIdx.x % a.c.nHead, lane = threadIdx.x & 63;
     const int seq0 = blockIdx.x / a.c.nHead * a.group;
@@ -407,8 +415,9 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
             u.n = __builtin_amdgcn_readlane(s.n, b);
             u.slot = __builtin_amdgcn_readlane(s.slot, b);
             st = attn_rows(u, seq0 + b, rb, col);
+            st.off = 0x7fffffff;   // no step is a beam's own
         }
-        attn_pass<W>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+        attn_pass<W, true>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
         if (together) break;
         if (16 * ++rb >= u.n) {
             const uint64_t more = on & ~((2ull << b) - 1);   // b < 16
@@ -430,7 +439,7 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_rows(PagedAttn a) {
     if (seq < 0) return;
     AttnCols col;
     const AttnSteps st = attn_rows(pkv_seq(a.c, a.rows, a.nRows, seq), seq, rb, col);
-    attn_pass<W>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+    attn_pass<W, false>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
 }
 
 // Many rows a sequence: a work-group per 64 of them and head, a wave per 16, every wave over all pages.  The four waves share
@@ -439,7 +448,7 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_rows(PagedAttn a) {
 // work-group would read each page from L2 four times as often, which bounds that form (61 us for 8 prompts of up to 600 rows over
 // up to 2000 tokens).
 constexpr int ATTN_AHEAD = 2;   // pairs of pages
-__global__ __launch_bounds__(256) void k_pkv_attn_block(PagedAttn a) {
+__global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) f16x8 lds[2][2][8][64];   // two pages at a time: K (2 t + half), then V (4 + 2 i + b)
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
@@ -575,28 +584,36 @@ __global__ __launch_bounds__(256) void k_pkv_attn_block(PagedAttn a) {
     }
 }
 
-// Joins the splits: a wave per row and head; lane z holds split z's maximum and weight, then lane d dim d.
+// Joins the splits: a wave per row and head; lane z holds split z's maximum and weight, then lane d dim d.  BY_SEQ: blockIdx.x
+// is a sequence, with a row nearly always; else a row, whose sequence is looked up (a few dependent loads more).
+template <bool BY_SEQ>
 __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y * 4 + (threadIdx.x >> 6), row = blockIdx.x;
-    if (h >= a.c.nHead) return;
-    const int seq = pkv_seq_of_row(a.rows, a.c.nSeq, row);
-    if (seq < 0 || pkv_seq(a.c, a.rows, a.nRows, seq).n == 0) return;
-    const size_t at = (size_t)row * a.c.nHead + h, per = (size_t)a.nRows * a.c.nHead;
-    const int splits = max(1, min(__builtin_amdgcn_readfirstlane(__float_as_int(a.pml[at].z)), a.splits));
     static_assert(ATTN_SPLITS <= 64, "a lane a split");
-    const float4 ml = a.pml[at + per * min(lane, splits - 1)];
-    const bool on = lane < splits && ml.y != 0.f;
-    const float mx = wave_max_u(on ? ml.x : -INFINITY), f = on ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
-    const float L = wave_sum_u(on ? ml.y * f : 0.f);
-    float o = 0.f;
-    for (int z = 0; z < splits; z += 8) {   // eight loads under way; f is 0 past the last split
-        float v[8];
+    const int lane = threadIdx.x & 63, h = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (h >= a.c.nHead) return;
+    const int seq = BY_SEQ ? (int)blockIdx.x : pkv_seq_of_row(a.rows, a.c.nSeq, blockIdx.x);
+    if (seq < 0) return;
+    const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
+    if (s.n == 0) return;
+    const size_t per = (size_t)a.nRows * a.c.nHead;
+    const int row0 = BY_SEQ ? s.row0 : (int)blockIdx.x;
+    for (int row = row0; row < (BY_SEQ ? s.row0 + s.n : row0 + 1); ++row) {
+        const size_t at = (size_t)row * a.c.nHead + h;
+        const int splits = max(1, min(__builtin_amdgcn_readfirstlane(__float_as_int(a.pml[at].z)), a.splits));
+        const float4 ml = a.pml[at + per * min(lane, splits - 1)];
+        const bool on = lane < splits && ml.y != 0.f;
+        const float mx = wave_max_u(on ? ml.x : -INFINITY), f = on ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
+        const float L = wave_sum_u(on ? ml.y * f : 0.f);
+        float o = 0.f;
+        for (int z = 0; z < splits; z += 8) {   // eight loads under way; f is 0 past the last split
+            float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = a.po[(at + per * min(z + i, splits - 1)) * PKV_D + lane];
+            for (int i = 0; i < 8; ++i) v[i] = a.po[(at + per * min(z + i, splits - 1)) * PKV_D + lane];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o = fmaf(v[i], lane_f(f, z + i), o);
+            for (int i = 0; i < 8; ++i) o = fmaf(v[i], lane_f(f, z + i), o);
+        }
+        a.att[at * PKV_D + lane] = f2h(L != 0.f ? o / L : 0.f);
     }
-    a.att[at * PKV_D + lane] = f2h(L != 0.f ? o / L : 0.f);
 }
 
 // How the steps are split over work-groups: at least `per` of them each, into `splits` at most.  None for caches whose
@@ -651,9 +668,14 @@ extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2Pa
         hipLaunchKernelGGL(k_pkv_attn_rows<4>, dim3((nRows / 16 + c->nSeq) * c->nHead, a.splits), dim3(256), 0, stream(), a);
     } else {
         const int groups = c->nSeq / group * c->nHead;
-        if (a.splits == 1 && groups < 256) hipLaunchKernelGGL(k_pkv_attn_one<8>, dim3(groups), dim3(512), 0, stream(), a);
-        else hipLaunchKernelGGL(k_pkv_attn_one<4>, dim3(groups, a.splits), dim3(256), 0, stream(), a);
+        const bool wide = a.splits == 1 && groups < 256;
+        const auto fn = group > 1 ? (wide ? k_pkv_attn_beams<8> : k_pkv_attn_beams<4>) : wide ? k_pkv_attn_one<8> : k_pkv_attn_one<4>;
+        hipLaunchKernelGGL(fn, dim3(groups, a.splits), dim3(wide ? 512 : 256), 0, stream(), a);
     }
-    if (a.splits > 1) hipLaunchKernelGGL(k_pkv_attn_join, dim3(nRows, cdiv(c->nHead, 4)), dim3(256), 0, stream(), a);
+    if (a.splits > 1) {
+        const bool by_seq = nRows <= c->nSeq;
+        hipLaunchKernelGGL(by_seq ? k_pkv_attn_join<true> : k_pkv_attn_join<false>, dim3(by_seq ? c->nSeq : nRows, cdiv(c->nHead, 4)), dim3(256), 0,
+                           stream(), a);
+    }
     check_launch("k_pkv_attn");
 }

@@ -8,15 +8,16 @@
 // A logit and its token are one 32-bit key, (logit's bits in order) << 16 | (65535 - token): keys of a row are unique, and
 // the larger key is the larger logit or, of equal ones, the lower token.  0 is no key.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "gpt2_pagedkv.h"
 
 namespace g2 {
 
-constexpr int BEAM_NV = 4;                              // 16-byte pieces a thread
-constexpr int BEAM_PART = 256 * BEAM_NV;                // pieces a work-group: 8192 logits
-constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / BEAM_PART;
+// 16-byte pieces a thread: a work-group takes 4096 logits of few rows, 8192 of many.
+constexpr int BEAM_FEW = 2, BEAM_MANY = 4;
+constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / (256 * BEAM_FEW);
 struct BeamPart {
     double sum;                                         // of exp(x - m)
     float m;
@@ -36,6 +37,26 @@ __device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
     return max(max(a, b), max(c, d));
 }
 
+// Sum over the wave in fp64, in a fixed order: rows of 16 lanes by DPP, then the four rows.
+__device__ __forceinline__ double wave_sum64(double v) {
+    auto add = [&](auto ctrl) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, ctrl.value, 0xF, 0xF, true);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), ctrl.value, 0xF, 0xF, true);
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    add(std::integral_constant<int, 0xB1>{});
+    add(std::integral_constant<int, 0x4E>{});
+    add(std::integral_constant<int, 0x141>{});
+    add(std::integral_constant<int, 0x140>{});
+    auto row = [&](int l) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+        return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    return (row(0) + row(16)) + (row(32) + row(48));
+}
+
 // Two logits as they count: NaN as -inf, +inf as 65504, -0 as +0; and their bits in order.
 __device__ __forceinline__ f16x2 beam_logits(f16x2 x) {
     x = x + f16x2{(f16)0.f, (f16)0.f};
@@ -51,15 +72,17 @@ __device__ __forceinline__ float beam_key_logit(uint32_t key) {
     return h2f((uint16_t)(o & 0x8000u ? o & 0x7fffu : ~o));
 }
 
-// One part of a row: its 16-byte pieces [part * BEAM_PART, ...), the first part also the logits before the first whole
+// One part of a row: its 16-byte pieces [256 NV part, ...), the first part also the logits before the first whole
 // piece and after the last.
 //
 // A thread's logits stay in registers as keys of their own, order << 16 | (63 - i) for its i-th; the tokens of a thread
 // ascend with i, so its largest is its best.  A wave's `beams`-th best thread is a lower bound for the part's result, and the
 // keys at or above the waves' best bound (those of 4 beams - 3 threads at most) are ranked by counting.
+template <int NV>
 __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, const uint16_t *__restrict__ logits, long ld, int V,
                                                    int beams, int parts) {
-    constexpr int N = 8 * BEAM_NV;
+    constexpr int N = 8 * NV;
+    static_assert(N <= 64, "a thread's keys hold its index in 6 bits");
     __shared__ float lds_m[4];
     __shared__ double lds_s[4];
     __shared__ uint32_t lds_t[4], lds_k[(4 * GPT2_BEAM_MAX - 3) * (N + 1)];
@@ -67,12 +90,12 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, part = blockIdx.x;
     const uint16_t *x = logits + (size_t)blockIdx.y * ld;
     const int head = min(V, (int)(((16 - ((uintptr_t)x & 15)) & 15) >> 1)), pieces = (V - head) >> 3;
-    const int first = part * BEAM_PART + tid, left = V - 8 * pieces, odd = tid < head ? tid : 8 * pieces + tid;
+    const int first = part * 256 * NV + tid, left = V - 8 * pieces, odd = tid < head ? tid : 8 * pieces + tid;
     if (tid == 0) lds_n = 0;
     f16x2 v[N / 2], vodd;
     uint32_t key[N], kodd;
 #pragma unroll
-    for (int j = 0; j < BEAM_NV; ++j) {
+    for (int j = 0; j < NV; ++j) {
         i32x4 h = {(int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00};
         if (first + 256 * j < pieces) h = *reinterpret_cast<const i32x4 *>(x + head + 8 * (first + 256 * j));
 #pragma unroll
@@ -81,15 +104,17 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     const bool has_odd = part == 0 && tid < left;
     vodd = f16x2{(f16)-INFINITY, (f16)-INFINITY};
     if (has_odd) vodd[0] = __builtin_bit_cast(f16, x[odd]);
-    uint32_t best = 0;
+    uint32_t best = 0, piece[NV] = {};   // the largest of a piece
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
         v[i] = beam_logits(v[i]);
         const uint32_t o = first + 256 * (i / 4) < pieces ? beam_order(v[i]) : 0u;
-        key[2 * i] = o << 16 | (uint32_t)(63 - 2 * i);
-        key[2 * i + 1] = (o & 0xffff0000u) | (uint32_t)(63 - 2 * i - 1);
-        best = max(best, max(key[2 * i], key[2 * i + 1]));
+        key[2 * i] = __builtin_amdgcn_perm(o, (uint32_t)(63 - 2 * i), 0x05040100u);       // o << 16 | ..
+        key[2 * i + 1] = __builtin_amdgcn_perm(o, (uint32_t)(62 - 2 * i), 0x07060100u);   // o's upper half | ..
+        piece[i / 4] = max(piece[i / 4], max(key[2 * i], key[2 * i + 1]));
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) best = max(best, piece[j]);
     vodd = beam_logits(vodd);
     const int token0 = head + 8 * first;
     auto token = [&](uint32_t k) {   // of one of the thread's own keys
@@ -117,9 +142,7 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
         s32 += __builtin_amdgcn_exp2f(fmaf((float)v[i][1], l2e, -c));
     }
     s32 += __builtin_amdgcn_exp2f(fmaf((float)vodd[0], l2e, -c));
-    double sum = s32;   // 33 terms at most in fp32, the rest in fp64
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    const double sum = wave_sum64((double)s32);   // 33 terms at most in fp32, the rest in fp64
     if (lane == 0) {
         lds_t[w] = bound;
         lds_m[w] = m;
@@ -132,8 +155,11 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
         const int d = 65535 - (int)(bound & 0xffffu) - token0, n = d < 0 ? 0 : min(N, 8 * (d >> 11) + min((d & 2047) + 1, 8));
         const uint32_t own = bound ? (bound & 0xffff0000u) + (uint32_t)(64 - n) : 0x10000u;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (key[i] >= own) lds_k[atomicAdd(&lds_n, 1)] = (key[i] & 0xffff0000u) | (uint32_t)(65535 - token(key[i]));
+        for (int j = 0; j < NV; ++j)
+            if (__ballot(piece[j] >= own))
+#pragma unroll
+                for (int i = 8 * j; i < 8 * j + 8; ++i)
+                    if (key[i] >= own) lds_k[atomicAdd(&lds_n, 1)] = (key[i] & 0xffff0000u) | (uint32_t)(65535 - token(key[i]));
         if (kodd && kodd >= bound) lds_k[atomicAdd(&lds_n, 1)] = kodd;
     }
     __syncthreads();
@@ -146,18 +172,20 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
         for (int j = 0; j < n; ++j) rank += lds_k[j] > mine;
         if (rank < beams) o->key[rank] = mine;
     }
-    if (tid == 0) {
-        const float mx = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
-        double all = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lds_m[i] != -INFINITY) all += lds_m[i] == mx ? lds_s[i] : lds_s[i] * exp((double)lds_m[i] - (double)mx);
-        o->m = mx;
-        o->sum = all;
+    if (w == 0) {   // lane i: wave i's sum, to the largest maximum
+        const float mi = lds_m[lane & 3], mx = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+        const double term = mi == -INFINITY ? 0.0 : mi == mx ? lds_s[lane & 3] : lds_s[lane & 3] * exp((double)mi - (double)mx);
+        const double all = (__shfl(term, 0, 64) + __shfl(term, 1, 64)) + (__shfl(term, 2, 64) + __shfl(term, 3, 64));
+        if (lane == 0) {
+            o->m = mx;
+            o->sum = all;
+        }
     }
 }
 
 // A work-group per group, a wave per row: the row's parts are joined, then a thread per candidate counts those ahead of it.
+// K: a lane's keys, four parts each.
+template <int K>
 __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restrict__ token, int *__restrict__ parent, float *score_out, int *done_out,
                                                                   const BeamPart *__restrict__ part, const float *score, const int *done,
                                                                   int beams, int V, int eos, int parts) {
@@ -168,9 +196,13 @@ __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restric
     const BeamPart *p = part + (size_t)row * parts;
     const double from = (double)score[row];
     const bool ended = eos >= 0 && done[row];
-    static_assert(BEAM_PARTS * GPT2_BEAM_MAX <= 128 && BEAM_PARTS <= 64, "two keys a lane, a part a lane");
-    const int n = parts * beams;
-    uint32_t k0 = lane < n ? p[lane / beams].key[lane % beams] : 0u, k1 = lane + 64 < n ? p[(lane + 64) / beams].key[(lane + 64) % beams] : 0u;
+    static_assert(GPT2_BEAM_MAX == 16 && BEAM_PARTS <= 16, "16 places a part, a part a lane, four keys a lane");
+    uint32_t key[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int at = 4 * i + (lane >> 4);
+        key[i] = at < parts && (lane & 15) < beams ? p[at].key[lane & 15] : 0u;
+    }
     const float mp = lane < parts ? p[lane].m : -INFINITY;
     const double sp = lane < parts ? p[lane].sum : 0.0;
     const float m = wave_max_u(mp);
@@ -180,24 +212,31 @@ __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restric
     const double lse = log(sum);
     uint32_t mine = 0;   // lane k: the row's k-th best
     for (int k = 0; k < beams; ++k) {
-        const uint32_t top = wave_max_key(max(k0, k1));
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i) best = max(best, key[i]);
+        const uint32_t top = wave_max_key(best);
         if (lane == k) mine = top;
-        k0 = k0 == top ? 0u : k0;
-        k1 = k1 == top ? 0u : k1;
+#pragma unroll
+        for (int i = 0; i < K; ++i) key[i] = key[i] == top ? 0u : key[i];
     }
     if (lane < beams) {
         double s = ended ? from : from + ((double)beam_key_logit(mine) - (double)m) - lse;
         if (s != s) s = -INFINITY;
-        cand[b * beams + lane] = s;
-        tok[b * beams + lane] = ended ? (lane == 0 ? eos : -1) : mine ? 65535 - (int)(mine & 0xffffu) : -1;
+        const bool there = ended ? lane == 0 : mine != 0;
+        cand[b * beams + lane] = there ? s : (double)NAN;   // one that is not there is ahead of none
+        tok[b * beams + lane] = !there ? -1 : ended ? eos : 65535 - (int)(mine & 0xffffu);
     }
     __syncthreads();
     const int all = beams * beams;
     if (tid >= all || tok[tid] < 0) return;
     const double s = cand[tid];
     int rank = 0;
-    for (int i = 0; i < all; ++i)
-        if (tok[i] >= 0) rank += cand[i] > s || (cand[i] == s && i < tid);
+#pragma unroll 4
+    for (int i = 0; i < all; ++i) {
+        const double c = cand[i];
+        rank += i < tid ? c >= s : c > s;
+    }
     if (rank < beams) {
         const int at = blockIdx.x * beams + rank;
         token[at] = tok[tid];
@@ -207,15 +246,18 @@ __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restric
     }
 }
 
-static int beam_parts(int V) { return V < 8 ? 1 : cdiv(V / 8, BEAM_PART); }
+// Many rows fill the card with large parts, which have less to do for each logit (64 x 8 rows of 50257: see k_beam_part);
+// few are done sooner in small ones.
+static int beam_pieces(int rows, int V) { return (long)rows * (V / 8) >= 256L * 6000 ? BEAM_MANY : BEAM_FEW; }
+static int beam_parts(int rows, int V) { return V < 8 ? 1 : cdiv(V / 8, 256 * beam_pieces(rows, V)); }
 
 }  // namespace g2
 
 using namespace g2;
 
 extern "C" size_t gpt2_beam_select_ws(int groups, int beams, int V) {
-    if (groups < 1 || beams < 1 || V < 1) return 16;
-    return (size_t)groups * beams * beam_parts(V) * sizeof(BeamPart);
+    if (groups < 1 || beams < 1 || V < 1 || (long)groups * beams > 65535) return 16;
+    return (size_t)groups * beams * beam_parts(groups * beams, V) * sizeof(BeamPart);
 }
 
 extern "C" void gpt2_beam_select(int *token, int *parent, float *score_out, int *done_out, const gpt2_half *logits, long ld,
@@ -233,10 +275,12 @@ extern "C" void gpt2_beam_select(int *token, int *parent, float *score_out, int 
         arg_fail("gpt2_beam_select: workspace too small or unaligned");
         return;
     }
-    const int parts = beam_parts(V);
+    const int rows = groups * beams, parts = beam_parts(rows, V);
     BeamPart *part = (BeamPart *)ws;
-    hipLaunchKernelGGL(k_beam_part, dim3(parts, groups * beams), dim3(256), 0, stream(), part, logits, ld, V, beams, parts);
-    hipLaunchKernelGGL(k_beam_join, dim3(groups), dim3(64 * beams), 0, stream(), token, parent, score_out, done_out, part, score, done,
+    const auto fn = beam_pieces(rows, V) == BEAM_MANY ? k_beam_part<BEAM_MANY> : k_beam_part<BEAM_FEW>;
+    hipLaunchKernelGGL(fn, dim3(parts, rows), dim3(256), 0, stream(), part, logits, ld, V, beams, parts);
+    const auto join = parts <= 4 ? k_beam_join<1> : parts <= 8 ? k_beam_join<2> : k_beam_join<4>;
+    hipLaunchKernelGGL(join, dim3(groups), dim3(64 * beams), 0, stream(), token, parent, score_out, done_out, part, score, done,
                        beams, V, eos, parts);
     check_launch("k_beam_select");
 }

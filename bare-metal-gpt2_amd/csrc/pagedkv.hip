@@ -71,55 +71,62 @@ __global__ void k_pkv_reset(GPT2PagedKV c) {
 
 // ------------------------------------------------------------------ grow
 // One work-group: needs and their sums over the sequences, then a walk over refs that hands the lowest free pages out in
-// order, which stops when enough are found.  Table entries past the complete pages mean nothing, so they are written as
-// pages are found; refs and lengths follow once all are.
-__global__ __launch_bounds__(1024) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
-    __shared__ int off[GPT2_PKV_MAX_SEQ], lds[16];
-    constexpr int PER = GPT2_PKV_MAX_SEQ / 1024;
-    const int tid = threadIdx.x;
+// order, which stops when enough are found (its first step is under way meanwhile).  Table entries past the complete pages mean
+// nothing, so they are written as pages are found; refs and lengths follow once all are.  Bound by the latency of its few dependent
+// loads and barriers: T = 256 threads where they are enough (48 sequences, one of them needing a page: see DESIGN.md's table).
+template <int T>
+__global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
+    constexpr int NW = T / 64, PER = GPT2_PKV_MAX_SEQ / 1024, FREE = 8;
+    __shared__ int off[PER * T], lds[2][NW + 2], flags[NW];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const PkvPlan plan = pkv_plan(c);
-    int len[PER], need[PER], sum = 0;
+    int ref[FREE];
+    auto load_refs = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < FREE; ++j) ref[j] = base + FREE * tid + j < c.nPages ? c.refs[base + FREE * tid + j] : 1;
+    };
+    load_refs(0);
+    int len[PER], add[PER], need[PER], sum = 0;
     bool bad_arg = false, bad_len = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int s = tid * PER + j;
-        len[j] = need[j] = 0;
+        len[j] = add[j] = need[j] = 0;
         if (s < c.nSeq) {
             const int a = rows[s], b = rows[s + 1];
             len[j] = c.len[s];
+            add[j] = b - a;
             bad_arg |= a < 0 || b < a || b > nRows || len[j] < 0;
-            const long after = (long)len[j] + (b - a);
+            const long after = (long)len[j] + add[j];
             bad_len |= after > (long)c.maxPages * PKV_P;
-            need[j] = (bad_arg || bad_len) ? 0 : (int)(after / PKV_P) - len[j] / PKV_P;
+            if (!bad_arg && !bad_len) need[j] = (int)(after / PKV_P) - len[j] / PKV_P;
         }
         sum += need[j];
     }
-    const bool arg = __syncthreads_or(bad_arg), cap = __syncthreads_or(bad_len);
-    int total;
-    int at = block_scan<16>(sum, lds, total);
-    bool full = cap;
-    if (!arg && !cap && total > 0) {
+    const int flag = (__ballot(bad_arg) ? 1 : 0) | (__ballot(bad_len) ? 2 : 0);
+    if (lane == 0) flags[w] = flag;
+    int total, all = 0;
+    int at = block_scan<NW>(sum, lds[0], total);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) all |= flags[i];
+    bool full = all & 2;
+    if (!all && total > 0) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             off[tid * PER + j] = at;
             at += need[j];
         }
-        __syncthreads();
         int found = 0;
-        for (int base = 0; base < c.nPages && found < total; base += 4 * 1024) {
-            const int p0 = base + 4 * tid;
-            bool is_free[4];
+        for (int base = 0; base < c.nPages && found < total; base += FREE * T) {
+            if (base) load_refs(base);
             int n = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                is_free[j] = p0 + j < c.nPages && c.refs[p0 + j] == 0;
-                n += is_free[j];
-            }
-            int here, k = found + block_scan<16>(n, lds, here);
+            for (int j = 0; j < FREE; ++j) n += ref[j] == 0;
+            int here, k = found + block_scan<NW>(n, lds[1], here);   // its barriers order off's writes, too
             found += here;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (is_free[j]) {
+            for (int j = 0; j < FREE; ++j)
+                if (ref[j] == 0) {
                     if (k < total) {
                         // the last sequence whose pages begin at or before the k-th; it needs one
                         int lo = 0, hi = c.nSeq;
@@ -128,8 +135,8 @@ __global__ __launch_bounds__(1024) void k_pkv_grow(GPT2PagedKV c, const int *__r
                             if (off[mid] <= k) lo = mid;
                             else hi = mid;
                         }
-                        c.table[(size_t)lo * c.maxPages + c.len[lo] / PKV_P + (k - off[lo])] = p0 + j;
-                        plan.map[k] = p0 + j;
+                        c.table[(size_t)lo * c.maxPages + c.len[lo] / PKV_P + (k - off[lo])] = base + FREE * tid + j;
+                        plan.map[k] = base + FREE * tid + j;
                     }
                     ++k;
                 }
@@ -137,16 +144,16 @@ __global__ __launch_bounds__(1024) void k_pkv_grow(GPT2PagedKV c, const int *__r
         full = found < total;   // the same in every thread
         __syncthreads();
         if (!full)
-            for (int k = tid; k < total; k += 1024) c.refs[plan.map[k]] = 1;
+            for (int k = tid; k < total; k += T) c.refs[plan.map[k]] = 1;
     }
-    const bool refuse = arg || full;
-    if (refuse && tid == 0) atomicCAS(c.status, 0, arg ? E_ARG : E_CAPACITY);
+    const bool refuse = (all & 1) || full;
+    if (refuse && tid == 0) atomicCAS(c.status, 0, all & 1 ? E_ARG : E_CAPACITY);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int s = tid * PER + j;
         if (s < c.nSeq) {
             c.start[s] = len[j];
-            if (!refuse) c.len[s] = len[j] + (rows[s + 1] - rows[s]);
+            if (!refuse) c.len[s] = len[j] + add[j];
         }
     }
 }
@@ -573,7 +580,7 @@ __global__ __launch_bounds__(1024) void k_pkv_compact_plan(GPT2PagedKV c) {
     }
 }
 
-// Second launch: the first `copiers` work-groups move pages (a unit is a page's codes and scales of one layer), the
+// Second launch: the first `copiers` work-groups move pages (a unit is eight tiles of one layer, and their scales), the
 // others renumber the page tables.
 __global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers) {
     const int tid = threadIdx.x;
@@ -587,15 +594,21 @@ __global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers)
         if (pkv_page_ok(c, page)) c.table[i] = plan.map[page];
         return;
     }
-    const long units = (long)plan.word[0] * c.nLayer;
-    const int pieces = 2 * c.nHead * (PKV_TILE / 16);
+    const int parts = (2 * c.nHead + 7) / 8, per = parts * c.nLayer;
+    const long units = (long)plan.word[0] * per;
     for (long u = blockIdx.x; u < units; u += copiers) {
-        const int k = (int)(u / c.nLayer), L = (int)(u % c.nLayer);
-        const size_t from = pkv_tile(c, c.nPages, L, plan.mover[k], 0, 0), to = pkv_tile(c, c.nPages, L, plan.hole[k], 0, 0);
-        const i32x4 *src = reinterpret_cast<const i32x4 *>(c.codes + from * PKV_TILE);
-        i32x4 *dst = reinterpret_cast<i32x4 *>(c.codes + to * PKV_TILE);
-        for (int i = tid; i < pieces; i += 256) dst[i] = src[i];
-        for (int i = tid; i < 2 * c.nHead; i += 256) c.scales[to + i] = c.scales[from + i];
+        const int k = (int)(u / per), r = (int)(u % per), L = r / parts, t0 = 8 * (r % parts);   // tiles t0 .. + 7, two at a time
+        const size_t from = pkv_tile(c, c.nPages, L, plan.mover[k], 0, 0) + t0, to = pkv_tile(c, c.nPages, L, plan.hole[k], 0, 0) + t0;
+        const i32x4 *src = reinterpret_cast<const i32x4 *>(c.codes + from * PKV_TILE) + tid;
+        i32x4 *dst = reinterpret_cast<i32x4 *>(c.codes + to * PKV_TILE) + tid;
+        const int n = min(8, 2 * c.nHead - t0), half = tid >> 7;
+        i32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = src[2 * i + half < n ? 256 * i : 0];   // past the last: what is there anyhow
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (2 * i + half < n) dst[256 * i] = v[i];
+        if (tid < n) c.scales[to + tid] = c.scales[from + tid];
     }
 }
 
@@ -685,7 +698,8 @@ extern "C" int gpt2_pkv_status(GPT2PagedKV *c) {
 
 extern "C" void gpt2_pkv_grow(GPT2PagedKV *c, const int *rows, int nRows) {
     if (pkv_refused_batch(c, 0, rows, nRows, "gpt2_pkv_grow: bad cache or rows")) return;
-    hipLaunchKernelGGL(k_pkv_grow, dim3(1), dim3(1024), 0, stream(), *c, rows, nRows);
+    if (c->nSeq <= 1024 && c->nPages <= 1 << 14 && nRows <= 256 * PKV_P) hipLaunchKernelGGL(k_pkv_grow<256>, dim3(1), dim3(256), 0, stream(), *c, rows, nRows);
+    else hipLaunchKernelGGL(k_pkv_grow<1024>, dim3(1), dim3(1024), 0, stream(), *c, rows, nRows);
     check_launch("k_pkv_grow");
 }
 

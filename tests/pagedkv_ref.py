@@ -236,7 +236,7 @@ def beam(logits, score, done, groups, beams, eos):
             with np.errstate(invalid="ignore", divide="ignore"):
                 s = cum + (x[r] - m) - np.log(np.exp(x[r] - m).sum())
             s = np.where(np.isnan(s), -np.inf, s)
-            for t in sorted(range(x.shape[1]), key=lambda t: (-x[r, t], t))[:beams]:
+            for t in np.argsort(-x[r], kind="stable")[:beams].tolist():
                 cand.append((s[t], r, -x[r, t], t, t))
         cand.sort(key=lambda c: (-c[0], c[1], c[2], c[3]))
         for a, b in zip(cand[:beams], cand[1:]):

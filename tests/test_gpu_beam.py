@@ -29,7 +29,8 @@ def check(pkg, L, logits, score, done, groups, beams, eos, **kw):
     got = select(pkg, L, logits, score, done, groups, beams, eos, **kw)
     token, parent, want, mark, gap = beam(logits, np.asarray(score, np.float32), done, groups, beams, eos)
     # The log of the sum: each exponential's argument is off by half a step 2^-24 of at most 60, the result by one step
-    # 2^-23 more, partial sums of 33 terms in fp32: below 2^-24 (60 + 2 + 33) of the sum.  The score's rounding: 2^-24 of it.
+    # 2^-23 more, a thread's sum of 33 of them at most in fp32: below 2^-24 (60 + 2 + 33) of the sum.  The score's rounding:
+    # 2^-24 of it.
     tol = 2.0 ** -24 * 95
     assert gap > 4 * tol, "two candidates too close to tell apart: not a case of this test"
     np.testing.assert_array_equal(got[0], token)
@@ -51,6 +52,17 @@ def test_select(pkg, L, groups, beams, V):
     rng = np.random.default_rng(1000 * beams + V)
     x, score, done = some(rng, groups * beams, V)
     check(pkg, L, x, score, done, groups, beams, V - 1)
+
+
+@pytest.mark.parametrize("V,shift", [(50257, 0), (50255, 3)])
+def test_many_rows(pkg, L, V, shift):
+    """As many rows as take the larger parts."""
+    rng = np.random.default_rng(V)
+    x, score, done = some(rng, 256, V)
+    x[7] = -np.inf
+    x[9, 5000:] = -np.inf
+    x[11] = 0
+    check(pkg, L, x, score, done, 32, 8, V - 1, shift=shift)
 
 
 @pytest.mark.parametrize("shift", range(8))
