@@ -70,12 +70,12 @@ __device__ __forceinline__ void page_take(const char *__restrict__ stage, PageRa
 }
 
 // A page as the products take it: fragments of K (k[t]: dims 16 g .. + 7 and + 8 .. + 15 of the lane's key of tile t) and of V
-// (v[2 i + b]: tokens 8 g .. + 7 of dim 32 i + 2 jq + b), its scales and first token; column jq sees keys below `lim`, which
-// `masked` says matters (the same in every lane).
+// (v[2 i + b]: tokens 8 g .. + 7 of dim 32 i + 2 jq + b), its scales and first token.  `masked`: not every column sees all of
+// it; then `only`: none does but that one (-1: all as their limits say).
 struct PageFrag {
     f16x8 k[2][2], v[4];
     float sk, sv;
-    int key0, lim;
+    int key0, only;
     bool masked;
 };
 
@@ -83,65 +83,83 @@ struct PageFrag {
 // compiler does not see what `inf` is, or it would make a maximum of it.
 __device__ __forceinline__ float max_by(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
-// N pages against the columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it where few
-// waves share a SIMD, and two pages go down it in little more than the time of one.
-template <int N>
-__device__ __forceinline__ void attn_pages(AttnAcc &A, const PageFrag (&P)[N], const f16x8 (&q)[2]) {
-    const int g = (threadIdx.x & 63) >> 4;
-    float s[N][8], scale[N], mx = -INFINITY, inf = INFINITY;
+// N pages against Q times 16 columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it
+// where few waves share a SIMD, and two pages go down it in little more than the time of one.  Column jq sees keys below lim.
+template <int N, int Q>
+__device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[N], const f16x8 (&q)[Q][2], const int (&lim)[Q]) {
+    const int jq = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    float s[Q][N][8], scale[N], mn[Q], base[Q], inf = INFINITY;
     asm("" : "+s"(inf));
+    bool moved = false;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         scale[n] = P[n].sk * (0.125f * 1.4426950408889634f);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][0], q[0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][1], q[1], y, 0, 0, 0);
+        for (int u = 0; u < Q; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][4 * t + r] = y[r];
-        }
+            for (int t = 0; t < 2; ++t) {
+                f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][0], q[u][0], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].k[t][1], q[u][1], y, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[u][n][4 * t + r] = y[r];
+            }
     }
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        if (P[n].masked) {
-            const int left = P[n].lim - P[n].key0 - 8 * g;
+    for (int n = 0; n < N; ++n)
+        if (P[n].masked)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[n][e] = e < left ? s[n][e] : -INFINITY;
-        }
-        const float m = max_by(max_by(max_by(s[n][0], s[n][1], inf), max_by(s[n][2], s[n][3], inf), inf),
-                               max_by(max_by(s[n][4], s[n][5], inf), max_by(s[n][6], s[n][7], inf), inf), inf);
-        mx = fmaxf(mx, m * scale[n]);
+            for (int u = 0; u < Q; ++u) {
+                const int left = (P[n].only < 0 || P[n].only == jq ? lim[u] : 0) - P[n].key0 - 8 * g;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[u][n][e] = e < left ? s[u][n][e] : -INFINITY;
+            }
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            mx = fmaxf(mx, max_by(max_by(max_by(s[u][n][0], s[u][n][1], inf), max_by(s[u][n][2], s[u][n][3], inf), inf),
+                                  max_by(max_by(s[u][n][4], s[u][n][5], inf), max_by(s[u][n][6], s[u][n][7], inf), inf), inf) * scale[n]);
+        mn[u] = fmaxf(A[u].m, group_max(mx));
+        base[u] = mn[u] == -INFINITY ? 0.f : mn[u];   // a column that sees none of these keys
+        moved |= mn[u] > A[u].m;
     }
-    const float mn = fmaxf(A.m, group_max(mx));
-    const float base = mn == -INFINITY ? 0.f : mn;   // a column that sees none of these keys
-    if (__ballot(mn > A.m)) {   // the maximum moves rarely after the first pages
-        const float corr = __builtin_amdgcn_exp2f(A.m - base);
-        A.m = mn;
-        A.l *= corr;
+    if (__ballot(moved)) {   // the maximum moves rarely after the first pages
 #pragma unroll
-        for (int i = 0; i < 4; ++i) A.o[i] *= corr;
+        for (int u = 0; u < Q; ++u) {
+            const float corr = __builtin_amdgcn_exp2f(A[u].m - base[u]);
+            A[u].m = mn[u];
+            A[u].l *= corr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A[u].o[i] *= corr;
+        }
     }
     // The weights are rounded to fp16, which costs an output about as much as its own rounding (1.2e-4 of it against
     // 2.1e-4; with s_v in them, so that P.V could add to o in the product, 2e-4: the largest weight is then no longer 1 exactly,
     // and it was no faster).
-    f16x8 p[N];
+    f16x8 p[Q][N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+    for (int u = 0; u < Q; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[n][e], scale[n], -base));
-    }
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[u][n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[u][n][e], scale[n], -base[u]));
     // their sum, of the fp16 values as they are multiplied, on the matrix units too: a row of ones
     const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
-    for (int n = 0; n < N; ++n) A.l = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, p[n], A.l, 0, 0, 0);
+    for (int u = 0; u < Q; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) A[u].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, p[u][n], A[u].l, 0, 0, 0);
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].v[i], p[n], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) A.o[i][r] = fmaf(y[r], P[n].sv, A.o[i][r]);
-        }
+            for (int u = 0; u < Q; ++u) {
+                const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(P[n].v[i], p[u][n], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) A[u].o[i][r] = fmaf(y[r], P[n].sv, A[u].o[i][r]);
+            }
 }
 
 __device__ __forceinline__ void page_widen(const PageRaw &R, PageFrag &P) {
@@ -180,32 +198,40 @@ struct AttnSteps {
     int beams, seq, len, slot, off;   // off: own pages of the beams before
 };
 
-// One pass: 16 columns (column jq: row `row` of the activations, -1 for none, which sees the keys below `lim`; every
+// One pass: Q times 16 columns (column jq: row `row` of the activations, -1 for none, which sees the keys below `lim`; every
 // column sees those below `first`), one head, split z of the steps.  The W waves take steps in turn and join in LDS.
 // One loop, two steps at a time, and little code around it: the instructions of a short call come from L2 (the call with one
 // token took 4.4 us with 8.5 KB of code and 5.4 with 11.6).
 template <int W>
 constexpr int ATTN_STAGES = W > 4 ? 4 : 2;   // of 4 KB
-template <int W>
+template <int W, int Q>
 struct AttnLds {
     char ring[W][ATTN_STAGES<W> * 2 * PKV_TILE];
-    float m[W][16], l[W][16];
+    float m[W][16 * Q], l[W][16 * Q];
+    static_assert(Q * 4 * 64 * 16 <= ATTN_STAGES<W> * 2 * PKV_TILE, "a wave's sums take its ring's place");
 };
-template <int W, bool BEAMS>
-__device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &st, int h, int z, int row, int lim, int first, AttnLds<W> &lds) {
+template <int Q>
+struct AttnCols {
+    int row[Q], lim[Q], first;
+};
+template <int W, bool BEAMS, int Q>
+__device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &st, int h, int z, const AttnCols<Q> &col, AttnLds<W, Q> &lds) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
     const int E = c.nHead * PKV_D;
     const int splits = min(a.splits, max(1, (st.total + a.per - 1) / a.per)), stride = splits * W;
     if (z >= splits) return;   // the whole work-group
-    const uint16_t *qrow = a.qkv + (size_t)max(row, 0) * 3 * E + h * PKV_D + 16 * g;
-    f16x8 q[2] = {};
-    if (row >= 0) {
-        q[0] = *reinterpret_cast<const f16x8 *>(qrow);
-        q[1] = *reinterpret_cast<const f16x8 *>(qrow + 8);
+    f16x8 q[Q][2] = {};
+    AttnAcc A[Q];
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        const uint16_t *qrow = a.qkv + (size_t)max(col.row[u], 0) * 3 * E + h * PKV_D + 16 * g;
+        if (col.row[u] >= 0) {
+            q[u][0] = *reinterpret_cast<const f16x8 *>(qrow);
+            q[u][1] = *reinterpret_cast<const f16x8 *>(qrow + 8);
+        }
+        attn_clear(A[u]);
     }
-    AttnAcc A;
-    attn_clear(A);
 
     const size_t vstep = (size_t)c.nHead * PKV_TILE;   // from a page's K tile to its V tile
     const int8_t *const layer = c.codes + pkv_tile(c, c.nPages, a.L, 0, 0, h) * PKV_TILE;
@@ -264,8 +290,8 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
                 const int j = open ? __builtin_ctzll(opened) : none ? 0 : __builtin_ctzll(left);
                 const int x = __builtin_amdgcn_readlane(who, j), bj = (x & 31) - 1;
                 P[n].key0 = (x >> 5) * PKV_P;
-                P[n].lim = none || (BEAMS && bj >= 0 && bj != jq) ? 0 : lim;
-                P[n].masked = none || open || (BEAMS && bj >= 0) || P[n].key0 + PKV_P > first;
+                P[n].only = none ? 16 : BEAMS ? bj : -1;
+                P[n].masked = none || open || (BEAMS && bj >= 0) || P[n].key0 + PKV_P > col.first;
                 if (open) {
                     const int slot = BEAMS && bj >= 0 ? __builtin_amdgcn_readlane(st.slot, max(bj, 0)) : st.slot0;
                     const uint16_t *k = c.open + pkv_tile(c, c.nSeq, a.L, slot, 0, h) * PKV_TILE;
@@ -284,61 +310,74 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
             if (todo) issue(stage);
             if (todo) issue(stage + 1);
             stage = (stage + 2) % ATTN_STAGES<W>;
-            attn_pages<2>(A, P, q);
+            attn_pages(A, P, q, col.lim);
         }
     }
     // the waves' sums to one maximum, then together
-    const float l = A.l[0];
-    if (g == 0) lds.m[w][jq] = l != 0.f ? A.m : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < Q; ++u)
+        if (g == 0) lds.m[w][16 * u + jq] = A[u].l[0] != 0.f ? A[u].m : -INFINITY;
     __syncthreads();
-    float mx = -INFINITY;
+    float mx[Q];
 #pragma unroll
-    for (int u = 0; u < W; ++u) mx = fmaxf(mx, lds.m[u][jq]);
-    const float f = l != 0.f ? __builtin_amdgcn_exp2f(A.m - mx) : 0.f;
-    if (row >= 0) {
-        if (g == 0) lds.l[w][jq] = l * f;
+    for (int u = 0; u < Q; ++u) {
+        mx[u] = -INFINITY;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) reinterpret_cast<f32x4 *>(lds.ring[w])[64 * d + lane] = A.o[d] * f;   // the ring is idle
+        for (int v = 0; v < W; ++v) mx[u] = fmaxf(mx[u], lds.m[v][16 * u + jq]);
+        const float f = A[u].l[0] != 0.f ? __builtin_amdgcn_exp2f(A[u].m - mx[u]) : 0.f;
+        if (col.row[u] >= 0) {
+            if (g == 0) lds.l[w][16 * u + jq] = A[u].l[0] * f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) reinterpret_cast<f32x4 *>(lds.ring[w])[64 * (4 * u + d) + lane] = A[u].o[d] * f;   // the ring is idle
+        }
     }
     __syncthreads();
-    if (w < 2 && row >= 0) {   // dims 32 w + 8 g .. + 7 of the column's row
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        // two waves a column block: dims 32 d + 8 g .. + 7 of the column's row
+        const int d = w - 2 * u, row = col.row[u];
+        if (d < 0 || d > 1 || row < 0) continue;
         float L = 0.f;
         f32x4 y[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int u = 0; u < W; ++u) {
-            const f32x4 *o = reinterpret_cast<const f32x4 *>(lds.ring[u]);
-            L += lds.l[u][jq];
-            y[0] += o[128 * w + lane];
-            y[1] += o[128 * w + 64 + lane];
+        for (int v = 0; v < W; ++v) {
+            const f32x4 *o = reinterpret_cast<const f32x4 *>(lds.ring[v]) + 64 * (4 * u + 2 * d) + lane;
+            L += lds.l[v][16 * u + jq];
+            y[0] += o[0];
+            y[1] += o[64];
         }
         if (a.splits == 1) {
             const float inv = L != 0.f ? 1.f / L : 0.f;   // no key: 0
             f16x8 o;
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = (f16)(y[e & 1][e >> 1] * inv);
-            *reinterpret_cast<f16x8 *>(a.att + (size_t)row * E + h * PKV_D + 32 * w + 8 * g) = o;
+            *reinterpret_cast<f16x8 *>(a.att + (size_t)row * E + h * PKV_D + 32 * d + 8 * g) = o;
         } else {
             const size_t at = ((size_t)z * a.nRows + row) * c.nHead + h;
-            float *o = a.po + at * PKV_D + 32 * w + 8 * g;
+            float *o = a.po + at * PKV_D + 32 * d + 8 * g;
             *reinterpret_cast<f32x4 *>(o) = f32x4{y[0][0], y[1][0], y[0][1], y[1][1]};
             *reinterpret_cast<f32x4 *>(o + 4) = f32x4{y[0][2], y[1][2], y[0][3], y[1][3]};
-            if (w == 0 && g == 0) a.pml[at] = float4{mx, L, __int_as_float(splits), 0.f};
+            if (d == 0 && g == 0) a.pml[at] = float4{mx[u], L, __int_as_float(splits), 0.f};
         }
     }
 }
 
-// Rows 16 rb .. + 15 of one sequence, as a pass.
-struct AttnCols {
-    int row, lim, first;
-};
-__device__ __forceinline__ AttnSteps attn_rows(const PkvSeq &s, int seq, int rb, AttnCols &col) {
-    const int i0 = 16 * rb, i = i0 + (threadIdx.x & 15), pages = (s.start + min(s.n, i0 + 16) + PKV_P - 1) / PKV_P;
-    col = {i < s.n ? s.row0 + i : -1, i < s.n ? s.start + i + 1 : 0, s.start + i0 + 1};
+// Rows 16 Q rb .. of one sequence, 16 Q of them, as a pass.
+template <int Q>
+__device__ __forceinline__ AttnSteps attn_rows(const PkvSeq &s, int seq, int rb, AttnCols<Q> &col) {
+    const int i0 = 16 * Q * rb, pages = (s.start + min(s.n, i0 + 16 * Q) + PKV_P - 1) / PKV_P;
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        const int i = i0 + 16 * u + (threadIdx.x & 15);
+        col.row[u] = i < s.n ? s.row0 + i : -1;
+        col.lim[u] = i < s.n ? s.start + i + 1 : 0;
+    }
+    col.first = s.start + i0 + 1;
     return {seq, s.len, s.slot, pages, pages, 0, 0, 0, 0, 0};
 }
 
 // The beams of a group, one row each at most, as a pass.  Lane b holds beam b's sequence; `on`: those with a row.
-__device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq &s, int seq0, uint64_t on, AttnCols &col) {
+__device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq &s, int seq0, uint64_t on, AttnCols<1> &col) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, jq = lane & 15, one = __builtin_ctzll(on);
     // the leading pages that all share, complete in each
@@ -370,29 +409,29 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
     }
     const int total = shared + __builtin_amdgcn_readlane(sum, 15);
     const int n = __shfl(s.n, jq, 64), row = __shfl(s.row0, jq, 64), len = __shfl(s.len, jq, 64);
-    col = {n ? row : -1, n ? len : 0, shared * PKV_P};
+    col = {{n ? row : -1}, {n ? len : 0}, shared * PKV_P};
     return {seq0 + one, __builtin_amdgcn_readlane(s.len, one), 0, shared, total, a.group, seq0 + min(lane, a.group - 1), s.len, s.slot, sum - own};
 }
 
 // One row a sequence, nearly always (no more rows than sequences): a work-group per sequence, head and split ...
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
-    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+    __shared__ __attribute__((aligned(1024))) AttnLds<W, 1> lds;
     const int h = blockIdx.x % a.c.nHead, seq = blockIdx.x / a.c.nHead;
     const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
 #pragma nounroll
     for (int rb = 0; 16 * rb < s.n; ++rb) {
         if (rb) __syncthreads();
-        AttnCols col;
+        AttnCols<1> col;
         const AttnSteps st = attn_rows(s, seq, rb, col);
-        attn_pass<W, false>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+        attn_pass<W, false, 1>(a, st, h, blockIdx.y, col, lds);
     }
 }
 
 // ... or per group of beams, together where they have a row each at most and there are two.
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
-    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+    __shared__ __attribute__((aligned(1024))) AttnLds<W, 1> lds;
     const int h = blockIdx.x % a.c.nHead, lane = threadIdx.x & 63;
     const int seq0 = blockIdx.x / a.c.nHead * a.group;
     PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq0 + min(lane, a.group - 1));
@@ -403,7 +442,7 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
     int b = __builtin_ctzll(on), rb = 0;
     for (;;) {
         AttnSteps st;
-        AttnCols col;
+        AttnCols<1> col;
         PkvSeq u;
         u.n = 0;
         if (together) {
@@ -417,7 +456,7 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
             st = attn_rows(u, seq0 + b, rb, col);
             st.off = 0x7fffffff;   // no step is a beam's own
         }
-        attn_pass<W, true>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+        attn_pass<W, true, 1>(a, st, h, blockIdx.y, col, lds);
         if (together) break;
         if (16 * ++rb >= u.n) {
             const uint64_t more = on & ~((2ull << b) - 1);   // b < 16
@@ -429,17 +468,18 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
     }
 }
 
-// Any number of rows a sequence: a work-group per 16 of them, head and split.
-template <int W>
-__global__ __launch_bounds__(64 * W) void k_pkv_attn_rows(PagedAttn a) {
-    __shared__ __attribute__((aligned(1024))) AttnLds<W> lds;
+// Any number of rows a sequence: a work-group per 16 Q of them, head and split.
+template <int Q>
+__global__ __launch_bounds__(256) void k_pkv_attn_rows(PagedAttn a) {
+    __shared__ __attribute__((aligned(1024))) AttnLds<4, Q> lds;
     const int h = blockIdx.x % a.c.nHead;
     int rb = blockIdx.x / a.c.nHead;
-    const int seq = pkv_seq_of_unit(rb, a.c.nSeq, [&](int s) { return (pkv_seq(a.c, a.rows, a.nRows, s).n + 15) / 16; });
+    const int seq = pkv_seq_of_unit(rb, a.c.nSeq, [&](int s) { return (pkv_seq(a.c, a.rows, a.nRows, s).n + 16 * Q - 1) / (16 * Q); });
     if (seq < 0) return;
-    AttnCols col;
-    const AttnSteps st = attn_rows(pkv_seq(a.c, a.rows, a.nRows, seq), seq, rb, col);
-    attn_pass<W, false>(a, st, h, blockIdx.y, col.row, col.lim, col.first, lds);
+    const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
+    AttnCols<Q> col;
+    const AttnSteps st = attn_rows(s, seq, (s.n + 16 * Q - 1) / (16 * Q) - 1 - rb, col);   // the longest first
+    attn_pass<4, false, Q>(a, st, h, blockIdx.y, col, lds);
 }
 
 // Many rows a sequence: a work-group per 64 of them and head, a wave per 16, every wave over all pages.  The four waves share
@@ -463,9 +503,10 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
     const int first = s.start + i0 + 1, lim = i < s.n ? s.start + i + 1 : 0;                 // keys that the wave's rows, and row i, see
     const int end = i0 < s.n ? s.start + min(s.n, i0 + 16) : 0;                               // ... and any of the wave's
     const uint16_t *qrow = a.qkv + (size_t)(s.row0 + min(i, s.n - 1)) * 3 * E + h * PKV_D + 16 * g;
-    const f16x8 q[2] = {*reinterpret_cast<const f16x8 *>(qrow), *reinterpret_cast<const f16x8 *>(qrow + 8)};
-    AttnAcc A;
-    attn_clear(A);
+    const f16x8 q[1][2] = {{*reinterpret_cast<const f16x8 *>(qrow), *reinterpret_cast<const f16x8 *>(qrow + 8)}};
+    AttnAcc A[1];
+    attn_clear(A[0]);
+    const int limit[1] = {lim};
 
     // The wave's quarter of a page: where its 16 bytes a lane lie in the tile, and the fragments' slots that they fill.  K: wave
     // t takes keys 8 x + 4 t + y, lane 16 x + 4 y + z dims 16 z .. + 15 of one, for lane 16 z + 4 x + y of the product.
@@ -510,7 +551,7 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
         P.sk = k;
         P.sv = v;
         P.key0 = p * PKV_P;
-        P.lim = lim;
+        P.only = -1;
         P.masked = P.key0 + PKV_P > first;
     };
     const int whole = min(pages, full);
@@ -544,11 +585,11 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
                             get(j & 1, k, base + pk, lane_f(sk, at), lane_f(sv, at), P[k]);
                             if (pk >= n || __builtin_amdgcn_readlane(page, at) < 0) {
                                 P[k].sk = P[k].sv = 1.f;
-                                P[k].lim = 0;
+                                P[k].only = 16;
                                 P[k].masked = true;
                             }
                         }
-                        attn_pages<2>(A, P, q);
+                        attn_pages(A, P, q, limit);
                     }
                     lds_barrier();
                 }
@@ -568,17 +609,17 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
         if (full * PKV_P < end) {
             PageFrag P[1];
             get(0, 0, full, 1.f, 1.f, P[0]);
-            attn_pages<1>(A, P, q);
+            attn_pages(A, P, q, limit);
         }
     }
-    const float inv = A.l[0] != 0.f ? 1.f / A.l[0] : 0.f;
+    const float inv = A[0].l[0] != 0.f ? 1.f / A[0].l[0] : 0.f;
     if (i < s.n) {
         uint16_t *out = a.att + (size_t)(s.row0 + i) * E + h * PKV_D + 8 * g;
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
             f16x8 o;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = (f16)(A.o[2 * d + (e & 1)][e >> 1] * inv);
+            for (int e = 0; e < 8; ++e) o[e] = (f16)(A[0].o[2 * d + (e & 1)][e >> 1] * inv);
             *reinterpret_cast<f16x8 *>(out + 32 * d) = o;
         }
     }
@@ -616,20 +657,33 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
     }
 }
 
-// How the steps are split over work-groups: at least `per` of them each, into `splits` at most.  None for caches whose
-// sequences a work-group's waves get through in the time of a second launch, nor where the rows alone make enough
-// work-groups.  Where splits of 64 pages fill the card they stream best (16 contexts up to 16384 tokens: 51 us, 59 with 16 pages
-// each); fewer sequences need smaller ones (one of 16384: 8.6 us, 14).
-struct AttnSplit {
-    int splits, per;
+// How a call runs: its form, and how the steps are split over work-groups: at least `per` of them each, into `splits` at most.
+//   ONE    no more rows than sequences: a sequence (or group of beams) a work-group.
+//   ROWS1  16 rows a work-group, keys split over its waves.
+//   ROWS2  32 of them, from 32 rows a sequence on: a page is made fp16 once for twice the rows (a prompt of 1000 rows 12 us; 19 with BLOCK).
+//   BLOCK  64, pages shared through LDS, where that makes eight work-groups a CU: 32 prompts of up to 1000 rows 85 us, 104 with
+//          ROWS2; 8 of up to 600 over 2000 tokens 64 us, 58 with ROWS2.
+// No splits for caches whose sequences a work-group's waves get through in the time of a second launch, nor where the rows alone
+// make enough work-groups.  Where splits of 64 pages fill the card they stream best (16 contexts up to 16384 tokens: 51 us, 59 with 16
+// pages each); fewer sequences need smaller ones (one of 16384: 8.6 us, 14).
+enum AttnForm { ATTN_ONE, ATTN_ROWS1, ATTN_ROWS2, ATTN_BLOCK };
+struct AttnPlan {
+    AttnForm form;
+    int groups, splits, per;   // work-groups of a split
 };
-static bool attn_by_block(const GPT2PagedKV *c, int nRows) { return nRows / 32 >= c->nSeq && (long)(nRows / 64) * c->nHead >= 128; }
-static AttnSplit attn_split(const GPT2PagedKV *c, int nRows) {
-    if (attn_by_block(c, nRows)) return {1, 64};
-    if (c->maxPages <= 64 || (nRows > c->nSeq && (long)(nRows / 16) * c->nHead >= 512)) return {1, 64};
-    const long groups = (long)(nRows > c->nSeq ? nRows / 16 + 1 : c->nSeq) * c->nHead;
-    const int per = groups * (c->maxPages / 64) >= 512 ? 64 : 16, n = cdiv(c->maxPages, per);
-    return {n > ATTN_SPLITS ? ATTN_SPLITS : n, per};
+static AttnPlan attn_plan(const GPT2PagedKV *c, int nRows, int group) {
+    AttnPlan p;
+    p.form = nRows <= c->nSeq ? ATTN_ONE : nRows / 32 < c->nSeq ? ATTN_ROWS1 : (long)(nRows / 64) * c->nHead < 2048 ? ATTN_ROWS2 : ATTN_BLOCK;
+    const int rows = p.form == ATTN_ROWS1 ? 16 : p.form == ATTN_ROWS2 ? 32 : 64;   // of a work-group
+    p.groups = (p.form == ATTN_ONE ? c->nSeq / group : nRows / rows + c->nSeq) * c->nHead;
+    p.splits = 1;
+    p.per = 64;
+    const long busy = (long)(p.form == ATTN_ONE ? c->nSeq : nRows / rows + 1) * c->nHead;   // work-groups with something to do, about
+    if (p.form == ATTN_BLOCK || c->maxPages <= 64 || (p.form != ATTN_ONE && busy >= 512)) return p;
+    if (busy * (c->maxPages / 64) < 512) p.per = 16;
+    p.splits = cdiv(c->maxPages, p.per);
+    if (p.splits > ATTN_SPLITS) p.splits = ATTN_SPLITS;
+    return p;
 }
 
 }  // namespace g2
@@ -638,7 +692,7 @@ using namespace g2;
 
 extern "C" size_t gpt2_pkv_attn_ws(const GPT2PagedKV *c, int nRows) {
     if (!c || nRows < 1 || c->nHead < 1 || c->maxPages < 1) return 16;
-    const int n = attn_split(c, nRows).splits;
+    const int n = attn_plan(c, nRows, 1).splits;   // the same for any group
     return n == 1 ? 16 : (size_t)n * nRows * c->nHead * (PKV_D + 4) * 4;
 }
 
@@ -657,23 +711,21 @@ extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2Pa
     a.L = L;
     a.nRows = nRows;
     a.group = group;
-    const AttnSplit sp = attn_split(c, nRows);
-    a.splits = sp.splits;
-    a.per = sp.per;
+    const AttnPlan p = attn_plan(c, nRows, group);
+    a.splits = p.splits;
+    a.per = p.per;
     a.po = (float *)ws;
     a.pml = (float4 *)(a.po + (size_t)a.splits * nRows * c->nHead * PKV_D);
-    if (attn_by_block(c, nRows)) {
-        hipLaunchKernelGGL(k_pkv_attn_block, dim3((nRows / 64 + c->nSeq) * c->nHead), dim3(256), 0, stream(), a);
-    } else if (nRows > c->nSeq) {
-        hipLaunchKernelGGL(k_pkv_attn_rows<4>, dim3((nRows / 16 + c->nSeq) * c->nHead, a.splits), dim3(256), 0, stream(), a);
-    } else {
-        const int groups = c->nSeq / group * c->nHead;
-        const bool wide = a.splits == 1 && groups < 256;
-        const auto fn = group > 1 ? (wide ? k_pkv_attn_beams<8> : k_pkv_attn_beams<4>) : wide ? k_pkv_attn_one<8> : k_pkv_attn_one<4>;
-        hipLaunchKernelGGL(fn, dim3(groups, a.splits), dim3(wide ? 512 : 256), 0, stream(), a);
-    }
+    const bool wide = p.form == ATTN_ONE && p.splits == 1 && p.groups < 256;   // eight waves where that leaves CUs idle
+    const auto fn = p.form == ATTN_BLOCK   ? k_pkv_attn_block
+                    : p.form == ATTN_ROWS2 ? k_pkv_attn_rows<2>
+                    : p.form == ATTN_ROWS1 ? k_pkv_attn_rows<1>
+                    : group > 1            ? (wide ? k_pkv_attn_beams<8> : k_pkv_attn_beams<4>)
+                    : wide                 ? k_pkv_attn_one<8>
+                                           : k_pkv_attn_one<4>;
+    hipLaunchKernelGGL(fn, dim3(p.groups, p.splits), dim3(wide ? 512 : 256), 0, stream(), a);
     if (a.splits > 1) {
-        const bool by_seq = nRows <= c->nSeq;
+        const bool by_seq = p.form == ATTN_ONE;
         hipLaunchKernelGGL(by_seq ? k_pkv_attn_join<true> : k_pkv_attn_join<false>, dim3(by_seq ? c->nSeq : nRows, cdiv(c->nHead, 4)), dim3(256), 0,
                            stream(), a);
     }

@@ -71,13 +71,13 @@ __global__ void k_pkv_reset(GPT2PagedKV c) {
 
 // ------------------------------------------------------------------ grow
 // One work-group: needs and their sums over the sequences, then a walk over refs that hands the lowest free pages out in
-// order, which stops when enough are found (its first step is under way meanwhile).  Table entries past the complete pages mean
-// nothing, so they are written as pages are found; refs and lengths follow once all are.  Bound by the latency of its few dependent
+// order, which stops when enough are found (its first step is under way meanwhile); tables, refs and lengths are written once they
+// are.  Bound by the latency of its few dependent
 // loads and barriers: T = 256 threads where they are enough (48 sequences, one of them needing a page: see DESIGN.md's table).
 template <int T>
 __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
     constexpr int NW = T / 64, PER = GPT2_PKV_MAX_SEQ / 1024, FREE = 8;
-    __shared__ int off[PER * T], lds[2][NW + 2], flags[NW];
+    __shared__ int off[PER * T], place[PER * T], lds[2][NW + 2], flags[NW];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const PkvPlan plan = pkv_plan(c);
     int ref[FREE];
@@ -114,6 +114,7 @@ __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__rest
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             off[tid * PER + j] = at;
+            place[tid * PER + j] = (tid * PER + j) * c.maxPages + len[j] / PKV_P - at;   // of the k-th page handed out, less k
             at += need[j];
         }
         int found = 0;
@@ -122,29 +123,30 @@ __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__rest
             int n = 0;
 #pragma unroll
             for (int j = 0; j < FREE; ++j) n += ref[j] == 0;
-            int here, k = found + block_scan<NW>(n, lds[1], here);   // its barriers order off's writes, too
+            int here, k = found + block_scan<NW>(n, lds[1], here);
             found += here;
 #pragma unroll
             for (int j = 0; j < FREE; ++j)
                 if (ref[j] == 0) {
-                    if (k < total) {
-                        // the last sequence whose pages begin at or before the k-th; it needs one
-                        int lo = 0, hi = c.nSeq;
-                        while (hi - lo > 1) {
-                            const int mid = (lo + hi) >> 1;
-                            if (off[mid] <= k) lo = mid;
-                            else hi = mid;
-                        }
-                        c.table[(size_t)lo * c.maxPages + c.len[lo] / PKV_P + (k - off[lo])] = base + FREE * tid + j;
-                        plan.map[k] = base + FREE * tid + j;
-                    }
+                    if (k < total) plan.map[k] = base + FREE * tid + j;
                     ++k;
                 }
         }
         full = found < total;   // the same in every thread
         __syncthreads();
         if (!full)
-            for (int k = tid; k < total; k += T) c.refs[plan.map[k]] = 1;
+            for (int k = tid; k < total; k += T) {
+                // the last sequence whose pages begin at or before the k-th; it needs one
+                int lo = 0, hi = c.nSeq;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (off[mid] <= k) lo = mid;
+                    else hi = mid;
+                }
+                const int page = plan.map[k];
+                c.table[place[lo] + k] = page;
+                c.refs[page] = 1;
+            }
     }
     const bool refuse = (all & 1) || full;
     if (refuse && tid == 0) atomicCAS(c.status, 0, all & 1 ? E_ARG : E_CAPACITY);
@@ -338,19 +340,14 @@ __global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const 
                                                     const int *__restrict__ rows, int nRows) {
     __shared__ __attribute__((aligned(16))) char lds[4][PKV_P * PKV_ROW];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kh = blockIdx.y * 4 + w;
-    if (kh >= 2 * c.nHead) return;   // wave-uniform; no barrier follows
     int u = BY_SEQ ? 0 : blockIdx.x;
     const int seq = BY_SEQ ? (int)blockIdx.x : pkv_seq_of_unit(u, c.nSeq, [&](int s) { return pkv_append_units(pkv_seq(c, rows, nRows, s)); });
     if (seq < 0) return;
     const PkvSeq q = pkv_seq(c, rows, nRows, seq);
-    const int kv = kh >= c.nHead, h = kh - kv * c.nHead;
-    if constexpr (BY_SEQ) {
-        const int n = pkv_append_units(q);
-        for (u = 0; u < n; ++u) pkv_append_unit(c, L, qkv, q, seq, u, kv, h, lds[w]);
-    } else {
-        pkv_append_unit(c, L, qkv, q, seq, u, kv, h, lds[w]);
-    }
+    const int n = BY_SEQ ? pkv_append_units(q) : u + 1;
+    for (; u < n; ++u)
+        for (int kh = blockIdx.y * 4 + w; kh < 2 * c.nHead; kh += 4 * gridDim.y)   // wave-uniform; there is no barrier
+            pkv_append_unit(c, L, qkv, q, seq, u, kh >= c.nHead, kh % c.nHead, lds[w]);
 }
 
 // ------------------------------------------------------------------ read
@@ -717,7 +714,10 @@ extern "C" void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, con
     if (nRows == 0) return;
     if (!qkv || !aligned16(qkv)) { arg_fail("gpt2_pkv_append: null/unaligned"); return; }
     const bool by_seq = nRows <= c->nSeq;
-    const dim3 grid(by_seq ? c->nSeq : nRows / PKV_P + c->nSeq, cdiv(2 * c->nHead, 4));
+    // a wave takes one tile of a unit, two where there are work-groups for more than two rounds of the card: 48 prompts of 250 to
+    // 1000 rows 37.6 -> 33.9 us (4.1 TB/s), 8 prompts of up to 700 10.9 -> 12.9
+    const int units = by_seq ? c->nSeq : nRows / PKV_P + c->nSeq, per = !by_seq && (long)units * c->nHead >= 8192 ? 2 : 1;
+    const dim3 grid(units, cdiv(2 * c->nHead, 4 * per));
     const auto fn = by_seq ? k_pkv_append<true> : k_pkv_append<false>;
     hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream(), *c, L, qkv, rows, nRows);
     check_launch("k_pkv_append");

@@ -184,10 +184,15 @@ def test_attention_many_sequences(pkg, L):
     (12, [0, 0, 0], [704, 0, 33]),
     (16, [31, 32], [1, 640]),
     (12, [2100], [770]),
+    (1024, [40, 0], [100, 33]),
+    (700, [33], [200]),
+    (1, [33, 1], [400, 100]),
 ])
-def test_attention_blocks(pkg, L, heads, before, counts):
-    """Batches of enough rows for work-groups of 64: prompts from nothing, prompts on top of cached ones, ragged."""
-    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=100, seqs=len(counts), max_len=3000), np.random.default_rng(20)
+def test_attention_many_rows(pkg, L, heads, before, counts):
+    """Batches of many rows a sequence, which take work-groups of 32 and of 64 rows, with splits and without: prompts from
+    nothing, prompts on top of cached ones, ragged."""
+    pages = sum(-(-(b + n) // P) for b, n in zip(before, counts))
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=pages, seqs=len(counts), max_len=3000), np.random.default_rng(20)
     p.step(rng, before)
     x = p.step(rng, counts)
     p.same()
