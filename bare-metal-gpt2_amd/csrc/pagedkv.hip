@@ -161,21 +161,25 @@ __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__rest
 }
 
 // ------------------------------------------------------------------ embed
-__global__ __launch_bounds__(256) void k_pkv_embed(uint16_t *__restrict__ x, const uint16_t *__restrict__ wte,
-                                                   const uint16_t *__restrict__ wpe, const int *__restrict__ ids, GPT2PagedKV c,
-                                                   const int *__restrict__ rows, int nRows) {
+// A work-group a row, four values a thread: 8-byte loads and stores.
+constexpr int EMBED_THREADS = GPT2_N_EMBD / 4;
+__global__ __launch_bounds__(EMBED_THREADS) void k_pkv_embed(uint16_t *__restrict__ x, const uint16_t *__restrict__ wte,
+                                                             const uint16_t *__restrict__ wpe, const int *__restrict__ ids, GPT2PagedKV c,
+                                                             const int *__restrict__ rows, int nRows) {
     constexpr int E = GPT2_N_EMBD;
-    const int row = blockIdx.x;
+    static_assert(E % 4 == 0, "four values a thread");
+    const int row = blockIdx.x, e = 4 * threadIdx.x;
     const int s = pkv_seq_of_row(rows, c.nSeq, row);
     if (s < 0) return;
     const PkvSeq q = pkv_seq(c, rows, nRows, s);
     if (q.n == 0) return;
     const int pos = q.start + row - q.row0, id = ids[row];
-    for (int e = threadIdx.x; e < E; e += 256) {
-        const float te = (unsigned)id < (unsigned)GPT2_VOCAB ? h2f(wte[(size_t)id * E + e]) : 0.f;
-        const float pe = (unsigned)pos < (unsigned)GPT2_N_CTX ? h2f(wpe[(size_t)pos * E + e]) : 0.f;
-        x[(size_t)row * E + e] = f2h(te + pe);
-    }
+    f16x4 te = {}, pe = {}, y;
+    if ((unsigned)id < (unsigned)GPT2_VOCAB) te = *reinterpret_cast<const f16x4 *>(wte + (size_t)id * E + e);
+    if ((unsigned)pos < (unsigned)GPT2_N_CTX) pe = *reinterpret_cast<const f16x4 *>(wpe + (size_t)pos * E + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (f16)((float)te[i] + (float)pe[i]);
+    *reinterpret_cast<f16x4 *>(x + (size_t)row * E + e) = y;
 }
 
 // ------------------------------------------------------------------ append
@@ -610,6 +614,7 @@ __global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers)
 }
 
 // ------------------------------------------------------------------ host
+constexpr int PKV_MAX_ROWS = 1 << 23;   // a launch of a work-group a row has fewer than 2^32 threads
 bool pkv_refused(const GPT2PagedKV *c, const char *what) {
     if (!c) return arg_fail(what);
     const void *p[] = {c->scales, c->table, c->len, c->start, c->slot, c->refs, c->status, c->plan};
@@ -625,7 +630,7 @@ bool pkv_refused(const GPT2PagedKV *c, const char *what) {
 
 bool pkv_refused_batch(const GPT2PagedKV *c, int L, const int *rows, int nRows, const char *what) {
     if (pkv_refused(c, what)) return true;
-    if (L < 0 || L >= c->nLayer || !rows || ((uintptr_t)rows & 3) || nRows < 0 || nRows > (1 << 24)) return arg_fail(what);
+    if (L < 0 || L >= c->nLayer || !rows || ((uintptr_t)rows & 3) || nRows < 0 || nRows > PKV_MAX_ROWS) return arg_fail(what);
     return false;
 }
 
@@ -640,6 +645,8 @@ extern "C" int gpt2_pkv_alloc(GPT2PagedKV *c, int nLayer, int nHead, int nPages,
     memset(c, 0, sizeof(*c));
     if (nLayer < 1 || nLayer > 32000 || nHead < 1 || nHead > 4096 || nPages < 1 || nPages > (1 << 26) || nSeq < 1 || nSeq > GPT2_PKV_MAX_SEQ || maxLen < 1 ||
         maxLen > (1 << 30) || (long)nSeq * cdiv(maxLen, PKV_P) > (1L << 30))
+        return arg_fail("gpt2_pkv_alloc: sizes out of range"), 1;
+    if ((double)nLayer * nHead * ((double)nPages + nSeq) > 0x1p40)   // the sizes below would not fit 64 bits
         return arg_fail("gpt2_pkv_alloc: sizes out of range"), 1;
     const size_t maxPages = cdiv(maxLen, PKV_P), tiles = (size_t)nLayer * nPages * 2 * nHead, opens = (size_t)nLayer * nSeq * 2 * nHead;
     const size_t sizes[] = {tiles * PKV_TILE, tiles * 4, opens * PKV_TILE * 2, (size_t)nSeq * maxPages * 4, (size_t)nSeq * 4, (size_t)nSeq * 4,
@@ -704,8 +711,11 @@ extern "C" void gpt2_pkv_embed(gpt2_half *x, const gpt2_half *wte, const gpt2_ha
                                const int *rows, int nRows) {
     if (pkv_refused_batch(c, 0, rows, nRows, "gpt2_pkv_embed: bad cache or rows")) return;
     if (nRows == 0) return;
-    if (!x || !wte || !wpe || !ids) { arg_fail("gpt2_pkv_embed: null pointer"); return; }
-    hipLaunchKernelGGL(k_pkv_embed, dim3(nRows), dim3(256), 0, stream(), x, wte, wpe, ids, *c, rows, nRows);
+    if (!x || !wte || !wpe || !ids || !aligned16(x) || !aligned16(wte) || !aligned16(wpe) || ((uintptr_t)ids & 3)) {
+        arg_fail("gpt2_pkv_embed: null/unaligned");
+        return;
+    }
+    hipLaunchKernelGGL(k_pkv_embed, dim3(nRows), dim3(EMBED_THREADS), 0, stream(), x, wte, wpe, ids, *c, rows, nRows);
     check_launch("k_pkv_embed");
 }
 

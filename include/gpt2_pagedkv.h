@@ -12,7 +12,8 @@
  *
  * A ragged batch.  `rows` is a device array of nSeq + 1 offsets: rows[s] .. rows[s+1] - 1 are sequence s's
  * new rows in the activations (qkv [nRows][3 E], x and att [nRows][E], E = nHead * headDim), none is fine.
- * Rows of the activations past rows[nSeq] are left as they are.  One step of a model over a batch:
+ * nRows, at most 2^23, is how many rows the buffers hold; those past rows[nSeq] are left as they are.  One step
+ * of a model over a batch:
  *     gpt2_pkv_grow(c, rows, nRows);              once: pages for the new rows, positions, lengths
  *     gpt2_pkv_embed(x, wte, wpe, ids, c, rows, nRows);
  *     per layer L: ... qkv ...; gpt2_pkv_append(c, L, qkv, rows, nRows);
@@ -80,10 +81,12 @@ int gpt2_pkv_status(GPT2PagedKV *c);
  * they complete (all layers). */
 void gpt2_pkv_grow(GPT2PagedKV *c, const int *rows, int nRows);
 /* x[row] = fp16(wte[ids[row]] + wpe[position of the row]) (GPT2_N_EMBD wide); a token outside the vocabulary or a
- * position past GPT2_N_CTX adds nothing, as gpt2_embed_one's kernel has it. */
+ * position past GPT2_N_CTX adds nothing, as gpt2_embed_one's kernel has it.  x, wte and wpe are
+ * 16-byte aligned. */
 void gpt2_pkv_embed(gpt2_half *x, const gpt2_half *wte, const gpt2_half *wpe, const int *ids, const GPT2PagedKV *c,
                     const int *rows, int nRows);
-/* The keys and values of the new rows into layer L: open pages, and the pages that they complete. */
+/* The keys and values of the new rows into layer L: open pages, and the pages that they complete:
+ * once for each layer after a grow. */
 void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, const int *rows, int nRows);
 /* att[row] = softmax(q . k / 8) v over the tokens up to the row's own, from the cache.  `group`: 1, or how many
  * consecutive sequences (at most 16) are beams of one prompt: the leading pages that all of a group share are then

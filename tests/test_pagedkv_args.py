@@ -51,7 +51,8 @@ def test_bad_caches(pkg, L, bad):
 def test_bad_batches(pkg, L):
     r = C.byref(cache(pkg))
     for call in (lambda: L.gpt2_pkv_grow(r, None, 4), lambda: L.gpt2_pkv_grow(r, ROWS + 2, 4), lambda: L.gpt2_pkv_grow(r, ROWS, -1),
-                 lambda: L.gpt2_pkv_grow(r, ROWS, (1 << 24) + 1),
+                 lambda: L.gpt2_pkv_grow(r, ROWS, (1 << 23) + 1),
+                 lambda: L.gpt2_pkv_embed(ROWS + 2, ROWS, ROWS, ROWS, r, ROWS, 4), lambda: L.gpt2_pkv_embed(ROWS, ROWS, ROWS + 8, ROWS, r, ROWS, 4),
                  lambda: L.gpt2_pkv_embed(None, ROWS, ROWS, ROWS, r, ROWS, 4), lambda: L.gpt2_pkv_embed(ROWS, ROWS, ROWS, None, r, ROWS, 4),
                  lambda: L.gpt2_pkv_append(r, 2, ROWS, ROWS, 4), lambda: L.gpt2_pkv_append(r, -1, ROWS, ROWS, 4),
                  lambda: L.gpt2_pkv_append(r, 0, None, ROWS, 4), lambda: L.gpt2_pkv_append(r, 0, ROWS + 2, ROWS, 4),
@@ -87,7 +88,7 @@ def test_empty_batches_do_nothing(pkg, L):
 def test_alloc_sizes(pkg, L):
     c = pkg.GPT2PagedKV()
     for bad in ((0, 12, 10, 4, 100), (1, 0, 10, 4, 100), (1, 12, 0, 4, 100), (1, 12, 10, 0, 100), (1, 12, 10, 4097, 100), (1, 12, 10, 4, 0),
-                (1, 12, 1 << 27, 4, 100), (1, 12, 10, 4096, 1 << 30)):
+                (1, 12, 1 << 27, 4, 100), (16384, 4096, 1 << 26, 4, 100), (1 << 14, 1 << 11, 1 << 26, 1, 100), (1, 12, 10, 4096, 1 << 30)):
         assert L.gpt2_pkv_alloc(C.byref(c), *bad) != 0
         assert L.gpt2_last_error() == ARG
     assert L.gpt2_pkv_alloc(None, 1, 12, 10, 4, 100) != 0
