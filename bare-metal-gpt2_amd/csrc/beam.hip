@@ -3,7 +3,7 @@
 //
 // score_b + x - m_b - log(sum_b) orders a row's tokens as its logits do, so a row's candidates are its best `beams` logits:
 // one pass over the logits takes each part of a row's maximum, its sum of exponentials and its best, and a second launch, a
-// work-group a group, joins the parts and ranks the beams x beams candidates in fp64.  Bound by reading the logits once.
+// work-group a group, joins the parts and merges the rows' lists of candidates in fp64.  Bound by reading the logits once.
 //
 // A logit and its token are one 32-bit key, (logit's bits in order) << 16 | (65535 - token): keys of a row are unique, and
 // the larger key is the larger logit or, of equal ones, the lower token.  0 is no key.
@@ -15,9 +15,10 @@
 
 namespace g2 {
 
-// 16-byte pieces a thread: a work-group takes 4096 logits of few rows, 8192 of many.
-constexpr int BEAM_FEW = 2, BEAM_MANY = 4;
-constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / (256 * BEAM_FEW);
+// 16-byte pieces a thread, 8192 logits a work-group.  Half as many were slower (512 rows of 50257: 21 us, 18; four rows: as
+// long, and longer to join), twice as many too (30 us).
+constexpr int BEAM_PIECES = 4;
+constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / (256 * BEAM_PIECES);
 struct BeamPart {
     double sum;                                         // of exp(x - m)
     float m;
@@ -76,16 +77,16 @@ __device__ __forceinline__ float beam_key_logit(uint32_t key) {
 // piece and after the last.
 //
 // A thread's logits stay in registers as keys of their own, order << 16 | (63 - i) for its i-th; the tokens of a thread
-// ascend with i, so its largest is its best.  A wave's `beams`-th best thread is a lower bound for the part's result, and the
-// keys at or above the waves' best bound (those of 4 beams - 3 threads at most) are ranked by counting.
-template <int NV>
+// ascend with i, so its largest is its best.  A key that `beams` threads of a wave reach is a lower bound for the part's result;
+// the highest such is found bit by bit, a comparison and a count each, until just `beams` reach it.  The keys at or above the
+// waves' best bound (those of 4 beams threads at most) are ranked by counting.
 __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, const uint16_t *__restrict__ logits, long ld, int V,
                                                    int beams, int parts) {
-    constexpr int N = 8 * NV;
+    constexpr int NV = BEAM_PIECES, N = 8 * NV;
     static_assert(N <= 64, "a thread's keys hold its index in 6 bits");
     __shared__ float lds_m[4];
     __shared__ double lds_s[4];
-    __shared__ uint32_t lds_t[4], lds_k[(4 * GPT2_BEAM_MAX - 3) * (N + 1)];
+    __shared__ uint32_t lds_t[4], lds_k[4 * GPT2_BEAM_MAX * (N + 1)];
     __shared__ int lds_n;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, part = blockIdx.x;
     const uint16_t *x = logits + (size_t)blockIdx.y * ld;
@@ -108,10 +109,16 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
         v[i] = beam_logits(v[i]);
-        const uint32_t o = first + 256 * (i / 4) < pieces ? beam_order(v[i]) : 0u;
+        const uint32_t o = beam_order(v[i]);
         key[2 * i] = __builtin_amdgcn_perm(o, (uint32_t)(63 - 2 * i), 0x05040100u);       // o << 16 | ..
         key[2 * i + 1] = __builtin_amdgcn_perm(o, (uint32_t)(62 - 2 * i), 0x07060100u);   // o's upper half | ..
         piece[i / 4] = max(piece[i / 4], max(key[2 * i], key[2 * i + 1]));
+    }
+    if (256 * NV * (part + 1) > pieces) {   // the last part: pieces that are none have no keys
+#pragma unroll
+        for (int i = 0; i < N; ++i) key[i] = first + 256 * (i / 8) < pieces ? key[i] : 0u;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) piece[j] = first + 256 * j < pieces ? piece[j] : 0u;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) best = max(best, piece[j]);
@@ -126,12 +133,22 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     best = max(best, kodd);
 
     // the wave's maximum, and the bound
-    uint32_t top = wave_max_key(best), bound = top, rest = best;
+    const uint32_t top = wave_max_key(best);
     const float m = top ? beam_key_logit(top) : -INFINITY;
-    for (int k = 1; k < beams; ++k) {
-        rest = rest == bound ? 0u : rest;
-        bound = wave_max_key(rest);
-    }
+    uint32_t bound = 0u;
+    if (beams <= 4) {   // maximum after maximum is quicker for few (4 rows, 4 beams: 5.0 us, 5.2)
+        bound = top;
+        uint32_t rest = best;
+        for (int k = 1; k < beams; ++k) {
+            rest = rest == bound ? 0u : rest;
+            bound = wave_max_key(rest);
+        }
+    } else
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            const int n = __popcll(__ballot(best >= (bound | bit)));
+            if (n >= beams) bound |= bit;
+            if (n == beams) break;
+        }
     // exp(x - m) as 2^(x l - c), l = log2 e in fp32, c = m l rounded; what the rounding takes is put back in fp64
     constexpr float l2e = 1.4426950408889634f;
     const float c = m == -INFINITY ? 0.f : m * l2e;
@@ -183,20 +200,19 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     }
 }
 
-// A work-group per group, a wave per row: the row's parts are joined, then a thread per candidate counts those ahead of it.
-// K: a lane's keys, four parts each.
-template <int K>
+// A work-group per group, a wave per row: the row's parts are joined, then one wave merges the rows' candidates.
 __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restrict__ token, int *__restrict__ parent, float *score_out, int *done_out,
                                                                   const BeamPart *__restrict__ part, const float *score, const int *done,
                                                                   int beams, int V, int eos, int parts) {
+    constexpr int K = BEAM_PARTS / 4;   // a lane's keys, four parts each
     __shared__ double cand[GPT2_BEAM_MAX * GPT2_BEAM_MAX];
-    __shared__ int tok[GPT2_BEAM_MAX * GPT2_BEAM_MAX];   // beam b's at b * beams; -1: no candidate
+    __shared__ int tok[GPT2_BEAM_MAX * GPT2_BEAM_MAX];   // beam b's at b * beams
     const int tid = threadIdx.x, lane = tid & 63, b = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row = blockIdx.x * beams + b;
     const BeamPart *p = part + (size_t)row * parts;
     const double from = (double)score[row];
     const bool ended = eos >= 0 && done[row];
-    static_assert(GPT2_BEAM_MAX == 16 && BEAM_PARTS <= 16, "16 places a part, a part a lane, four keys a lane");
+    static_assert(GPT2_BEAM_MAX == 16 && BEAM_PARTS <= 8, "16 places a part, a part a lane, two keys a lane");
     uint32_t key[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) {
@@ -224,32 +240,48 @@ __global__ __launch_bounds__(64 * GPT2_BEAM_MAX) void k_beam_join(int *__restric
         double s = ended ? from : from + ((double)beam_key_logit(mine) - (double)m) - lse;
         if (s != s) s = -INFINITY;
         const bool there = ended ? lane == 0 : mine != 0;
-        cand[b * beams + lane] = there ? s : (double)NAN;   // one that is not there is ahead of none
-        tok[b * beams + lane] = !there ? -1 : ended ? eos : 65535 - (int)(mine & 0xffffu);
+        cand[b * beams + lane] = there ? s : (double)NAN;   // NaN: not there
+        tok[b * beams + lane] = ended ? eos : 65535 - (int)(mine & 0xffffu);
     }
     __syncthreads();
-    const int all = beams * beams;
-    if (tid >= all || tok[tid] < 0) return;
-    const double s = cand[tid];
-    int rank = 0;
-#pragma unroll 4
-    for (int i = 0; i < all; ++i) {
-        const double c = cand[i];
-        rank += i < tid ? c >= s : c > s;
+    if (b) return;
+    // the rows' lists, each in order, merged: lane r has row r's next candidate
+    int at = min(lane, beams - 1) * beams, my_row = 0, my_at = 0;
+    const int last = at + beams - 1;
+    double next = lane < beams ? cand[at] : (double)NAN;
+    for (int k = 0; k < beams; ++k) {
+        double best = next;   // NaN gives way to numbers, and a number is left: every row has a candidate
+        auto step = [&](auto ctrl) {
+            const uint64_t v = __builtin_bit_cast(uint64_t, best);
+            const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, ctrl.value, 0xF, 0xF, true);
+            const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), ctrl.value, 0xF, 0xF, true);
+            best = fmax(best, __builtin_bit_cast(double, (uint64_t)hi << 32 | lo));
+        };
+        step(std::integral_constant<int, 0xB1>{});
+        step(std::integral_constant<int, 0x4E>{});
+        step(std::integral_constant<int, 0x141>{});
+        step(std::integral_constant<int, 0x140>{});
+        const int r = __builtin_ctzll(__ballot(next == best) | 1ull << 63);   // of equal scores the lower row
+        const int from = __builtin_amdgcn_readlane(at, r);
+        if (lane == k) {
+            my_row = r;
+            my_at = from;
+        }
+        if (lane == r) {
+            next = at < last ? cand[at + 1] : (double)NAN;
+            ++at;
+        }
     }
-    if (rank < beams) {
-        const int at = blockIdx.x * beams + rank;
-        token[at] = tok[tid];
-        parent[at] = blockIdx.x * beams + tid / beams;
-        score_out[at] = (float)s;
-        done_out[at] = eos >= 0 && tok[tid] == eos;
+    if (lane < beams) {
+        const int o = blockIdx.x * beams + lane, t = tok[my_at];
+        token[o] = t;
+        parent[o] = blockIdx.x * beams + my_row;
+        score_out[o] = (float)cand[my_at];
+        done_out[o] = eos >= 0 && t == eos;
     }
 }
 
-// Many rows fill the card with large parts, which have less to do for each logit (64 x 8 rows of 50257: see k_beam_part);
-// few are done sooner in small ones.
-static int beam_pieces(int rows, int V) { return (long)rows * (V / 8) >= 256L * 6000 ? BEAM_MANY : BEAM_FEW; }
-static int beam_parts(int rows, int V) { return V < 8 ? 1 : cdiv(V / 8, 256 * beam_pieces(rows, V)); }
+static int beam_parts(int V) { return V < 8 ? 1 : cdiv(V / 8, 256 * BEAM_PIECES); }
 
 }  // namespace g2
 
@@ -257,7 +289,7 @@ using namespace g2;
 
 extern "C" size_t gpt2_beam_select_ws(int groups, int beams, int V) {
     if (groups < 1 || beams < 1 || V < 1 || (long)groups * beams > 65535) return 16;
-    return (size_t)groups * beams * beam_parts(groups * beams, V) * sizeof(BeamPart);
+    return (size_t)groups * beams * beam_parts(V) * sizeof(BeamPart);
 }
 
 extern "C" void gpt2_beam_select(int *token, int *parent, float *score_out, int *done_out, const gpt2_half *logits, long ld,
@@ -275,12 +307,10 @@ extern "C" void gpt2_beam_select(int *token, int *parent, float *score_out, int 
         arg_fail("gpt2_beam_select: workspace too small or unaligned");
         return;
     }
-    const int rows = groups * beams, parts = beam_parts(rows, V);
+    const int rows = groups * beams, parts = beam_parts(V);
     BeamPart *part = (BeamPart *)ws;
-    const auto fn = beam_pieces(rows, V) == BEAM_MANY ? k_beam_part<BEAM_MANY> : k_beam_part<BEAM_FEW>;
-    hipLaunchKernelGGL(fn, dim3(parts, rows), dim3(256), 0, stream(), part, logits, ld, V, beams, parts);
-    const auto join = parts <= 4 ? k_beam_join<1> : parts <= 8 ? k_beam_join<2> : k_beam_join<4>;
-    hipLaunchKernelGGL(join, dim3(groups), dim3(64 * beams), 0, stream(), token, parent, score_out, done_out, part, score, done,
+    hipLaunchKernelGGL(k_beam_part, dim3(parts, rows), dim3(256), 0, stream(), part, logits, ld, V, beams, parts);
+    hipLaunchKernelGGL(k_beam_join, dim3(groups), dim3(64 * beams), 0, stream(), token, parent, score_out, done_out, part, score, done,
                        beams, V, eos, parts);
     check_launch("k_beam_select");
 }

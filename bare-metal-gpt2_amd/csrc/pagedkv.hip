@@ -751,7 +751,8 @@ extern "C" void gpt2_pkv_fork(GPT2PagedKV *c, const int *parent) {
 
 extern "C" void gpt2_pkv_compact(GPT2PagedKV *c) {
     if (pkv_refused(c, "gpt2_pkv_compact: bad cache")) return;
-    const int copiers = 2048;
+    const long units = (long)(c->nPages / 2) * ((2 * c->nHead + 7) / 8) * c->nLayer;   // at most: as many holes as movers
+    const int copiers = (int)(units < 2048 ? units : 2048);
     hipLaunchKernelGGL(k_pkv_compact_plan, dim3(1), dim3(1024), 0, stream(), *c);
     hipLaunchKernelGGL(k_pkv_compact, dim3(copiers + cdiv((long)c->nSeq * c->maxPages, 256)), dim3(256), 0, stream(), *c, copiers);
     check_launch("k_pkv_compact");
