@@ -3,7 +3,10 @@
 //
 // score_b + x - m_b - log(sum_b) orders a row's tokens as its logits do, so a row's candidates are its best `beams` logits:
 // one pass over the logits takes each part of a row's maximum, its sum of exponentials and its best, and a second launch, a
-// work-group a group, joins the parts and merges the rows' lists of candidates in fp64.  Bound by reading the logits once.
+// work-group a group, joins the parts and merges the rows' lists of candidates in fp64.  64 groups of
+// 8 rows of 50257 take 18.5 us (2.8 TB/s) and 5.3; 512 groups of one row, which need no bounds, 15: instructions, some 14 a pair of
+// logits and the bounds and sums of every wave, take longer than the reading (10 us).  Four rows take 5.0 and 3.6, the latency of
+// two short launches.
 //
 // A logit and its token are one 32-bit key, (logit's bits in order) << 16 | (65535 - token): keys of a row are unique, and
 // the larger key is the larger logit or, of equal ones, the lower token.  0 is no key.

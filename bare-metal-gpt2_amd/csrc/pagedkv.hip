@@ -72,8 +72,8 @@ __global__ void k_pkv_reset(GPT2PagedKV c) {
 // ------------------------------------------------------------------ grow
 // One work-group: needs and their sums over the sequences, then a walk over refs that hands the lowest free pages out in
 // order, which stops when enough are found (its first step is under way meanwhile); tables, refs and lengths are written once they
-// are.  Bound by the latency of its few dependent
-// loads and barriers: T = 256 threads where they are enough (48 sequences, one of them needing a page: see DESIGN.md's table).
+// are.  Bound by the latency of its few dependent loads and barriers: 4.3 us for 48 sequences with T = 256 threads, 5.4 with 1024; where
+// hundreds of pages are handed out (48 prompts of up to 1000 rows) 6.8 and 6.1.
 template <int T>
 __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
     constexpr int NW = T / 64, PER = GPT2_PKV_MAX_SEQ / 1024, FREE = 8;
@@ -276,7 +276,8 @@ __device__ __forceinline__ int pkv_append_units(const PkvSeq &q) {
 }
 
 // One wave per unit, K|V and head: whole row pieces in, 16 bytes a lane, the tile's maximum over the wave, 8 bytes of codes a
-// lane and store, 512 contiguous.
+// lane and store, 512 contiguous.  48 prompts of 250 to 1000 rows: 34 to 40 us, 4.1 to 3.4 TB/s of rows in and codes out (a row's
+// piece of a head is 128 bytes, every 4.5 KB); a decode step's 48 rows 6.4 us, its chain of loads and the code's own way from memory.
 __device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, const uint16_t *__restrict__ qkv, const PkvSeq &q,
                                                 int seq, int u, int kv, int h, char *lds) {
     const int lane = threadIdx.x & 63;
@@ -287,17 +288,20 @@ __device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, con
     uint32_t d[16];
     if (had + u < full) {
         const int page = c.table[(size_t)seq * c.maxPages + had + u], kept = u ? 0 : q.start % PKV_P;
+        i32x4 old[4] = {};   // the open page's tokens from before the call, under way with the rows
+        if (kept)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) old[i] = *reinterpret_cast<const i32x4 *>(open + 8 * (64 * i + lane));
         pkv_load_rows(src, 3 * (size_t)E, (had + u) * PKV_P, q, d);
         if (kv) pkv_by_dims(d, lds);
-        if (kept) {   // the open page's tokens from before the call
+        if (kept) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const i32x4 v = *reinterpret_cast<const i32x4 *>(open + 8 * (64 * i + lane));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int n = kv ? kept - (8 * i + 2 * j) : kept > 8 * i + (lane >> 3) ? 2 : 0;   // of the pair, how many
                     const uint32_t keep = n >= 2 ? ~0u : n == 1 ? 0xffffu : 0u;
-                    d[4 * i + j] = ((uint32_t)v[j] & keep) | (d[4 * i + j] & ~keep);
+                    d[4 * i + j] = ((uint32_t)old[i][j] & keep) | (d[4 * i + j] & ~keep);
                 }
             }
         }
@@ -356,7 +360,7 @@ __global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const 
 
 // ------------------------------------------------------------------ read
 // A unit is a page that the rows of a sequence touch; a wave takes one K|V and head of it: the tile in its own order,
-// 8 values a lane and piece, V through LDS to rows, 16-byte stores.
+// 8 values a lane and piece, V through LDS to rows, 16-byte stores.  Bound by memory: 46 MB of codes to 92 MB of rows in 26 us, 5.3 TB/s.
 struct PkvRead {
     long pos;        // of the sequence's first row
     int row0, n;
@@ -427,15 +431,17 @@ __global__ __launch_bounds__(256) void k_pkv_read(uint16_t *__restrict__ out, GP
 }
 
 // ------------------------------------------------------------------ fork
-// First launch: work-group s < nSeq stages sequence s's page table and settles its pages' counts by its children; the last
-// one settles the open pages: a parent's first child keeps its slot, the others (and empty ones) take, in order, the slots of the
+// First launch: work-group 1 + s stages sequence s's page table and settles its pages' counts by its children; the first, which
+// takes longest, settles the open pages: a parent's first child keeps its slot, the others (and empty ones) take, in order, the slots of the
 // sequences without a child, of which there are as many.
 __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int *__restrict__ parent) {
-    __shared__ int lds[4], children[GPT2_PKV_MAX_SEQ], first[GPT2_PKV_MAX_SEQ], spare[GPT2_PKV_MAX_SEQ];
-    const int tid = threadIdx.x, me = blockIdx.x;
+    // the books are read once, all of them under way together; what follows is in LDS
+    __shared__ int lds[4], par[GPT2_PKV_MAX_SEQ], len[GPT2_PKV_MAX_SEQ], slot[GPT2_PKV_MAX_SEQ], first[GPT2_PKV_MAX_SEQ], spare[GPT2_PKV_MAX_SEQ];
+    const int tid = threadIdx.x, me = (int)blockIdx.x - 1;
     const PkvPlan plan = pkv_plan(c);
     bool bad = false;
-    if (me < c.nSeq) {
+    if (me >= 0) {
+        const int full = min(c.len[me] / PKV_P, c.maxPages);
         int mine = 0;
         for (int i = tid; i < c.nSeq; i += 256) {
             const int p = parent[i];
@@ -445,7 +451,6 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
         if (__syncthreads_or(bad)) return;
         int n;
         block_scan<4>(mine, lds, n);
-        const int full = min(c.len[me] / PKV_P, c.maxPages);
         for (int t = tid; t < full; t += 256) {
             const int page = c.table[(size_t)me * c.maxPages + t];
             plan.tables[(size_t)me * c.maxPages + t] = page;
@@ -453,18 +458,18 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
         }
         return;
     }
+#pragma nounroll
     for (int i = tid; i < c.nSeq; i += 256) {
-        children[i] = 0;
-        first[i] = c.nSeq;
+        par[i] = parent[i];
+        len[i] = c.len[i];
+        slot[i] = c.slot[i];
+        first[i] = c.nSeq;   // no child
     }
     __syncthreads();
     for (int i = tid; i < c.nSeq; i += 256) {
-        const int p = parent[i];
+        const int p = par[i];
         if (p < -1 || p >= c.nSeq) bad = true;
-        else if (p >= 0) {
-            atomicAdd(children + p, 1);
-            atomicMin(first + p, i);
-        }
+        else if (p >= 0) atomicMin(first + p, i);
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) {
@@ -474,34 +479,37 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
     if (bad) return;
     const int per = (c.nSeq + 255) / 256, i0 = min(tid * per, c.nSeq), i1 = min(i0 + per, c.nSeq);
     int n = 0, total;
-    for (int i = i0; i < i1; ++i) n += children[i] == 0;
+    for (int i = i0; i < i1; ++i) n += first[i] == c.nSeq;
     int k = block_scan<4>(n, lds, total);
     for (int i = i0; i < i1; ++i)
-        if (children[i] == 0) spare[k++] = c.slot[i];
+        if (first[i] == c.nSeq) spare[k++] = slot[i];
     n = 0;
-    for (int i = i0; i < i1; ++i) n += parent[i] < 0 || first[parent[i]] != i;
+    for (int i = i0; i < i1; ++i) n += par[i] < 0 || first[par[i]] != i;
     k = block_scan<4>(n, lds, total);   // its barriers order spare's writes before the reads below
     for (int i = i0; i < i1; ++i) {
-        const int p = parent[i];
+        const int p = par[i];
         const bool heir = p >= 0 && first[p] == i;
-        plan.len[i] = p >= 0 ? c.len[p] : 0;
-        plan.slot[i] = heir ? c.slot[p] : spare[k++];
-        plan.from[i] = heir || p < 0 ? -1 : c.slot[p];
+        plan.len[i] = p >= 0 ? len[p] : 0;
+        plan.slot[i] = heir ? slot[p] : spare[k++];
+        plan.from[i] = heir || p < 0 ? -1 : slot[p];
     }
 }
 
-// Second launch: blockIdx.y 0 the books, then the open page of sequence blockIdx.x, a layer's K or V each, only the tokens in
-// it.  A thread copies piece `tid` (16 bytes) of every head's tile, four heads under way; of a V tile's octet that the tokens end
-// in, it puts those that are there among what was.
+// Second launch: blockIdx.y 0 the books, then the open page of sequence blockIdx.x, a layer's K or V and four heads each, only the
+// tokens in it.  A thread copies piece `tid` (16 bytes) of the four tiles, all under way together; of a V tile's octet that the tokens
+// end in, it puts those that are there among what was.  32 prompts of 8 beams, all layers: 151 MB that have to move in
+// 35 us (42 where nothing is in a cache yet: 3.6 TB/s, 4.3 with the rest of those octets); a work-group for all the heads took 36.6
+// (44), and for one prompt's four beams 4.0 us, 3.4 here.
 __global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__restrict__ parent) {
     const int me = blockIdx.x, tid = threadIdx.x;
     const PkvPlan plan = pkv_plan(c);
     if (!plan.word[1]) {
-        if (blockIdx.y == 0 && tid == 0) c.start[me] = c.len[me];
+        if (blockIdx.y == 0 && blockIdx.z == 0 && tid == 0) c.start[me] = c.len[me];
         return;
     }
     const int p = parent[me], len = plan.len[me];
     if (blockIdx.y == 0) {
+        if (blockIdx.z) return;
         if (tid == 0) {
             c.len[me] = c.start[me] = len;
             c.slot[me] = plan.slot[me];
@@ -521,17 +529,16 @@ __global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__re
     for (int e = 0; e < 4; ++e) keep[e] = n >= 2 * e + 2 ? -1 : n == 2 * e + 1 ? 0xffff : 0;
     const i32x4 *src = reinterpret_cast<const i32x4 *>(c.open + pkv_tile(c, c.nSeq, L, from, kv, 0) * PKV_TILE) + tid;
     i32x4 *dst = reinterpret_cast<i32x4 *>(c.open + pkv_tile(c, c.nSeq, L, to, kv, 0) * PKV_TILE) + tid;
-    for (int h = 0; h < c.nHead; h += 4) {
-        i32x4 v[4];
+    const int h = 4 * blockIdx.z;
+    i32x4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = src[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)];
-        if (n < 8)
+    for (int i = 0; i < 4; ++i) v[i] = src[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)];
+    if (n < 8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (v[i] & keep) | (dst[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)] & ~keep);
+        for (int i = 0; i < 4; ++i) v[i] = (v[i] & keep) | (dst[(size_t)min(h + i, c.nHead - 1) * (PKV_TILE / 8)] & ~keep);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (h + i < c.nHead) dst[(size_t)(h + i) * (PKV_TILE / 8)] = v[i];
-    }
+    for (int i = 0; i < 4; ++i)
+        if (h + i < c.nHead) dst[(size_t)(h + i) * (PKV_TILE / 8)] = v[i];
 }
 
 // ------------------------------------------------------------------ compact
@@ -582,7 +589,7 @@ __global__ __launch_bounds__(1024) void k_pkv_compact_plan(GPT2PagedKV c) {
 }
 
 // Second launch: the first `copiers` work-groups move pages (a unit is eight tiles of one layer, and their scales), the
-// others renumber the page tables.
+// others renumber the page tables.  Bound by memory: 373 pages of 12 layers, 441 MB in and out, in 92 us, 4.8 TB/s.
 __global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers) {
     const int tid = threadIdx.x;
     const PkvPlan plan = pkv_plan(c);
@@ -745,7 +752,7 @@ extern "C" void gpt2_pkv_fork(GPT2PagedKV *c, const int *parent) {
     if (pkv_refused(c, "gpt2_pkv_fork: bad cache")) return;
     if (!parent || ((uintptr_t)parent & 3)) { arg_fail("gpt2_pkv_fork: null/unaligned"); return; }
     hipLaunchKernelGGL(k_pkv_fork_plan, dim3(c->nSeq + 1), dim3(256), 0, stream(), *c, parent);
-    hipLaunchKernelGGL(k_pkv_fork, dim3(c->nSeq, 1 + 2 * c->nLayer), dim3(256), 0, stream(), *c, parent);
+    hipLaunchKernelGGL(k_pkv_fork, dim3(c->nSeq, 1 + 2 * c->nLayer, cdiv(c->nHead, 4)), dim3(256), 0, stream(), *c, parent);
     check_launch("k_pkv_fork");
 }
 
