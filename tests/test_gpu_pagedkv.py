@@ -392,3 +392,30 @@ def test_embed_positions(pkg, L):
             for i, q in zip(ids, pos)]
     np.testing.assert_array_equal(got[:8], np.stack(want))
     assert (got[8:] == 7).all()
+
+
+@pytest.mark.parametrize("heads,before,counts,group", [
+    (3, [96, 70, 130, 0], [1, 1, 1, 1], 1), (3, [96, 70, 130, 0], [1, 1, 1, 1], 4), (3, [96, 40], [20, 30], 1), (3, [96], [90], 1),
+    (1030, [64], [130], 1),
+])
+def test_attention_pages_of_zeros(pkg, L, heads, before, counts, group):
+    """Pages whose keys or values are all zero, whose scale says nothing of their size: keys that weigh the same exactly, values that
+    add nothing to others a thousand times smaller than the queries; one head's values are all zero, and so is what it gives."""
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=30, seqs=len(counts), max_len=256), np.random.default_rng(36)
+    E = heads * D
+    for step in (before, counts):
+        assert p.grow(step)
+        x = qkv_of(rng, p.n, heads)
+        x[:, :E] *= np.float16(6)
+        kv = x[:, E:].reshape(-1, 2, heads, D)
+        kv[:, 1] *= np.float16(2 ** -10)
+        kv[:, 1, 1 % heads] = 0
+        for s in range(len(counts)):   # the first 40 tokens
+            rows = kv[p.rows[s]:p.rows[s + 1]]
+            rows[:max(0, 40 - int(p.r.start[s])), 0, 0] = 0
+            rows[:max(0, 40 - int(p.r.start[s])), 1, heads - 1] = 0
+        p.append(0, x)
+    p.same()
+    p.check_attention(0, x, group=group)
+    got = p.attend(0, x, group=group).reshape(-1, heads, D)
+    assert (got[:, 1 % heads] == 0).all()
