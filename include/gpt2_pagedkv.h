@@ -91,7 +91,8 @@ void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, const int *row
 /* att[row] = softmax(q . k / 8) v over the tokens up to the row's own, from the cache.  `group`: 1, or how many
  * consecutive sequences (at most 16) are beams of one prompt: the leading pages that all of a group share are then
  * read once for its one-row sequences; results are the same but for the order of sums.  ws: at least gpt2_pkv_attn_ws
- * bytes of device memory, 16-byte aligned, with no meaning between calls; calls that may overlap need one each. */
+ * bytes of device memory, 16-byte aligned, with no meaning between calls; calls that may overlap need one each.  More rows may need
+ * less (they are split less): a workspace for calls of several sizes has the largest of theirs. */
 size_t gpt2_pkv_attn_ws(const GPT2PagedKV *c, int nRows);
 void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2PagedKV *c, int L, const int *rows, int nRows,
                    int group, void *ws, size_t wsBytes);
