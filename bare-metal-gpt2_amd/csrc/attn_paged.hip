@@ -413,15 +413,16 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
     return {seq0 + one, __builtin_amdgcn_readlane(s.len, one), 0, shared, total, a.group, seq0 + min(lane, a.group - 1), s.len, s.slot, sum - own};
 }
 
-// One row a sequence, nearly always (no more rows than sequences): a work-group per sequence, head and split ...
+// One row a sequence, nearly always (no more rows than sequences): a work-group per sequence, head and split (gridDim.z of them, for
+// sequences that have more than 16 rows after all) ...
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) AttnLds<W, 1> lds;
     const int h = blockIdx.x % a.c.nHead, seq = blockIdx.x / a.c.nHead;
     const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
 #pragma nounroll
-    for (int rb = 0; 16 * rb < s.n; ++rb) {
-        if (rb) __syncthreads();
+    for (int rb = blockIdx.z; 16 * rb < s.n; rb += gridDim.z) {
+        if (rb >= (int)gridDim.z) __syncthreads();
         AttnCols<1> col;
         const AttnSteps st = attn_rows(s, seq, rb, col);
         attn_pass<W, false, 1>(a, st, h, blockIdx.y, col, lds);
@@ -658,7 +659,9 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
 }
 
 // How a call runs: its form, and how the steps are split over work-groups: at least `per` of them each, into `splits` at most.
-//   ONE    no more rows than sequences: a sequence (or group of beams) a work-group.
+//   ONE    no more rows than sequences: a sequence (or group of beams) a work-group.  Without a group up to 4 of them take turns at the
+//          16-row blocks of a sequence that has a whole prompt: 200 rows after 800 tokens, 256 sequences in the cache, 77 us with one, 42 with
+//          two, 30 with four; 256 single rows 24.5, 24.0, 25.8.
 //   ROWS1  16 rows a work-group, keys split over its waves.
 //   ROWS2  32 of them, from 32 rows a sequence on: a page is made fp16 once for twice the rows (a prompt of 1000 rows 12 us; 19 with BLOCK).
 //   BLOCK  64, pages shared through LDS, where that makes eight work-groups a CU: 32 prompts of up to 1000 rows 85 us, 104 with
@@ -669,7 +672,7 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
 enum AttnForm { ATTN_ONE, ATTN_ROWS1, ATTN_ROWS2, ATTN_BLOCK };
 struct AttnPlan {
     AttnForm form;
-    int groups, splits, per;   // work-groups of a split
+    int groups, splits, per, deep;   // work-groups of a split; deep: times as many, where a sequence may have many rows
 };
 static AttnPlan attn_plan(const GPT2PagedKV *c, int nRows, int group) {
     AttnPlan p;
@@ -678,6 +681,7 @@ static AttnPlan attn_plan(const GPT2PagedKV *c, int nRows, int group) {
     p.groups = (p.form == ATTN_ONE ? c->nSeq / group : nRows / rows + c->nSeq) * c->nHead;
     p.splits = 1;
     p.per = 64;
+    p.deep = p.form == ATTN_ONE && group == 1 ? min(cdiv(nRows, 16), p.groups < 2048 ? 4 : 2) : 1;
     const long busy = (long)(p.form == ATTN_ONE ? c->nSeq : nRows / rows + 1) * c->nHead;   // work-groups with something to do, about
     if (p.form == ATTN_BLOCK || c->maxPages <= 64 || (p.form != ATTN_ONE && busy >= 512)) return p;
     if (busy * (c->maxPages / 64) < 512) p.per = 16;
@@ -723,7 +727,7 @@ extern "C" void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2Pa
                     : group > 1            ? (wide ? k_pkv_attn_beams<8> : k_pkv_attn_beams<4>)
                     : wide                 ? k_pkv_attn_one<8>
                                            : k_pkv_attn_one<4>;
-    hipLaunchKernelGGL(fn, dim3(p.groups, p.splits), dim3(wide ? 512 : 256), 0, stream(), a);
+    hipLaunchKernelGGL(fn, dim3(p.groups, p.splits, p.deep), dim3(wide ? 512 : 256), 0, stream(), a);
     if (a.splits > 1) {
         const bool by_seq = p.form == ATTN_ONE;
         hipLaunchKernelGGL(by_seq ? k_pkv_attn_join<true> : k_pkv_attn_join<false>, dim3(by_seq ? c->nSeq : nRows, cdiv(c->nHead, 4)), dim3(256), 0,

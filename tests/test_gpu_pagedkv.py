@@ -419,3 +419,17 @@ def test_attention_pages_of_zeros(pkg, L, heads, before, counts, group):
     p.check_attention(0, x, group=group)
     got = p.attend(0, x, group=group).reshape(-1, heads, D)
     assert (got[:, 1 % heads] == 0).all()
+
+
+@pytest.mark.parametrize("max_len,group", [(320, 1), (4000, 1), (320, 4)])
+def test_prompts_in_a_cache_of_many_sequences(pkg, L, max_len, group):
+    """No more rows than sequences, but nearly all of them one sequence's: its rows and pages are shared out."""
+    p, rng = Pair(pkg, L, layers=1, heads=3, pages=60, seqs=140, max_len=max_len), np.random.default_rng(37)
+    counts = np.zeros(140, int)
+    for before, new in ((40, 100), (3, 130)):
+        counts[[3, 50, 99]] = [before, 33, 5]
+        p.step(rng, counts)
+        counts[[3, 50, 99]] = [new, 5, 2]
+        x = p.step(rng, counts)
+        p.same()
+        p.check_attention(0, x[0], group=group, extra=2)
