@@ -435,8 +435,11 @@ __global__ __launch_bounds__(256) void k_pkv_read(uint16_t *__restrict__ out, GP
 // takes longest, settles the open pages: a parent's first child keeps its slot, the others (and empty ones) take, in order, the slots of the
 // sequences without a child, of which there are as many.
 __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int *__restrict__ parent) {
-    // the books are read once, all of them under way together; what follows is in LDS
-    __shared__ int lds[4], par[GPT2_PKV_MAX_SEQ], len[GPT2_PKV_MAX_SEQ], slot[GPT2_PKV_MAX_SEQ], first[GPT2_PKV_MAX_SEQ], spare[GPT2_PKV_MAX_SEQ];
+    // the books are read once, all of them under way together; what follows is in LDS (sequences and slots in 16 bits: every
+    // work-group of the launch takes this much of it)
+    __shared__ int lds[4], len[GPT2_PKV_MAX_SEQ], first[GPT2_PKV_MAX_SEQ];
+    __shared__ short par[GPT2_PKV_MAX_SEQ], slot[GPT2_PKV_MAX_SEQ], spare[GPT2_PKV_MAX_SEQ];
+    static_assert(GPT2_PKV_MAX_SEQ < 32768, "16 bits");
     const int tid = threadIdx.x, me = (int)blockIdx.x - 1;
     const PkvPlan plan = pkv_plan(c);
     bool bad = false;
@@ -460,16 +463,12 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
     }
 #pragma nounroll
     for (int i = tid; i < c.nSeq; i += 256) {
-        par[i] = parent[i];
+        const int p = parent[i], at = c.slot[i];
+        bad |= p < -1 || p >= c.nSeq;
+        par[i] = (short)p;
         len[i] = c.len[i];
-        slot[i] = c.slot[i];
+        slot[i] = (short)((unsigned)at < (unsigned)c.nSeq ? at : -1);   // one that is none stays so
         first[i] = c.nSeq;   // no child
-    }
-    __syncthreads();
-    for (int i = tid; i < c.nSeq; i += 256) {
-        const int p = par[i];
-        if (p < -1 || p >= c.nSeq) bad = true;
-        else if (p >= 0) atomicMin(first + p, i);
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) {
@@ -477,6 +476,9 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
         if (bad) atomicCAS(c.status, 0, E_ARG);
     }
     if (bad) return;
+    for (int i = tid; i < c.nSeq; i += 256)
+        if (par[i] >= 0) atomicMin(first + par[i], i);
+    __syncthreads();
     const int per = (c.nSeq + 255) / 256, i0 = min(tid * per, c.nSeq), i1 = min(i0 + per, c.nSeq);
     int n = 0, total;
     for (int i = i0; i < i1; ++i) n += first[i] == c.nSeq;
