@@ -667,8 +667,10 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
 //   BLOCK  64, pages shared through LDS, where that makes eight work-groups a CU: 32 prompts of up to 1000 rows 85 us, 104 with
 //          ROWS2; 8 of up to 600 over 2000 tokens 64 us, 58 with ROWS2.
 // No splits for caches whose sequences a work-group's waves get through in the time of a second launch, nor where the rows alone
-// make enough work-groups.  Where splits of 64 pages fill the card they stream best (16 contexts up to 16384 tokens: 51 us, 59 with 16
-// pages each); fewer sequences need smaller ones (one of 16384: 8.6 us, 14).
+// make one work-group a CU (8 prompts of up to 200 rows over up to 2000 tokens: 26 us, 26 + 7 with two splits).  Where splits of 64
+// pages fill the card they stream best (16 contexts up to 16384 tokens: 48.7 us, 49.9 with 32 pages each, 55.4 with 96); with fewer
+// sequences, or groups of beams, as many as make 512 work-groups, of 16 pages at least (8 x 8 beams over 2100 tokens: 5 splits 11.2 us,
+// 2 splits 17.6, 9 splits 13.8; over 4096: 5 15.8, 2 19.0, 8 18.7).
 enum AttnForm { ATTN_ONE, ATTN_ROWS1, ATTN_ROWS2, ATTN_BLOCK };
 struct AttnPlan {
     AttnForm form;
@@ -682,9 +684,10 @@ static AttnPlan attn_plan(const GPT2PagedKV *c, int nRows, int group) {
     p.splits = 1;
     p.per = 64;
     p.deep = p.form == ATTN_ONE && group == 1 ? min(cdiv(nRows, 16), p.groups < 2048 ? 4 : 2) : 1;
-    const long busy = (long)(p.form == ATTN_ONE ? c->nSeq : nRows / rows + 1) * c->nHead;   // work-groups with something to do, about
-    if (p.form == ATTN_BLOCK || c->maxPages <= 64 || (p.form != ATTN_ONE && busy >= 512)) return p;
-    if (busy * (c->maxPages / 64) < 512) p.per = 16;
+    const long busy = (long)(p.form == ATTN_ONE ? c->nSeq / group : nRows / rows + 1) * c->nHead;   // work-groups with something to do, about
+    if (p.form == ATTN_BLOCK || c->maxPages <= 64 || (p.form != ATTN_ONE && busy > 256)) return p;
+    const long share = 512 / max(busy, 1L);   // splits that fill the card
+    p.per = min(64, max(16, share > 0 ? cdiv(c->maxPages, (int)share) : 64));
     p.splits = cdiv(c->maxPages, p.per);
     if (p.splits > ATTN_SPLITS) p.splits = ATTN_SPLITS;
     return p;
@@ -696,7 +699,7 @@ using namespace g2;
 
 extern "C" size_t gpt2_pkv_attn_ws(const GPT2PagedKV *c, int nRows) {
     if (!c || nRows < 1 || c->nHead < 1 || c->maxPages < 1) return 16;
-    const int n = attn_plan(c, nRows, 1).splits;   // the same for any group
+    const int n = attn_plan(c, nRows, 16).splits;   // the most that any group has
     return n == 1 ? 16 : (size_t)n * nRows * c->nHead * (PKV_D + 4) * 4;
 }
 

@@ -187,6 +187,7 @@ def test_attention_many_sequences(pkg, L):
     (1024, [40, 0], [100, 33]),
     (700, [33], [200]),
     (1, [33, 1], [400, 100]),
+    (2, [2100, 5], [300, 40]),
 ])
 def test_attention_many_rows(pkg, L, heads, before, counts):
     """Batches of many rows a sequence, which take work-groups of 32 and of 64 rows, with splits and without: prompts from
