@@ -328,3 +328,59 @@ def test_pages_past_4_gib(pkg, L, new):
     read_back()
     assert int(small.download(pkg, big, "table")[0, 0]) < 12
     big.free()
+
+
+def test_one_cache_read_on_two_streams(pkg, L):
+    """Attention and reads of one cache on two streams at once, a workspace each, a split form among them: the bits of one alone."""
+    hip = hip_runtime()
+    p, rng = Pair(pkg, L, layers=1, heads=4, pages=260, seqs=3, max_len=6000), np.random.default_rng(38)
+    p.step(rng, [4100, 300, 2000])
+    x = p.step(rng, [1, 1, 1])[0]
+    p.check_attention(0, x)
+    want = p.attend(0, x)
+    n = len(x)
+    atts, outs = [pkg.Dev(n * 4 * D * 2) for _ in range(4)], [pkg.Dev(200 * 2 * 4 * D * 2) for _ in range(4)]
+    need = L.gpt2_pkv_attn_ws(ref(p.c), n)
+    assert need > 16
+    ws = [Ws(pkg, need) for _ in range(2)]
+    d_rows, first = pkg.Dev.from_numpy(np.array([0, 150, 150, 200], np.int32)), pkg.Dev.from_numpy(np.array([3900, 0, 1960], np.int32))
+    d_x = pkg.Dev.from_numpy(x)
+    L.gpt2_sync()
+    streams = [C.c_void_p(), C.c_void_p()]
+    try:
+        for st in streams:
+            assert hip.hipStreamCreate(C.byref(st)) == 0
+        for i in range(4):
+            L.gpt2_set_stream(streams[i % 2])
+            L.gpt2_pkv_attn(atts[i].ptr, d_x.ptr, ref(p.c), 0, p.d_rows.ptr, n, 1, *ws[i % 2].args)
+            L.gpt2_pkv_read(outs[i].ptr, ref(p.c), 0, d_rows.ptr, first.ptr, 200)
+        for st in streams:
+            assert hip.hipStreamSynchronize(st) == 0
+    finally:
+        L.gpt2_set_stream(None)
+        for st in streams:
+            if st:
+                hip.hipStreamDestroy(st)
+    pkg.check("two streams")
+    back = np.concatenate([p.r.read(0, 0, 3900, 150), p.r.read(0, 2, 1960, 50)]).view(np.uint16)
+    for a, o in zip(atts, outs):
+        np.testing.assert_array_equal(a.numpy(np.float16, want.shape), want)
+        np.testing.assert_array_equal(o.numpy(np.uint16, back.shape), back)
+
+
+def test_most_sequences(pkg, L):
+    """As many sequences as there may be: pages handed out, forked, freed and packed."""
+    rng = np.random.default_rng(39)
+    p = Pair(pkg, L, layers=1, heads=1, pages=5000, seqs=4096, max_len=96)
+    p.step(rng, rng.integers(0, 40, 4096))
+    p.same()
+    p.fork(rng.integers(-1, 4096, 4096))
+    p.same()
+    x = p.step(rng, (rng.random(4096) < 0.6).astype(int))
+    L.gpt2_pkv_compact(ref(p.c))
+    p.r.compact()
+    p.same()
+    p.check_attention(0, x[0])
+    p.fork(np.where(np.arange(4096) < 4000, -1, np.arange(4096)))
+    p.same()
+    assert L.gpt2_pkv_status(ref(p.c)) == 0
