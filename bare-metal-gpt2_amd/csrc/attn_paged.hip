@@ -34,7 +34,7 @@ struct PageRaw {
 };
 
 // Attention of 16 rows as it accumulates: column jq is a row; o[2 i + b] element r is dim 32 i + 8 g + 2 r + b.
-// m: the running maximum of x; l: the sum of the weights (in every element); o: the weighted sum of the values.
+// m: the running maximum of x; l: the sum of the weights (in every element); o: the weighted sum of the values (both lifted).
 struct AttnAcc {
     float m;
     f32x4 l, o[4];
@@ -83,6 +83,7 @@ struct PageFrag {
 // compiler does not see what `inf` is, or it would make a maximum of it.
 __device__ __forceinline__ float max_by(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
+constexpr float ATTN_LIFT = 15.f;
 // N pages against Q times 16 columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it
 // where few waves share a SIMD, and two pages go down it in little more than the time of one.  Column jq sees keys below lim.
 template <int N, int Q>
@@ -134,16 +135,45 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
             for (int i = 0; i < 4; ++i) A[u].o[i] *= corr;
         }
     }
-    // The weights are rounded to fp16, which costs an output about as much as its own rounding (1.2e-4 of it against
+    // The weights are held 2^ATTN_LIFT times as large, the largest at 2^15, so that the many small ones of a long context stay above
+    // what fp16 rounds to fewer bits (2^-29 of the largest) or to nothing (2^-40).
+    // They are rounded to fp16, which costs an output about as much as its own rounding (1.2e-4 of it against
     // 2.1e-4; with s_v in them, so that P.V could add to o in the product, 2e-4: the largest weight is then no longer 1 exactly,
     // and it was no faster).
     f16x8 p[Q][N];
+    float lift[Q], rate[N];
+    bool huge = false;
+#pragma unroll
+    for (int n = 0; n < N; ++n) rate[n] = scale[n];
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+        lift[u] = ATTN_LIFT - base[u];
+        huge |= fabsf(base[u]) >= 0x1p20f;
+    }
+    if (__ballot(huge)) {
+        // The maximum is a rounded product and x an exact one, which may pass it by 2^-24 of its size: by so much that fp16 could
+        // overflow.  Here x is the rounded product, too.
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int u = 0; u < Q; ++u) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = s[u][n][e] * scale[n];
+                    s[u][n][e] = x - base[u];
+                }
+            lift[u] = ATTN_LIFT;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) rate[n] = 1.f;
+    }
 #pragma unroll
     for (int u = 0; u < Q; ++u)
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[u][n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[u][n][e], scale[n], -base[u]));
+            for (int e = 0; e < 8; ++e) p[u][n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[u][n][e], rate[n], lift[u]));
     // their sum, of the fp16 values as they are multiplied, on the matrix units too: a row of ones
     const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll

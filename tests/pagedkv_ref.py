@@ -131,12 +131,12 @@ class Ref:
                 out[rows[s] + i] = (np.einsum("ht,htd->hd", w, vv) / np.where(tot == 0, 1, tot)).reshape(-1)
                 on[rows[s] + i] = True
                 # Weights rounded to fp16, half a step 2^-11 each against the average they form (2 vmax), those below
-                # 2^-14 by 2^-25 each; scores' sums of 64 fp32 products (each half a step 2^-24 of the running sum, at
+                # 2^-29 of the largest by 2^-40 each; scores' sums of 64 fp32 products (each half a step 2^-24 of the running sum, at
                 # most S = sum |q k| / 8, times 64, and the weight by as much, on both sides of the average); the output's own
                 # rounding, 2^-11 of at most vmax (and 2^-25 when subnormal).
                 vmax = np.abs(vv).max(axis=(1, 2))
                 S = (np.abs(q)[:, None] * np.abs(np.nan_to_num(k[:, :vis]))).sum(axis=2).max(axis=1) / 8
-                t = vmax * (2 * 2.0 ** -11 + vis * 2.0 ** -25 * 2 + 2 * (64 + 4) * 2.0 ** -24 * (S + 1) + 2.0 ** -11) + 2.0 ** -25
+                t = vmax * (2 * 2.0 ** -11 + vis * 2.0 ** -40 * 2 + 2 * (64 + 4) * 2.0 ** -24 * (S + 1) + 2.0 ** -11) + 2.0 ** -25
                 tol[rows[s] + i] = np.repeat(t, D)
         return out, tol, on
 

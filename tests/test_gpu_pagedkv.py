@@ -434,3 +434,52 @@ def test_prompts_in_a_cache_of_many_sequences(pkg, L, max_len, group):
         x = p.step(rng, counts)
         p.same()
         p.check_attention(0, x[0], group=group, extra=2)
+
+
+@pytest.mark.parametrize("rows,group", [(1, 1), (1, 2), (30, 1), (100, 1)])
+def test_attention_many_small_weights(pkg, L, rows, group):
+    """One key far ahead of thousands whose weights add up all the same: 2^-19 to 2^-23 of the largest each."""
+    heads, cached = 2, 5000
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=420, seqs=2, max_len=6000), np.random.default_rng(40)
+    E = heads * D
+    for counts in ([cached, 70], [rows, 1]):
+        assert p.grow(counts)
+        x = np.zeros((p.n, 3, heads, D), np.float16)
+        x[:, 0, :, 0] = 8          # q . k / 8 is the key's first dim
+        x[:, 1, :, 0] = -np.log(2) * (19 + 4 * rng.random((p.n, heads)))
+        x[:, 2] = 1 + rng.random((p.n, heads, D))
+        if counts[0] == cached:    # the one key, with a value of its own
+            x[17, 1, :, 0], x[17, 2] = 0, -1
+            x[cached, 1, :, 0] = 0
+        x = x.reshape(p.n, 3 * E)
+        p.append(0, x)
+    p.check_attention(0, x, group=group)
+
+
+@pytest.mark.parametrize("size", [30, 1000, 4000])
+@pytest.mark.parametrize("rows,group", [(1, 1), (1, 2), (30, 1), (100, 1)])
+def test_attention_large_scores(pkg, L, rows, group, size):
+    """Scores up to size^2 64 / 8, equal or a size^2 / 8 apart and more: the weight is all the largest ones'."""
+    heads = 2
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=40, seqs=2, max_len=600), np.random.default_rng(41)
+    for counts in ([200, 70], [rows, 1]):
+        assert p.grow(counts)
+        x = np.zeros((p.n, 3, heads, D), np.float16)
+        x[:, 0] = size
+        ones = rng.integers(1, D + 1, p.n)
+        x[:, 1] = np.where(np.arange(D) < ones[:, None], size, 0)[:, None]
+        x[:, 1, 1] *= -1
+        x[:, 2] = rng.standard_normal((p.n, heads, D))
+        x = x.reshape(p.n, 3 * heads * D)
+        p.append(0, x)
+    # A score is a sum of 64 products in fp32, off by up to 64 2^-24 of the sum of their sizes, S = size^2 64 / 8, however near another is:
+    # 0.03 at 30, 30 at 1000, 500 at 4000.  check_attention's bound counts that (and says nothing from 1000 on).  At any size the row
+    # is an average of the values: weights that are rounded alike above and below, sums of 300 fp32 terms, the output's rounding.
+    p.check_attention(0, x, group=group)
+    got = p.attend(0, x, group=group).astype(np.float64).reshape(-1, heads, D)
+    for i in range(p.n):
+        s = 0 if i < rows else 1
+        v = p.r.held(0, s)[1][:, :int(p.r.start[s]) + (i - int(p.rows[s])) + 1]
+        off = np.abs(v).max() * (2.0 ** -11 + 300 * 2.0 ** -24)
+        assert (got[i] <= v.max(axis=1) + off).all() and (got[i] >= v.min(axis=1) - off).all()
+        assert (got[i] != 0).any(axis=1).all()
