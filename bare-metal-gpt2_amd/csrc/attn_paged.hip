@@ -9,7 +9,7 @@
 // is what the B operand of P.V holds in k-slots 8 g .. + 7; the dims are dealt so that a lane's 16 are contiguous in a K
 // row (16 g .. + 15), and the V tile's order is that of the A operand of V^T (8 tokens of a dim together).  Complete pages go from
 // memory to a ring in LDS, of each wave's own, by whole rows and without registers, and are made fp16, exactly, as they are taken.
-// The single new token of a sequence uses one of the 16 columns; the matrix units are idle otherwise, and the sums across
+// The single new token of a sequence uses two of the 16 columns; the matrix units are idle otherwise, and the sums across
 // lanes that a vector form needs cost more than the empty columns.
 #include <cmath>
 
@@ -83,12 +83,19 @@ struct PageFrag {
 // compiler does not see what `inf` is, or it would make a maximum of it.
 __device__ __forceinline__ float max_by(float a, float b, float inf) { return __builtin_amdgcn_fmed3f(a, b, inf); }
 
+// The value of the lane eight away in its row of 16.
+__device__ __forceinline__ float ror8(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));
+}
+
 constexpr float ATTN_LIFT = 15.f;
+// Where 8 rows or fewer are in a pass of 16 columns, column 8 + r has row r again and takes what the rounding of its weights to
+// fp16 leaves in column r (AttnCols::drop is -1 there).
 // N pages against Q times 16 columns, at once: a wave's chain from scores to maximum to weights to sums is what bounds it
 // where few waves share a SIMD, and two pages go down it in little more than the time of one.  Column jq sees keys below lim.
-template <int N, int Q>
-__device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[N], const f16x8 (&q)[Q][2], const int (&lim)[Q]) {
-    const int jq = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+template <bool SPARE, int N, int Q>
+__device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[N], const f16x8 (&q)[Q][2], const int (&lim)[Q], int id, float drop) {
+    const int g = (threadIdx.x & 63) >> 4;
     float s[Q][N][8], scale[N], mn[Q], base[Q], inf = INFINITY;
     asm("" : "+s"(inf));
     bool moved = false;
@@ -110,7 +117,7 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
         if (P[n].masked)
 #pragma unroll
             for (int u = 0; u < Q; ++u) {
-                const int left = (P[n].only < 0 || P[n].only == jq ? lim[u] : 0) - P[n].key0 - 8 * g;
+                const int left = (P[n].only < 0 || P[n].only == id ? lim[u] : 0) - P[n].key0 - 8 * g;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[u][n][e] = e < left ? s[u][n][e] : -INFINITY;
             }
@@ -137,9 +144,10 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
     }
     // The weights are held 2^ATTN_LIFT times as large, the largest at 2^15, so that the many small ones of a long context stay above
     // what fp16 rounds to fewer bits (2^-29 of the largest) or to nothing (2^-40).
-    // They are rounded to fp16, which costs an output about as much as its own rounding (1.2e-4 of it against
-    // 2.1e-4; with s_v in them, so that P.V could add to o in the product, 2e-4: the largest weight is then no longer 1 exactly,
-    // and it was no faster).
+    // They are rounded to fp16, which with 16 or 32 rows costs an output about half as much as its own rounding (1.1e-4 of it against
+    // 2.1e-4; second parts there, in products of their own, made 8 prompts of up to 600 rows take 66 us instead of 53).  With columns to
+    // spare a second column takes what is left, w - fp16(w), which is exact in fp32: 22 bits of a weight in all, for 0.3 us of a single
+    // token's 7.6 over 1000.
     f16x8 p[Q][N];
     float lift[Q], rate[N];
     bool huge = false;
@@ -173,7 +181,13 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[u][n][e] = (f16)__builtin_amdgcn_exp2f(fmaf(s[u][n][e], rate[n], lift[u]));
+            for (int e = 0; e < 8; e += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[u][n][e], rate[n], lift[u]));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[u][n][e + 1], rate[n], lift[u]));
+                const f16x2 w = {(f16)x, (f16)y};
+                p[u][n][e] = SPARE ? (f16)fmaf((float)w[0], drop, x) : w[0];
+                p[u][n][e + 1] = SPARE ? (f16)fmaf((float)w[1], drop, y) : w[1];
+            }
     // their sum, of the fp16 values as they are multiplied, on the matrix units too: a row of ones
     const f16x8 one = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
@@ -240,11 +254,13 @@ struct AttnLds {
     float m[W][16 * Q], l[W][16 * Q];
     static_assert(Q * 4 * 64 * 16 <= ATTN_STAGES<W> * 2 * PKV_TILE, "a wave's sums take its ring's place");
 };
+// id: which of the pass's rows or beams the column has; drop: 0, or -1 where it has the rest of that row's weights.
 template <int Q>
 struct AttnCols {
-    int row[Q], lim[Q], first;
+    int row[Q], lim[Q], first, id;
+    float drop;
 };
-template <int W, bool BEAMS, int Q>
+template <int W, bool BEAMS, bool SPARE, int Q>
 __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &st, int h, int z, const AttnCols<Q> &col, AttnLds<W, Q> &lds) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jq = lane & 15, g = lane >> 4;
@@ -340,13 +356,13 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
             if (todo) issue(stage);
             if (todo) issue(stage + 1);
             stage = (stage + 2) % ATTN_STAGES<W>;
-            attn_pages(A, P, q, col.lim);
+            attn_pages<SPARE>(A, P, q, col.lim, col.id, col.drop);
         }
     }
     // the waves' sums to one maximum, then together
 #pragma unroll
     for (int u = 0; u < Q; ++u)
-        if (g == 0) lds.m[w][16 * u + jq] = A[u].l[0] != 0.f ? A[u].m : -INFINITY;
+        if (g == 0) lds.m[w][16 * u + jq] = A[u].m;
     __syncthreads();
     float mx[Q];
 #pragma unroll
@@ -354,7 +370,7 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
         mx[u] = -INFINITY;
 #pragma unroll
         for (int v = 0; v < W; ++v) mx[u] = fmaxf(mx[u], lds.m[v][16 * u + jq]);
-        const float f = A[u].l[0] != 0.f ? __builtin_amdgcn_exp2f(A[u].m - mx[u]) : 0.f;
+        const float f = A[u].m != -INFINITY ? __builtin_amdgcn_exp2f(A[u].m - mx[u]) : 0.f;   // 0: the wave had no key for the column
         if (col.row[u] >= 0) {
             if (g == 0) lds.l[w][16 * u + jq] = A[u].l[0] * f;
 #pragma unroll
@@ -376,6 +392,16 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
             y[0] += o[0];
             y[1] += o[64];
         }
+        if constexpr (SPARE)
+            if (__ballot(col.drop != 0.f)) {   // a row's two columns, eight apart, together
+                L += ror8(L);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    y[0][r] += ror8(y[0][r]);
+                    y[1][r] += ror8(y[1][r]);
+                }
+                if (col.drop != 0.f) continue;
+            }
         if (a.splits == 1) {
             const float inv = L != 0.f ? 1.f / L : 0.f;   // no key: 0
             f16x8 o;
@@ -392,13 +418,16 @@ __device__ __forceinline__ void attn_pass(const PagedAttn &a, const AttnSteps &s
     }
 }
 
-// Rows 16 Q rb .. of one sequence, 16 Q of them, as a pass.
-template <int Q>
+// Rows 16 Q rb .. of one sequence, 16 Q of them, as a pass; with SPARE, up to 8 in two columns each.
+template <bool SPARE, int Q>
 __device__ __forceinline__ AttnSteps attn_rows(const PkvSeq &s, int seq, int rb, AttnCols<Q> &col) {
-    const int i0 = 16 * Q * rb, pages = (s.start + min(s.n, i0 + 16 * Q) + PKV_P - 1) / PKV_P;
+    const int i0 = 16 * Q * rb, pages = (s.start + min(s.n, i0 + 16 * Q) + PKV_P - 1) / PKV_P, jq = threadIdx.x & 15;
+    const bool two = SPARE && s.n <= 8;
+    col.id = two ? jq & 7 : jq;
+    col.drop = two && jq >= 8 ? -1.f : 0.f;
 #pragma unroll
     for (int u = 0; u < Q; ++u) {
-        const int i = i0 + 16 * u + (threadIdx.x & 15);
+        const int i = i0 + 16 * u + col.id;
         col.row[u] = i < s.n ? s.row0 + i : -1;
         col.lim[u] = i < s.n ? s.start + i + 1 : 0;
     }
@@ -410,6 +439,8 @@ __device__ __forceinline__ AttnSteps attn_rows(const PkvSeq &s, int seq, int rb,
 __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq &s, int seq0, uint64_t on, AttnCols<1> &col) {
     const GPT2PagedKV &c = a.c;
     const int lane = threadIdx.x & 63, jq = lane & 15, one = __builtin_ctzll(on);
+    const bool two = a.group <= 8;   // beams in two columns each
+    const int id = two ? jq & 7 : jq;
     // the leading pages that all share, complete in each
     int least = s.n ? s.len / PKV_P : 0x7fffffff;
 #pragma unroll
@@ -438,8 +469,8 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
         if (lane >= o) sum += v;
     }
     const int total = shared + __builtin_amdgcn_readlane(sum, 15);
-    const int n = __shfl(s.n, jq, 64), row = __shfl(s.row0, jq, 64), len = __shfl(s.len, jq, 64);
-    col = {{n ? row : -1}, {n ? len : 0}, shared * PKV_P};
+    const int n = __shfl(s.n, id, 64), row = __shfl(s.row0, id, 64), len = __shfl(s.len, id, 64);
+    col = {{n ? row : -1}, {n ? len : 0}, shared * PKV_P, id, two && jq >= 8 ? -1.f : 0.f};
     return {seq0 + one, __builtin_amdgcn_readlane(s.len, one), 0, shared, total, a.group, seq0 + min(lane, a.group - 1), s.len, s.slot, sum - own};
 }
 
@@ -455,8 +486,8 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
     for (int rb = blockIdx.z; 16 * rb < s.n; rb += gridDim.z) {
         if (rb >= (int)gridDim.z) __syncthreads();
         AttnCols<1> col;
-        const AttnSteps st = attn_rows(s, seq, rb, col);
-        attn_pass<W, false, 1>(a, st, h, blockIdx.y, col, lds);
+        const AttnSteps st = attn_rows<true>(s, seq, rb, col);
+        attn_pass<W, false, true, 1>(a, st, h, blockIdx.y, col, lds);
     }
 }
 
@@ -486,10 +517,10 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
             u.row0 = __builtin_amdgcn_readlane(s.row0, b);
             u.n = __builtin_amdgcn_readlane(s.n, b);
             u.slot = __builtin_amdgcn_readlane(s.slot, b);
-            st = attn_rows(u, seq0 + b, rb, col);
+            st = attn_rows<true>(u, seq0 + b, rb, col);
             st.off = 0x7fffffff;   // no step is a beam's own
         }
-        attn_pass<W, true, 1>(a, st, h, blockIdx.y, col, lds);
+        attn_pass<W, true, true, 1>(a, st, h, blockIdx.y, col, lds);
         if (together) break;
         if (16 * ++rb >= u.n) {
             const uint64_t more = on & ~((2ull << b) - 1);   // b < 16
@@ -513,8 +544,8 @@ __global__ __launch_bounds__(256) void k_pkv_attn_rows(PagedAttn a) {
     if (seq < 0) return;
     const PkvSeq s = pkv_seq(a.c, a.rows, a.nRows, seq);
     AttnCols<Q> col;
-    const AttnSteps st = attn_rows(s, seq, (s.n + 16 * Q - 1) / (16 * Q) - 1 - rb, col);   // the longest first
-    attn_pass<4, false, Q>(a, st, h, blockIdx.y, col, lds);
+    const AttnSteps st = attn_rows<false>(s, seq, (s.n + 16 * Q - 1) / (16 * Q) - 1 - rb, col);   // the longest first
+    attn_pass<4, false, false, Q>(a, st, h, blockIdx.y, col, lds);
 }
 
 // Many rows a sequence: a work-group per 64 of them and head, a wave per 16, every wave over all pages.  The four waves share
@@ -624,7 +655,7 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
                                 P[k].masked = true;
                             }
                         }
-                        attn_pages(A, P, q, limit);
+                        attn_pages<false>(A, P, q, limit, jq, 0.f);
                     }
                     lds_barrier();
                 }
@@ -644,7 +675,7 @@ __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
         if (full * PKV_P < end) {
             PageFrag P[1];
             get(0, 0, full, 1.f, 1.f, P[0]);
-            attn_pages(A, P, q, limit);
+            attn_pages<false>(A, P, q, limit, jq, 0.f);
         }
     }
     const float inv = A[0].l[0] != 0.f ? 1.f / A[0].l[0] : 0.f;

@@ -1,0 +1,93 @@
+"""The paged attention within a tight bound: with weights that two nearly equal keys tell apart."""
+import numpy as np
+import pytest
+
+from pagedkv_ref import D, P
+from test_gpu_pagedkv import Pair
+
+pytestmark = pytest.mark.gpu
+FINE, FP16 = 22, 11   # bits of a weight: half a step is 2^-bits of it
+
+
+class Keys:
+    """Keys and values of one sequence and head in 64 bits, [len, 64] each."""
+
+    def __init__(self, r, s, h):
+        n, full = int(r.len[s]), int(r.len[s]) // P
+        k, v = np.empty((n, D)), np.empty((n, D))
+        for j in range(-(-n // P)):
+            if j < full:
+                page = r.table[s, j]
+                a, b = (r.codes[0, page, i, h].astype(np.float64) * float(r.scales[0, page, i, h]) for i in (0, 1))
+            else:
+                a, b = (r.open[0, r.slot[s], i, h].astype(np.float64) for i in (0, 1))
+            m = min(P, n - j * P)
+            k[j * P:j * P + m] = a.reshape(P, D)[:m]
+            v[j * P:j * P + m] = b.reshape(P // 8, D, 8).transpose(0, 2, 1).reshape(P, D)[:m]
+        self.k, self.v = k, v
+
+    def row(self, q, vis, bits):
+        """The row's attention over its first `vis` keys, and how far a kernel may be off.
+
+        The output is sum w v / sum w.  A weight that is off by e of itself moves it by w e (v - out) / sum w.  e: the score's sum of 64 fp32
+        products, half a step 2^-24 of the running sum each, at most S = sum |q k| / 8 of them; its factors (6), the rounding of its
+        distance to the maximum and of the maximum M with the 2^15 that weights are held at (4 M + 48), in half steps; 2^-23 for an
+        exponential, of which there are up to 16 for moves of the maximum and joins; and the weight's own bits.  What is below fp16's range
+        is off by 2^-40 of the largest weight.  Sums: a page's 32 products, then three steps a page and 64 for joins, for values and weights.
+        The output's rounding: 2^-11 of it, or 2^-25."""
+        k, v = self.k[:vis], self.v[:vis]
+        x = k @ q / 8
+        w = np.exp(x - x.max())
+        tot = w.sum()
+        out = w @ v / tot
+        S, M = np.abs(k) @ np.abs(q) / 8, np.abs(x).max()
+        e = 2.0 ** -24 * (64 * S + 6 * np.abs(x) + 4 * M + 48) + 16 * 2.0 ** -23 + 2.0 ** -bits
+        away = np.abs(v - out)
+        sums = 2.0 ** -24 * (32 + 3 * -(-vis // P) + 64)
+        tol = (w * e) @ away + sums * (w @ np.abs(v)) * 2 + vis * 2.0 ** -40 * away.max(axis=0)
+        tol = tol / tot * (1 + 2.0 ** -8) + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
+        return out, tol, w
+
+
+def check(p, x, got, bits, heads, rows=None):
+    """`got` within the bound, for some heads and rows (None: all)."""
+    r = p.r
+    got = got.astype(np.float64).reshape(len(x), -1, D)
+    for s in range(r.seqs):
+        mine = [i for i in range(p.rows[s], p.rows[s + 1]) if rows is None or i in rows]
+        for h in heads if mine else []:
+            kv = Keys(r, s, h)
+            for i in mine:
+                vis = int(r.start[s]) + i - int(p.rows[s]) + 1
+                out, tol, w = kv.row(x[i, h * D:(h + 1) * D].astype(np.float64), vis, bits)
+                err = np.abs(got[i, h] - out)
+                assert (err <= tol).all(), f"sequence {s} row {i} head {h}: {(err / tol).max():.2f} of the bound ({err.max():.2e})"
+
+
+@pytest.mark.parametrize("seqs,rows,group,bits", [
+    (4, 1, 1, FINE), (4, 1, 2, FINE), (16, 1, 8, FINE), (4, 2, 1, FINE), (16, 8, 1, FINE), (16, 8, 4, FINE),
+    (16, 1, 16, FP16), (16, 9, 1, FP16), (4, 30, 1, FP16), (2, 70, 1, FP16),
+])
+@pytest.mark.parametrize("at,apart", [(40, 0.02), (46, 0.1), (50, 0.005), (127, 0.2)])
+def test_two_nearly_equal_keys(pkg, L, seqs, rows, group, bits, at, apart):
+    """Two keys of one page share nearly all of the weight and their values cancel, so that the output is how much they differ: weights of
+    fp16 show there.  The others are 2^-10 and less of them."""
+    heads = 2
+    p, rng = Pair(pkg, L, layers=1, heads=heads, pages=seqs * 7, seqs=seqs, max_len=320), np.random.default_rng(50 + at)
+    counts = [rows] + [1] * min(seqs - 1, max(seqs - rows, 1 if rows > seqs else 0)) + [0] * (rows - 1 if rows <= seqs else seqs - 2)
+    assert len(counts) == seqs and (sum(counts) <= seqs) == (bits == FINE or rows in (1, 9))
+    for step in ([at] * seqs, counts):
+        assert p.grow(step)
+        x = np.zeros((p.n, 3, heads, D), np.float16)
+        x[:, 0, :, 0] = 8          # q . k / 8 is the key's first dim
+        x[:, 1, :, 0] = -7 - rng.random((p.n, heads))
+        x[:, 2] = rng.standard_normal((p.n, heads, D))
+        on = np.flatnonzero(step)
+        if step is not counts:
+            v = rng.standard_normal((seqs, heads, D))
+            x[p.rows[on] + at - 4, 1, :, 0], x[p.rows[on] + at - 4, 2] = 0, v[on]
+        else:                      # each sequence's first new row: all of its rows see it
+            x[p.rows[on], 1, :, 0], x[p.rows[on], 2] = -apart * (0.5 + rng.random((len(on), heads))), -v[on]
+        x = x.reshape(p.n, -1)
+        p.append(0, x)
+    check(p, x, p.attend(0, x, group=group), bits, range(heads))
