@@ -1,9 +1,10 @@
-"""The paged attention within a tight bound: with weights that two nearly equal keys tell apart."""
+"""The paged attention within a bound that a lost page does not meet: with weights that two nearly equal keys tell
+apart, and over many pages."""
 import numpy as np
 import pytest
 
 from pagedkv_ref import D, P
-from test_gpu_pagedkv import Pair
+from test_gpu_pagedkv import Pair, qkv_of, rows_of
 
 pytestmark = pytest.mark.gpu
 FINE, FP16 = 22, 11   # bits of a weight: half a step is 2^-bits of it
@@ -48,10 +49,46 @@ class Keys:
         tol = tol / tot * (1 + 2.0 ** -8) + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
         return out, tol, w
 
+    def lost(self, out, tol, w):
+        """For each page, how far past twice the bound the row without it is, at its largest (a last page of few tokens aside)."""
+        n = -(-len(w) // P)
+        wv, ws = np.zeros((n * P, D)), np.zeros(n * P)
+        wv[:len(w)], ws[:len(w)] = w[:, None] * self.v[:len(w)], w
+        wv, ws = wv.reshape(n, P, D).sum(axis=1), ws.reshape(n, P).sum(axis=1)
+        left = ws.sum() - ws
+        with np.errstate(invalid="ignore", divide="ignore"):
+            without = (wv.sum(axis=0) - wv) / left[:, None]
+        far = np.where(left > 0, (np.abs(without - out) / (2 * tol)).max(axis=1), np.inf)
+        return far if len(w) % P == 0 or len(w) % P >= 8 else far[:-1]
 
-def check(p, x, got, bits, heads, rows=None):
-    """`got` within the bound, for some heads and rows (None: all)."""
-    r = p.r
+
+def filled(pkg, L, rng, heads, lens, new, max_len, share=0):
+    """A cache of those lengths whose last `new` tokens are the call's rows; pages anywhere in the pool (the second sequence has the first
+    one's first `share`), the values of every page about a vector of its own, so that none can go unnoticed."""
+    pages = sum(n // P for n in lens)
+    p = Pair(pkg, L, layers=1, heads=heads, pages=pages + 2, seqs=len(lens), max_len=max_len)
+    r, place, at = p.r, rng.permutation(pages + 2), 0
+    for s, n in enumerate(lens):
+        r.table[s, :n // P] = place[at:at + n // P]
+        at += n // P
+    r.table[1, :share] = r.table[0, :share]
+    r.codes[:] = rng.integers(-60, 61, r.codes.shape, dtype=np.int8)
+    v = r.codes[0, :, 1].reshape(-1, heads, P // 8, D, 8)
+    v[:] = v // 3 + rng.choice(np.array([-50, 50], np.int8), (len(v), heads, 1, D, 1))
+    r.codes[0, :, 1] = v.reshape(len(v), heads, -1)
+    r.scales[:] = rng.uniform(0.006, 0.01, r.scales.shape)
+    r.open[:] = rng.standard_normal(r.open.shape) * 0.2
+    v = r.open[0, :, 1].reshape(-1, heads, P // 8, D, 8)
+    r.open[0, :, 1] = (v + rng.choice([-0.4, 0.4], (len(v), heads, 1, D, 1))).reshape(len(v), heads, -1)
+    r.len[:], r.start[:], r.slot[:] = lens, np.asarray(lens) - new, rng.permutation(len(lens))
+    p.rows, p.n = rows_of(new), int(np.sum(new))
+    p.d_rows = pkg.Dev.from_numpy(p.rows)
+    return p
+
+
+def check(p, x, got, bits, heads, rows=None, pages=None):
+    """`got` within the bound, for some heads and rows (None: all); and all pages of those, or some, would be missed."""
+    r, seen = p.r, 0
     got = got.astype(np.float64).reshape(len(x), -1, D)
     for s in range(r.seqs):
         mine = [i for i in range(p.rows[s], p.rows[s + 1]) if rows is None or i in rows]
@@ -62,6 +99,11 @@ def check(p, x, got, bits, heads, rows=None):
                 out, tol, w = kv.row(x[i, h * D:(h + 1) * D].astype(np.float64), vis, bits)
                 err = np.abs(got[i, h] - out)
                 assert (err <= tol).all(), f"sequence {s} row {i} head {h}: {(err / tol).max():.2f} of the bound ({err.max():.2e})"
+                far = kv.lost(out, tol, w)
+                far = far if pages is None else far[[j for j in pages if j < len(far)]]
+                assert (far > 1).all(), f"sequence {s} row {i} head {h}: page {far.argmin()} would not be missed ({far.min():.2f})"
+                seen += len(far)
+    return seen
 
 
 @pytest.mark.parametrize("seqs,rows,group,bits", [
@@ -90,4 +132,18 @@ def test_two_nearly_equal_keys(pkg, L, seqs, rows, group, bits, at, apart):
             x[p.rows[on], 1, :, 0], x[p.rows[on], 2] = -apart * (0.5 + rng.random((len(on), heads))), -v[on]
         x = x.reshape(p.n, -1)
         p.append(0, x)
-    check(p, x, p.attend(0, x, group=group), bits, range(heads))
+    check(p, x, p.attend(0, x, group=group), bits, range(heads), pages=())
+
+
+@pytest.mark.parametrize("length", [33, 64, 500, 2047, 2500, 5000])
+@pytest.mark.parametrize("new,group,bits", [(1, 1, FINE), (3, 1, FINE), (1, 2, FINE), (9, 1, FP16)])
+def test_no_page_is_lost(pkg, L, length, new, group, bits):
+    """A work-group a sequence or group of beams, and 16 rows a work-group; split and not."""
+    rng = np.random.default_rng(length + new)
+    for max_len in (2048, 5120):
+        if length <= max_len:
+            lens = [length, max(length - 17, 1), 70, 5]
+            p = filled(pkg, L, rng, 2, lens, [1] * 4 if group > 1 else [new, 0, 0, 0], max_len, share=lens[1] // P // 2 if group > 1 else 0)
+            p.r.upload(pkg, p.c)
+            x = qkv_of(rng, p.n, 2)
+            assert check(p, x, p.attend(0, x, group=group), bits, (0, 1)) >= 2 * (length // P)
