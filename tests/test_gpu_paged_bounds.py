@@ -1,9 +1,9 @@
-"""The paged attention within a bound that a lost page does not meet: with weights that two nearly equal keys tell
-apart, and over many pages."""
+"""The paged attention within a bound that a lost page does not meet: every form, on both sides of the edges of its loops over
+pages, and with weights that two nearly equal keys tell apart."""
 import numpy as np
 import pytest
 
-from pagedkv_ref import D, P
+from pagedkv_ref import D, P, ref
 from test_gpu_pagedkv import Pair, qkv_of, rows_of
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +147,36 @@ def test_no_page_is_lost(pkg, L, length, new, group, bits):
             p.r.upload(pkg, p.c)
             x = qkv_of(rng, p.n, 2)
             assert check(p, x, p.attend(0, x, group=group), bits, (0, 1)) >= 2 * (length // P)
+
+
+@pytest.mark.parametrize("heads,lens,new,rows", [
+    (66, [8700, 9100, 300], [40, 19, 1], (0, 15, 16, 39, 40, 58, 59)),            # 16 rows a work-group, no splits
+    (66, [8230, 8600], [35, 65], (0, 31, 34, 35, 66, 99)),                        # 32
+    (121, [4190, 2112, 40], [700, 389, 11], (0, 63, 64, 699, 700, 1088, 1099)),   # 64, pages shared through LDS
+    (121, [2048, 2080, 6200], [500, 300, 300], (0, 499, 500, 799, 800, 1099)),
+])
+def test_long_contexts_unsplit(pkg, L, heads, lens, new, rows):
+    """More pages than a form looks up at once: 64 for 64 rows a work-group, 256 for the four waves of the others."""
+    rng = np.random.default_rng(heads + lens[0])
+    p = filled(pkg, L, rng, heads, lens, new, max(lens) + 200)
+    p.r.upload(pkg, p.c)
+    assert L.gpt2_pkv_attn_ws(ref(p.c), p.n) == 16, "not a case of this test: the call is split"
+    x = qkv_of(rng, p.n, heads)
+    x[:, :heads * D] *= np.float16(0.5)
+    assert check(p, x, p.attend(0, x), FP16, (0, heads // 2, heads - 1), rows) > 1000
+
+
+def test_half_a_million_tokens(pkg, L):
+    """More pages than the 64 splits of one row's call look up at once, 16384: eleven pages that have most of the weight between them,
+    on both sides of that edge and at the ends."""
+    rng = np.random.default_rng(60)
+    p, x = filled(pkg, L, rng, 1, [540010, 3], [1, 1], 540100), qkv_of(rng, 2, 1)
+    r, pages = p.r, [0, 1, 255, 256, 8191, 16383, 16384, 16385, 16639, 16640, 16874]
+    r.codes[0, :, 0, :, ::D] = 0
+    r.codes[0, r.table[0, pages], 0, :, ::D] = 127
+    r.scales[0, r.table[0, pages], 0] = 0.01
+    r.upload(pkg, p.c)
+    x[:, :D] *= np.float16(0.25)
+    x[0, 0] = 57   # scores 9 above the others
+    assert check(p, x, p.attend(0, x), FINE, (0,), rows=(0,), pages=pages) == 11
+    check(p, x, p.attend(0, x), FINE, (0,), rows=(1,))
