@@ -18,7 +18,7 @@
 
 namespace g2 {
 
-// 16-byte pieces a thread, 8192 logits a work-group.  Half as many were slower (512 rows of 50257: 21 us, 18; four rows: as
+// Pieces of eight logits a thread, 8192 a work-group.  Half as many were slower (512 rows of 50257: 21 us, 18; four rows: as
 // long, and longer to join), twice as many too (30 us).
 constexpr int BEAM_PIECES = 4;
 constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / (256 * BEAM_PIECES);
@@ -29,6 +29,7 @@ struct BeamPart {
 };
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4_dword __attribute__((ext_vector_type(4), aligned(4)));   // at any dword
 
 // Maximum over the wave, the same scalar for all: rows of 16 lanes by DPP, then the four rows.
 __device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
@@ -76,8 +77,10 @@ __device__ __forceinline__ float beam_key_logit(uint32_t key) {
     return h2f((uint16_t)(o & 0x8000u ? o & 0x7fffu : ~o));
 }
 
-// One part of a row: its 16-byte pieces [256 NV part, ...), the first part also the logits before the first whole
-// piece and after the last.
+// One part of a row: its pieces of eight [256 NV part, ...), the first part also the logits after the last whole piece.
+// A row's logits go to threads and sums by their number, wherever the row begins: equal rows have equal sums, so that
+// equal scores tie.  So a piece is loaded as dwords, from the one that has its first logit, and where that is a dword's upper half with
+// the one past them.
 //
 // A thread's logits stay in registers as keys of their own, order << 16 | (63 - i) for its i-th; the tokens of a thread
 // ascend with i, so its largest is its best.  A key that `beams` threads of a wave reach is a lower bound for the part's result;
@@ -93,21 +96,34 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     __shared__ int lds_n;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, part = blockIdx.x;
     const uint16_t *x = logits + (size_t)blockIdx.y * ld;
-    const int head = min(V, (int)(((16 - ((uintptr_t)x & 15)) & 15) >> 1)), pieces = (V - head) >> 3;
-    const int first = part * 256 * NV + tid, left = V - 8 * pieces, odd = tid < head ? tid : 8 * pieces + tid;
+    const int pieces = V >> 3, first = part * 256 * NV + tid, left = V & 7, odd = 8 * pieces + tid;
+    const bool upper = (uintptr_t)x & 2;   // the same for the whole row
     if (tid == 0) lds_n = 0;
     f16x2 v[N / 2], vodd;
     uint32_t key[N], kodd;
+    const int *dwords = reinterpret_cast<const int *>(x - upper);
+    i32x4 h[NV];
+    int next[NV] = {};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        i32x4 h = {(int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00};
-        if (first + 256 * j < pieces) h = *reinterpret_cast<const i32x4 *>(x + head + 8 * (first + 256 * j));
-#pragma unroll
-        for (int d = 0; d < 4; ++d) v[4 * j + d] = __builtin_bit_cast(f16x2, (int)h[d]);
+        h[j] = i32x4{(int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00, (int)0xfc00fc00};
+        if (first + 256 * j < pieces) {
+            h[j] = *reinterpret_cast<const i32x4_dword *>(dwords + 4 * (first + 256 * j));
+            if (upper) next[j] = dwords[4 * (first + 256 * j) + 4];
+        }
     }
     const bool has_odd = part == 0 && tid < left;
-    vodd = f16x2{(f16)-INFINITY, (f16)-INFINITY};
-    if (has_odd) vodd[0] = __builtin_bit_cast(f16, x[odd]);
+    uint16_t rest = 0xfc00;
+    if (has_odd) rest = x[odd];
+    if (upper)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (first + 256 * j < pieces)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) h[j][d] = (int)__builtin_amdgcn_alignbit((uint32_t)(d < 3 ? h[j][d + 1] : next[j]), (uint32_t)h[j][d], 16);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[i] = __builtin_bit_cast(f16x2, (int)h[i / 4][i % 4]);
+    vodd = f16x2{__builtin_bit_cast(f16, rest), (f16)-INFINITY};
     uint32_t best = 0, piece[NV] = {};   // the largest of a piece
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
@@ -126,7 +142,7 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
 #pragma unroll
     for (int j = 0; j < NV; ++j) best = max(best, piece[j]);
     vodd = beam_logits(vodd);
-    const int token0 = head + 8 * first;
+    const int token0 = 8 * first;
     auto token = [&](uint32_t k) {   // of one of the thread's own keys
         const int i = 63 - (int)(k & 63u);
         return token0 + 2048 * (i >> 3) + (i & 7);
@@ -166,7 +182,8 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     if (lane == 0) {
         lds_t[w] = bound;
         lds_m[w] = m;
-        lds_s[w] = m == -INFINITY ? 0.0 : sum * (1.0 + 0.6931471805599453 * ((double)c - (double)m * (double)l2e));
+        const double e = 0.6931471805599453 * ((double)c - (double)m * (double)l2e);   // 0.003 at most
+        lds_s[w] = m == -INFINITY ? 0.0 : sum * (1.0 + e * (1.0 + 0.5 * e));
     }
     __syncthreads();
     bound = max(max(lds_t[0], lds_t[1]), max(lds_t[2], lds_t[3]));

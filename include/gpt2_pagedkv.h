@@ -116,8 +116,10 @@ void gpt2_pkv_compact(GPT2PagedKV *c);
  * row), score_out, done_out, [groups * beams] each.  Equal scores: the lower row first, within a row the larger logit,
  * then the lower token.  A logit that is NaN counts as -inf, +inf as 65504, a score that is NaN as -inf.  A row with
  * done[r] != 0 has one continuation, `eos` at its own score; done_out marks rows that end with eos.  eos < 0: there is no
- * end token, and done is not read (may be NULL; done_out is 0).  score_out and done_out may be score and done.  Sums and
- * scores are formed in fp64.  ws as for gpt2_pkv_attn. */
+ * end token, and done is not read (may be NULL; done_out is 0).  score_out and done_out may be score and done.  Exponentials
+ * are fp32, and up to 33 of them are summed in fp32, what those make in fp64, where scores are formed and compared: a score is within 95
+ * 2^-24 of the exact one before it is rounded to fp32.  A row's sum depends on its logits alone, not on where it lies, so
+ * equal rows with equal scores tie.  ws as for gpt2_pkv_attn. */
 size_t gpt2_beam_select_ws(int groups, int beams, int V);
 void gpt2_beam_select(int *token, int *parent, float *score_out, int *done_out, const gpt2_half *logits, long ld,
                       const float *score, const int *done, int groups, int beams, int V, int eos, void *ws, size_t wsBytes);
