@@ -18,7 +18,9 @@
  *
  * A ragged batch.  `rows` is a device array of nSeq + 1 offsets: rows[s] .. rows[s+1] - 1 are sequence s's
  * new rows in the activations (qkv [nRows][3 E], x and att [nRows][E], E = nHead * headDim), none is fine.
- * nRows, at most 2^23, is how many rows the buffers hold; those past rows[nSeq] are left as they are.  One step
+ * nRows, at most 2^23, is how many rows the call may look at, all of rows[nSeq] at least; those past rows[nSeq] are left as they are.
+ * How a call runs goes by nRows, since the host does not know the offsets: up to nSeq, as for one row a sequence (a decode step passes
+ * nSeq, even if its buffers hold more); past it, as for prompts.  Results differ in the order of sums and the bits of weights.  One step
  * of a model over a batch:
  *     gpt2_pkv_grow(c, rows, nRows);              once: pages for the new rows, positions, lengths
  *     gpt2_pkv_embed(x, wte, wpe, ids, c, rows, nRows);
@@ -95,8 +97,8 @@ void gpt2_pkv_embed(gpt2_half *x, const gpt2_half *wte, const gpt2_half *wpe, co
  * once for each layer after a grow. */
 void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, const int *rows, int nRows);
 /* att[row] = softmax(q . k / 8) v over the tokens up to the row's own, from the cache.  `group`: 1, or how many
- * consecutive sequences (at most 16) are beams of one prompt: the leading pages that all of a group share are then
- * read once for its one-row sequences; results are the same but for the order of sums and the bits of the weights.  Scores and sums are
+ * consecutive sequences (at most 16) are beams of one prompt: in a call with nRows <= nSeq the leading pages that all of a group share are
+ * then read once, if its sequences have one row each at most (a batch with a prompt in it is faster with 1; past nSeq, group means nothing); results are the same but for the order of sums and the bits of the weights.  Scores and sums are
  * fp32.  The softmax's weights have 22 bits where the call has no more rows than sequences (nRows <= nSeq) and a sequence has at most 8 of
  * them, with one row a sequence a group at most 8 beams; elsewhere they are rounded to fp16, which takes an output's error against 64 bits
  * from 2.1e-4 of the result's norm, its own rounding, to 2.4e-4.  ws: at least gpt2_pkv_attn_ws
