@@ -11,6 +11,8 @@
 // memory to a ring in LDS, of each wave's own, by whole rows and without registers, and are made fp16, exactly, as they are taken.
 // The single new token of a sequence uses two of the 16 columns; the matrix units are idle otherwise, and the sums across
 // lanes that a vector form needs cost more than the empty columns.
+//
+// Times in this file: a launch under the tracer, the median over two sets of inputs in turn, one layer of 12 heads.
 #include <cmath>
 
 #include "pagedkv.h"
@@ -145,9 +147,9 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
     // The weights are held 2^ATTN_LIFT times as large, the largest at 2^15, so that the many small ones of a long context stay above
     // what fp16 rounds to fewer bits (2^-29 of the largest) or to nothing (2^-40).
     // They are rounded to fp16, which with 16 or 32 rows costs an output about half as much as its own rounding (1.1e-4 of it against
-    // 2.1e-4; second parts there, in products of their own, made 8 prompts of up to 600 rows take 66 us instead of 53).  With columns to
-    // spare a second column takes what is left, w - fp16(w), which is exact in fp32: 22 bits of a weight in all, for 0.3 us of a single
-    // token's 7.6 over 1000.
+    // 2.1e-4; second parts there, in products of their own, made 8 prompts of up to 600 rows take 66 us a call instead of 53).  With columns to
+    // spare a second column takes what is left, w - fp16(w), which is exact in fp32: 22 bits of a weight in all, for 0.3 us of the 7.6 that
+    // a call with a single token over 1000 takes.
     f16x8 p[Q][N];
     float lift[Q], rate[N];
     bool huge = false;
@@ -475,8 +477,8 @@ __device__ __forceinline__ AttnSteps attn_beams(const PagedAttn &a, const PkvSeq
 }
 
 // One row a sequence, nearly always (no more rows than sequences): a work-group per sequence, head and split (gridDim.z of them, for
-// sequences that have more than 16 rows after all).  16 contexts up to 16384 tokens: 56.4 us for 268 MB, 4.8 TB/s, bound by memory; one of
-// 1000 tokens 7.2, by the chain of loads from the books to the pages and by its code's way from L2 ...
+// sequences that have more than 16 rows after all).  16 contexts up to 16384 tokens: 57.8 us for 268 MB, 4.6 TB/s, bound by memory; 48
+// of up to 1000 16.9; one of 1000 tokens 7.5, by the chain of loads from the books to the pages and by its code's way from L2 ...
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) AttnLds<W, 1> lds;
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_one(PagedAttn a) {
 }
 
 // ... or per group of beams, together where they have a row each at most and there are two: shared pages are read once, and a beam is a
-// column.  8 x 8 beams over 900 tokens 12.4 us, as 64 sequences of their own 16.4; bound as the single row's, with the comparison of the tables in the chain.
+// column.  8 x 8 beams over 900 tokens 13.0 us, as 64 sequences of their own 14.0; bound as the single row's, with the comparison of the tables in the chain.
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) AttnLds<W, 1> lds;
@@ -533,8 +535,8 @@ __global__ __launch_bounds__(64 * W) void k_pkv_attn_beams(PagedAttn a) {
 }
 
 // Any number of rows a sequence: a work-group per 16 Q of them, head and split.  8 prompts of up to 600 rows over up to 2000 tokens, Q = 2:
-// 52 us, 0.33 PFLOP/s of what is not masked; vector instructions, 78% of the cycles (115 for 16 rows and a page), bound it, at the three
-// waves a SIMD that its registers leave.
+// 58 us (52 a call among others, whose first work-groups fill its uneven end: 0.33 PFLOP/s of what is not masked); vector instructions, 79% of
+// the cycles (some 115 for 16 rows and a page), bound it, at the three waves a SIMD that its registers leave.
 template <int Q>
 __global__ __launch_bounds__(256) void k_pkv_attn_rows(PagedAttn a) {
     __shared__ __attribute__((aligned(1024))) AttnLds<4, Q> lds;
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(256) void k_pkv_attn_rows(PagedAttn a) {
 // Many rows a sequence: a work-group per 64 of them and head, a wave per 16, every wave over all pages.  The four waves share
 // the work of turning a page into fragments: a wave takes a quarter (a K tile's half, or 16 of V's 32 pairs of dims) from memory to
 // registers, 16 bytes a lane, ATTN_AHEAD pairs of pages ahead, to fp16, and to LDS in the order in which all four read it.  16 rows a
-// work-group would read each page from L2 four times as often, which bounds that form (61 us for 8 prompts of up to 600 rows over
+// work-group would read each page from L2 four times as often, which bounds that form (66 us for 8 prompts of up to 600 rows over
 // up to 2000 tokens).
 constexpr int ATTN_AHEAD = 2;   // pairs of pages
 __global__ __launch_bounds__(256, 4) void k_pkv_attn_block(PagedAttn a) {
@@ -725,17 +727,18 @@ __global__ __launch_bounds__(256) void k_pkv_attn_join(PagedAttn a) {
 
 // How a call runs: its form, and how the steps are split over work-groups: at least `per` of them each, into `splits` at most.
 //   ONE    no more rows than sequences: a sequence (or group of beams) a work-group.  Without a group up to 4 of them take turns at the
-//          16-row blocks of a sequence that has a whole prompt: 200 rows after 800 tokens, 256 sequences in the cache, 77 us with one, 42 with
-//          two, 30 with four; 256 single rows 24.5, 24.0, 25.8.
+//          16-row blocks of a sequence that has a whole prompt: 200 rows after 800 tokens, 256 sequences in the cache, 80 us with one, 54 with
+//          two, 31 with four; 256 single rows over up to 400 tokens 29.0, 28.7, 31.3, over up to 100 20.0, 20.0, 23.1.
 //   ROWS1  16 rows a work-group, keys split over its waves.
-//   ROWS2  32 of them, from 32 rows a sequence on: a page is made fp16 once for twice the rows (a prompt of 1000 rows 12 us; 19 with BLOCK).
-//   BLOCK  64, pages shared through LDS, where that makes eight work-groups a CU: 32 prompts of up to 1000 rows 85 us, 104 with
-//          ROWS2; 8 of up to 600 over 2000 tokens 64 us, 58 with ROWS2.
+//   ROWS2  32 of them, from 32 rows a sequence on: a page is made fp16 once for twice the rows (8 prompts of up to 600 over 2000 tokens 58 us,
+//          66 with ROWS1; one of 1000 rows 11.8, 11.6 and with BLOCK 20).
+//   BLOCK  64, pages shared through LDS, where that makes eight work-groups a CU: 32 prompts of up to 1000 rows 83 us, 102 with
+//          ROWS2; 8 of up to 600 over 2000 tokens 62 us, 58 with ROWS2.
 // No splits for caches whose sequences a work-group's waves get through in the time of a second launch, nor where the rows alone
 // make one work-group a CU (8 prompts of up to 200 rows over up to 2000 tokens: 26 us, 26 + 7 with two splits).  Where splits of 64
-// pages fill the card they stream best (16 contexts up to 16384 tokens: 48.7 us, 49.9 with 32 pages each, 55.4 with 96); with fewer
-// sequences, or groups of beams, as many as make 512 work-groups, of 16 pages at least (8 x 8 beams over 2100 tokens: 5 splits 11.2 us,
-// 2 splits 17.6, 9 splits 13.8; over 4096: 5 15.8, 2 19.0, 8 18.7).
+// pages fill the card they stream best (16 contexts up to 16384 tokens: 57.8 us, 58.5 with 32 pages each, 67.3 with 96); with fewer
+// sequences, or groups of beams, as many as make 512 work-groups, of 16 pages at least (8 x 8 beams over 2100 tokens: 5 splits 13.0 us,
+// 2 splits 15.6, 9 splits 15.4; over 4096: 5 16.2, 3 20.0, 9 18.9).
 enum AttnForm { ATTN_ONE, ATTN_ROWS1, ATTN_ROWS2, ATTN_BLOCK };
 struct AttnPlan {
     AttnForm form;

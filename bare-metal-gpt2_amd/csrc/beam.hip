@@ -4,9 +4,9 @@
 // score_b + x - m_b - log(sum_b) orders a row's tokens as its logits do, so a row's candidates are its best `beams` logits:
 // one pass over the logits takes each part of a row's maximum, its sum of exponentials and its best, and a second launch, a
 // work-group a group, joins the parts and merges the rows' lists of candidates in fp64.  64 groups of
-// 8 rows of 50257 take 18.5 us (2.8 TB/s) and 5.3; 512 groups of one row, which need no bounds, 15: instructions, some 14 a pair of
-// logits and the bounds and sums of every wave, take longer than the reading (10 us).  Four rows take 5.0 and 3.6, the latency of
-// two short launches.
+// 8 rows of 50257 take 18.7 us (2.8 TB/s) and 5.4; 512 groups of one row, which need no bounds, 14.0: instructions, some 14 a pair of
+// logits and the bounds and sums of every wave, take longer than the reading (10 us).  Four rows take 5.2 and 3.8, the latency of
+// two short launches.  (Launches under the tracer, medians over two sets of inputs in turn.)
 //
 // A logit and its token are one 32-bit key, (logit's bits in order) << 16 | (65535 - token): keys of a row are unique, and
 // the larger key is the larger logit or, of equal ones, the lower token.  0 is no key.
@@ -18,8 +18,8 @@
 
 namespace g2 {
 
-// Pieces of eight logits a thread, 8192 a work-group.  Half as many were slower (512 rows of 50257: 21 us, 18; four rows: as
-// long, and longer to join), twice as many too (30 us).
+// Pieces of eight logits a thread, 8192 a work-group.  Half as many are slower where there are many rows (512 rows of 50257: 21.3
+// us and 6.0 to join for 18.7 and 5.4; four rows 4.6 and 4.0 for 5.2 and 3.8), twice as many too (20.0; 6.2).
 constexpr int BEAM_PIECES = 4;
 constexpr int BEAM_PARTS = GPT2_BEAM_MAX_VOCAB / 8 / (256 * BEAM_PIECES);
 struct BeamPart {
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256) void k_beam_part(BeamPart *__restrict__ out, c
     const uint32_t top = wave_max_key(best);
     const float m = top ? beam_key_logit(top) : -INFINITY;
     uint32_t bound = 0u;
-    if (beams <= 4) {   // maximum after maximum is quicker for few (4 rows, 4 beams: 5.0 us, 5.2)
+    if (beams <= 4) {   // maximum after maximum is quicker for few (4 rows, 4 beams: 5.2 us, 5.5)
         bound = top;
         uint32_t rest = best;
         for (int k = 1; k < beams; ++k) {

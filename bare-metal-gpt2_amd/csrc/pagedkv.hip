@@ -2,7 +2,8 @@
 // append that quantises complete pages, and reading rows back.  Its attention is attn_paged.hip.
 //
 // All of it is bound by memory or, at the sizes of a decode step, by launch latency: the kernels are few, take what
-// depends on the sequences' lengths from device memory, and never come back to the host.
+// depends on the sequences' lengths from device memory, and never come back to the host.  Times in this file: a launch under
+// the tracer, the median over two sets of inputs in turn, 12 heads, one layer unless said.
 #include <cmath>
 #include <cstring>
 
@@ -72,8 +73,8 @@ __global__ void k_pkv_reset(GPT2PagedKV c) {
 // ------------------------------------------------------------------ grow
 // One work-group: needs and their sums over the sequences, then a walk over refs that hands the lowest free pages out in
 // order, which stops when enough are found (its first step is under way meanwhile); tables, refs and lengths are written once they
-// are.  Bound by the latency of its few dependent loads and barriers: 4.3 us for 48 sequences with T = 256 threads, 5.4 with 1024; where
-// hundreds of pages are handed out (48 prompts of up to 1000 rows) 6.8 and 6.1.
+// are.  Bound by the latency of its few dependent loads and barriers: 4.3 us for 48 sequences with T = 256 threads, 5.2 with 1024; where
+// hundreds of pages are handed out (48 prompts of up to 1000 rows) 8.0 and 6.4.
 template <int T>
 __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__restrict__ rows, int nRows) {
     constexpr int NW = T / 64, PER = GPT2_PKV_MAX_SEQ / 1024, FREE = 8;
@@ -161,7 +162,8 @@ __global__ __launch_bounds__(T) void k_pkv_grow(GPT2PagedKV c, const int *__rest
 }
 
 // ------------------------------------------------------------------ embed
-// A work-group a row, four values a thread: 8-byte loads and stores.
+// A work-group a row, four values a thread: 8-byte loads and stores.  48 rows of 48 sequences 2.6 us, the chain from the offsets, looked up by
+// halving, to the books, the token and its row; 30666 rows 28 us, 94 MB in and 47 out (some of the table's rows are in a cache).
 constexpr int EMBED_THREADS = GPT2_N_EMBD / 4;
 __global__ __launch_bounds__(EMBED_THREADS) void k_pkv_embed(uint16_t *__restrict__ x, const uint16_t *__restrict__ wte,
                                                              const uint16_t *__restrict__ wpe, const int *__restrict__ ids, GPT2PagedKV c,
@@ -236,8 +238,8 @@ __device__ __forceinline__ void pkv_by_dims(uint32_t (&d)[16], char *lds) {
 }
 
 // Codes of a whole tile and its scale: q = rint(fl(x / s)), |x / s| <= 127 (1 + 2^-24).  x / s is y = x (1 / s) to within
-// 2^-16; only where that lies that near to the middle between two whole numbers (a tile in some twenty has such a value)
-// are the quotients formed.  y + 1.5 2^23 is the nearest whole number in its low byte.
+// 2^-16; only where y lies within twice that of the middle between two whole numbers are the quotients formed (three tiles in ten of
+// normal values have such a one, nearly always a middle itself: fp16 values have few bits).  y + 1.5 2^23 is the nearest whole number in its low byte.
 __device__ __forceinline__ float pkv_quantize(const uint32_t (&d)[16], uint32_t (&out)[8]) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 m = {0, 0};
@@ -276,8 +278,8 @@ __device__ __forceinline__ int pkv_append_units(const PkvSeq &q) {
 }
 
 // One wave per unit, K|V and head: whole row pieces in, 16 bytes a lane, the tile's maximum over the wave, 8 bytes of codes a
-// lane and store, 512 contiguous.  48 prompts of 250 to 1000 rows: 34 to 40 us, 4.1 to 3.4 TB/s of rows in and codes out (a row's
-// piece of a head is 128 bytes, every 4.5 KB); a decode step's 48 rows 6.4 us, its chain of loads and the code's own way from memory.
+// lane and store, 512 contiguous.  48 prompts of 250 to 1000 rows: 40 us, 3.4 TB/s of rows in and codes out (a row's
+// piece of a head is 128 bytes, every 4.5 KB); a decode step's 48 rows 6.8 us, its chain of loads and the code's own way from memory.
 __device__ __forceinline__ void pkv_append_unit(const GPT2PagedKV &c, int L, const uint16_t *__restrict__ qkv, const PkvSeq &q,
                                                 int seq, int u, int kv, int h, char *lds) {
     const int lane = threadIdx.x & 63;
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(256) void k_pkv_append(GPT2PagedKV c, int L, const 
 
 // ------------------------------------------------------------------ read
 // A unit is a page that the rows of a sequence touch; a wave takes one K|V and head of it: the tile in its own order,
-// 8 values a lane and piece, V through LDS to rows, 16-byte stores.  Bound by memory: 46 MB of codes to 92 MB of rows in 26 us, 5.3 TB/s.
+// 8 values a lane and piece, V through LDS to rows, 16-byte stores.  Bound by memory: 46 MB of codes to 92 MB of rows in 26.6 us, 5.2 TB/s.
 struct PkvRead {
     long pos;        // of the sequence's first row
     int row0, n;
@@ -500,8 +502,8 @@ __global__ __launch_bounds__(256) void k_pkv_fork_plan(GPT2PagedKV c, const int 
 // Second launch: blockIdx.y 0 the books, then the open page of sequence blockIdx.x, a layer's K or V and four heads each, only the
 // tokens in it.  A thread copies piece `tid` (16 bytes) of the four tiles, all under way together; of a V tile's octet that the tokens
 // end in, it puts those that are there among what was.  32 prompts of 8 beams, all layers: 151 MB that have to move in
-// 35 us (42 where nothing is in a cache yet: 3.6 TB/s, 4.3 with the rest of those octets); a work-group for all the heads took 36.6
-// (44), and for one prompt's four beams 4.0 us, 3.4 here.
+// 44 us (3.4 TB/s, 4.1 with the rest of those octets; 35 us over one set of inputs, which is then in a cache); there a work-group for all the
+// heads took 36.6, and for one prompt's four beams 4.0, 3.3 here.
 __global__ __launch_bounds__(256) void k_pkv_fork(GPT2PagedKV c, const int *__restrict__ parent) {
     const int me = blockIdx.x, tid = threadIdx.x;
     const PkvPlan plan = pkv_plan(c);
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(1024) void k_pkv_compact_plan(GPT2PagedKV c) {
 }
 
 // Second launch: the first `copiers` work-groups move pages (a unit is eight tiles of one layer, and their scales), the
-// others renumber the page tables.  Bound by memory: 373 pages of 12 layers, 441 MB in and out, in 92 us, 4.8 TB/s.
+// others renumber the page tables.  Bound by memory: 373 pages of 12 layers, 441 MB in and out, in 93 us, 4.7 TB/s.
 __global__ __launch_bounds__(256) void k_pkv_compact(GPT2PagedKV c, int copiers) {
     const int tid = threadIdx.x;
     const PkvPlan plan = pkv_plan(c);
@@ -734,10 +736,10 @@ extern "C" void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, con
     if (!qkv || !aligned16(qkv)) { arg_fail("gpt2_pkv_append: null/unaligned"); return; }
     const bool by_seq = nRows <= c->nSeq;
     // a wave takes one tile of a unit, two where there are work-groups for more than two rounds of the card: 48 prompts of 250 to
-    // 1000 rows 37.6 -> 33.9 us (4.1 TB/s), 8 prompts of up to 700 10.9 -> 12.9
+    // 1000 rows 42.3 -> 40.4 us, 8 prompts of up to 700 11.9 -> 13.3
     const int units = by_seq ? c->nSeq : nRows / PKV_P + c->nSeq, per = !by_seq && (long)units * c->nHead >= 8192 ? 2 : 1;
     // by sequences, up to four work-groups take turns at the units of one that has a whole prompt: 200 rows, 256 sequences in the cache
-    // 26.7 us with one, 14.4 with four; a decode step's rows as long with either
+    // 27.2 us with one, 14.1 with four; a decode step's rows as long with either
     const dim3 grid(units, cdiv(2 * c->nHead, 4 * per), by_seq ? min(4, nRows / PKV_P + 1) : 1);
     const auto fn = by_seq ? k_pkv_append<true> : k_pkv_append<false>;
     hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream(), *c, L, qkv, rows, nRows);
