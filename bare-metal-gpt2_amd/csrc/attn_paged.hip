@@ -147,7 +147,7 @@ __device__ __forceinline__ void attn_pages(AttnAcc (&A)[Q], const PageFrag (&P)[
     // The weights are held 2^ATTN_LIFT times as large, the largest at 2^15, so that the many small ones of a long context stay above
     // what fp16 rounds to fewer bits (2^-29 of the largest) or to nothing (2^-40).
     // They are rounded to fp16, which with 16 or 32 rows costs an output about half as much as its own rounding (1.1e-4 of it against
-    // 2.1e-4; second parts there, in products of their own, made 8 prompts of up to 600 rows take 66 us a call instead of 53).  With columns to
+    // 2.1e-4; second parts there, in products of their own, made 8 prompts of up to 600 rows take 58 us a call instead of 52).  With columns to
     // spare a second column takes what is left, w - fp16(w), which is exact in fp32: 22 bits of a weight in all, for 0.3 us of the 7.6 that
     // a call with a single token over 1000 takes.
     f16x8 p[Q][N];
