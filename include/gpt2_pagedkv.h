@@ -98,11 +98,11 @@ void gpt2_pkv_embed(gpt2_half *x, const gpt2_half *wte, const gpt2_half *wpe, co
 void gpt2_pkv_append(GPT2PagedKV *c, int L, const gpt2_half *qkv, const int *rows, int nRows);
 /* att[row] = softmax(q . k / 8) v over the tokens up to the row's own, from the cache.  `group`: 1, or how many
  * consecutive sequences (at most 16) are beams of one prompt: in a call with nRows <= nSeq the leading pages that all of a group share are
- * then read once, if its sequences have one row each at most (a batch with a prompt in it is faster with 1; past nSeq, group means nothing); results are the same but for the order of sums and the bits of the weights.  Scores and sums are
- * fp32.  The softmax's weights have 22 bits where the call has no more rows than sequences (nRows <= nSeq) and a sequence has at most 8 of
- * them, with one row a sequence a group at most 8 beams; elsewhere they are rounded to fp16, which takes an output's error against 64 bits
- * from 2.1e-4 of the result's norm, its own rounding, to 2.4e-4.  ws: at least gpt2_pkv_attn_ws
- * bytes of device memory, 16-byte aligned, with no meaning between calls; calls that may overlap need one each.  More rows may need
+ * then read once, if its sequences have one row each at most (a batch with a prompt in it is faster with 1; past nSeq, group means
+ * nothing); results are the same but for the order of sums and the bits of the weights.  Scores and sums are fp32.  The softmax's weights have
+ * 22 bits where the call has no more rows than sequences (nRows <= nSeq) and a sequence has at most 8 of them, a group of beams
+ * with one row each at most 8 beams; elsewhere they are rounded to fp16, which takes an output's error against 64 bits from 2.1e-4 of the
+ * result's norm, its own rounding, to 2.4e-4.  ws: at least gpt2_pkv_attn_ws bytes of device memory, 16-byte aligned, with no meaning between calls; calls that may overlap need one each.  More rows may need
  * less (they are split less): a workspace for calls of several sizes has the largest of theirs. */
 size_t gpt2_pkv_attn_ws(const GPT2PagedKV *c, int nRows);
 void gpt2_pkv_attn(gpt2_half *att, const gpt2_half *qkv, const GPT2PagedKV *c, int L, const int *rows, int nRows,
