@@ -22,6 +22,7 @@ N_LAYER, N_HEAD, N_EMBD, VOCAB, N_CTX = 12, 12, 768, 50257, 1024
 HEAD_DIM, FFN, QKV = 64, 3072, 2304
 TOTAL_PARAMS = 124439808
 PAGE_TOKENS, PAGE_TILE, BEAM_MAX = 32, 2048, 16           # include/gpt2_pagedkv.h
+EPI_NONE, EPI_GELU, EPI_ADD = 0, 1, 2                     # include/gpt2_int4.h
 DECODE_AUTO, DECODE_MULTI, DECODE_PERSISTENT = -1, 0, 1   # gpt2_decode_graph_create_mode modes
 N_QTENSORS = 1 + 4 * N_LAYER
 
@@ -90,6 +91,20 @@ class GPT2PagedKV(C.Structure):
                [(n, C.c_int) for n in ("nLayer", "nHead", "headDim", "nPages", "nSeq", "maxPages")] + [("arena", _vp)]
 
 
+class GPT2Int4W(C.Structure):
+    _fields_ = [("codes", _vp), ("scales", _vp), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int), ("arena", _vp)]
+
+
+class GPT2History(C.Structure):
+    _fields_ = [("tokens", _vp), ("len", _vp), ("start", _vp), ("arrived", _vp), ("nSeq", C.c_int), ("room", C.c_int), ("arena", _vp)]
+
+
+class GPT2LogitsRules(C.Structure):
+    _fields_ = [("history", C.POINTER(GPT2History)), ("repetition", _vp), ("presence", _vp), ("frequency", _vp), ("ngram", C.c_int),
+                ("n_bias", C.c_int), ("bias_start", _vp), ("bias_token", _vp), ("bias_value", _vp), ("mask", _vp), ("mask_row", _vp),
+                ("n_masks", C.c_int)]
+
+
 class GPT2Backend(C.Structure):
     _fields_ = [("name", C.c_char_p)] + [(n, _vp) for n in (
         "embed", "layernorm", "matmul", "attention", "gelu", "add", "matmul_q", "gemv", "gemv_q")]
@@ -99,6 +114,7 @@ class GPT2Backend(C.Structure):
 _i, _u, _sz, _d = C.c_int, C.c_uint, C.c_size_t, C.c_double
 _BE = C.POINTER(GPT2Backend)
 _PKV = C.POINTER(GPT2PagedKV)
+_Q4, _HIST = C.POINTER(GPT2Int4W), C.POINTER(GPT2History)
 SIGNATURES = {
     # include/gpt2_kernels.h
     "gpt2_load_weights": (_i, [C.c_char_p, C.POINTER(GPT2Weights)]),
@@ -186,6 +202,20 @@ SIGNATURES = {
     "gpt2_pkv_compact": (None, [_PKV]),
     "gpt2_beam_select_ws": (_sz, [_i, _i, _i]),
     "gpt2_beam_select": (None, [_vp, _vp, _vp, _vp, _vp, C.c_long, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
+    # include/gpt2_int4.h
+    "gpt2_int4_code_bytes": (_sz, [_i, _i]),
+    "gpt2_int4_scale_count": (_sz, [_i, _i, _i]),
+    "gpt2_int4_alloc": (_i, [_Q4, _i, _i, _i]),
+    "gpt2_int4_free": (None, [_Q4]),
+    "gpt2_quantize_int4": (None, [_Q4, _vp]),
+    "gpt2_dequantize_int4": (None, [_vp, _Q4]),
+    "gpt2_matmul_int4": (None, [_vp, _vp, _Q4, _vp, _i, _i, _vp]),
+    # include/gpt2_logits.h
+    "gpt2_history_alloc": (_i, [_HIST, _i, _i]),
+    "gpt2_history_free": (None, [_HIST]),
+    "gpt2_history_reset": (None, [_HIST]),
+    "gpt2_history_step": (None, [_HIST, _vp, _vp, _vp, _i, _i]),
+    "gpt2_logits_adjust": (None, [_vp, _vp, C.c_long, _i, _i, C.POINTER(GPT2LogitsRules)]),
     # bench / tuning hooks (not part of the reference interface)
     "gpt2_tune_gemm_count": (_i, []),
     "gpt2_tune_gemm_name": (C.c_char_p, [_i]),
@@ -377,6 +407,32 @@ class PagedKV:
 
     def free(self) -> None:
         lib().gpt2_pkv_free(C.byref(self.c))
+
+
+class Int4:
+    """Weights of 4 bits with group scales (gpt2_int4_alloc)."""
+
+    def __init__(self, N: int, K: int, group: int = 64):
+        self.w = GPT2Int4W()
+        if lib().gpt2_int4_alloc(C.byref(self.w), N, K, group):
+            check("gpt2_int4_alloc")
+            raise GPUError("gpt2_int4_alloc failed")
+
+    def free(self) -> None:
+        lib().gpt2_int4_free(C.byref(self.w))
+
+
+class History:
+    """Token histories of several sequences (gpt2_history_alloc)."""
+
+    def __init__(self, n_seq: int, room: int = N_CTX):
+        self.h = GPT2History()
+        if lib().gpt2_history_alloc(C.byref(self.h), n_seq, room):
+            check("gpt2_history_alloc")
+            raise GPUError("gpt2_history_alloc failed")
+
+    def free(self) -> None:
+        lib().gpt2_history_free(C.byref(self.h))
 
 
 def half_bits_to_f32(h: np.ndarray) -> np.ndarray:
