@@ -2,6 +2,7 @@
 // (gpt2_logits.h).
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "common.h"
 #include "gpt2_logits.h"
@@ -11,7 +12,7 @@ namespace g2 {
 // ------------------------------------------------------------------ histories
 // All sequences change at once, in place: a work-group has a few columns of every sequence's row in its registers before it writes
 // any.  The lengths, which every work-group reads, are written by the one that arrives last.
-constexpr int HIST_THREADS = 1024, HIST_ITEMS = 16;   // tokens a thread holds
+constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 4096 sequences at one piece each
 
 struct HistSeq {
     int from, past, after, row0;   // from: the sequence that it goes on as, or -1
@@ -32,27 +33,31 @@ __device__ __forceinline__ HistSeq hist_seq(const GPT2History &h, const int *__r
     return q;
 }
 
+// A thread's pieces are W consecutive tokens (4 where rows lie at 16 bytes, else 1).
+template <int W>
 __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, const int *__restrict__ parent, const int *__restrict__ rows,
                                                                const int *__restrict__ ids, int nRows, int prompt, int width_log2) {
-    const int tid = threadIdx.x, threads = blockDim.x, width = 1 << width_log2, c = (blockIdx.x << width_log2) + (tid & (width - 1));
+    typedef std::conditional_t<W == 4, i32x4, int> piece;
+    // neighbouring columns, which share cache lines, to one XCD: consecutive work-groups go round the eight
+    const int xcd = blockIdx.x & 7, slabs = gridDim.x, slab = xcd * (slabs >> 3) + min(xcd, slabs & 7) + (blockIdx.x >> 3);
+    const int tid = threadIdx.x, threads = blockDim.x, width = 1 << width_log2, c = W * ((slab << width_log2) + (tid & (width - 1)));
     const int per = threads >> width_log2, s0 = tid >> width_log2;   // sequences at once; this thread's first
-    int value[HIST_ITEMS];
-    uint32_t write = 0;
+    piece value[HIST_ITEMS];
+    uint32_t moved = 0, grown = 0;
+    int past[HIST_ITEMS], after[HIST_ITEMS];
 #pragma unroll
     for (int i = 0; i < HIST_ITEMS; ++i) {
         const int s = s0 + i * per;
-        value[i] = 0;
-        if (s < h.nSeq && c < h.room) {
+        past[i] = after[i] = 0;
+        if (s < h.nSeq) {
             const HistSeq q = hist_seq(h, parent, rows, nRows, s);
-            if (c < q.past) {
-                if (q.from != s) {
-                    value[i] = h.tokens[(size_t)q.from * h.room + c];
-                    write |= 1u << i;
-                }
-            } else if (c < q.after) {
-                value[i] = ids[q.row0 + (c - q.past)];
-                write |= 1u << i;
+            past[i] = q.past;
+            after[i] = q.after;
+            if (q.from != s && c < q.past) {
+                value[i] = *reinterpret_cast<const piece *>(h.tokens + (size_t)q.from * h.room + c);
+                moved |= 1u << i;
             }
+            if (q.after > q.past && c < q.after && c + W > q.past) grown |= 1u << i;   // so there are rows and ids
         }
     }
     // every token and length has been read: passing through here waits for the loads
@@ -60,8 +65,20 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
     for (int i = 0; i < HIST_ITEMS; ++i) asm volatile("" : "+v"(value[i]) : : "memory");
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i)
-        if (write >> i & 1) h.tokens[(size_t)(s0 + i * per) * h.room + c] = value[i];
+    for (int i = 0; i < HIST_ITEMS; ++i) {
+        int *to = h.tokens + (size_t)(s0 + i * per) * h.room + c;
+        if (moved >> i & 1) {
+            if (c + W <= past[i]) *reinterpret_cast<piece *>(to) = value[i];
+            else if constexpr (W == 4)
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    if (c + e < past[i]) to[e] = value[i][e];
+        }
+        if (grown >> i & 1) {   // few: tokens that are appended
+            const int row0 = rows[s0 + i * per];
+            for (int e = max(0, past[i] - c); e < W && c + e < after[i]; ++e) to[e] = ids[row0 + (c + e - past[i])];
+        }
+    }
     __shared__ int last;
     if (tid == 0) {
         __threadfence();
@@ -69,9 +86,10 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
     }
     __syncthreads();
     if (!last) return;
-    int len[HIST_ITEMS], start[HIST_ITEMS];   // at most 4096 sequences: 4 a thread of 1024, 16 of 256
+    constexpr int LENS = GPT2_PKV_MAX_SEQ / 256;   // at most 4096 sequences, 256 threads at least
+    int len[LENS], start[LENS];
 #pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i) {
+    for (int i = 0; i < LENS; ++i) {
         const int s = tid + i * threads;
         len[i] = start[i] = 0;
         if (s < h.nSeq) {
@@ -82,7 +100,7 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i) {
+    for (int i = 0; i < LENS; ++i) {
         const int s = tid + i * threads;
         if (s < h.nSeq) {
             h.len[s] = len[i];
@@ -107,9 +125,13 @@ static bool history_refused(const GPT2History *h, const char *what) {
 
 // ------------------------------------------------------------------ logits
 // A work-group has SLICE tokens of a row.  What the row's history says of each is counted in LDS: how often it was said since
-// `start`, whether it was said at all, whether it would end a known n-gram.  A bias list's entry of a token is its last, by the largest index.
-constexpr int SLICE = 4096;
+// `start`, whether it was said at all, whether it would end a known n-gram.  Of a bias list's entries for a token the last counts, by the largest
+// index, in a second table where there are biases.  Tokens go by octets: 16 bytes of logits, wherever a row begins, a byte of the mask.  The octets are
+// asked for first and the history is read meanwhile.
+constexpr int SLICE = 8192, LOGIT_THREADS = 512, OCTETS = SLICE / 8 / LOGIT_THREADS;
 constexpr uint32_t SEEN = 1u << 31, BANNED = 1u << 30, COUNT = BANNED - 1;
+typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 struct RowRules {
     float rep, freq, pres;
@@ -125,56 +147,112 @@ __device__ __forceinline__ float adjusted(float x, uint32_t said, float bias, co
     return x;
 }
 
-__global__ __launch_bounds__(256) void k_logits_adjust(uint16_t *out, const uint16_t *logits, long ld, int V, GPT2LogitsRules r, GPT2History h) {
-    __shared__ uint32_t said[SLICE], bias_at[SLICE];
+__global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, const uint16_t *logits, long ld, int V, GPT2LogitsRules r, GPT2History h) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t tables[];
+    uint32_t *const said = tables, *const bias_at = tables + SLICE;   // the second only where there are biases
     const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SLICE, nt = min(SLICE, V - t0);
     const uint16_t *x = logits + (size_t)row * ld + t0;
     uint16_t *y = out + (size_t)row * ld + t0;
-    for (int i = tid; i < SLICE; i += 256) {
-        said[i] = 0;
-        bias_at[i] = 0;
+    const uint8_t *mask = nullptr;
+    if (r.n_masks) {
+        const int m = r.mask_row ? r.mask_row[row] : row;
+        if ((unsigned)m < (unsigned)r.n_masks) mask = reinterpret_cast<const uint8_t *>(r.mask + (size_t)m * ((V + 31) >> 5)) + (t0 >> 3);
     }
+    const bool sparse = out == logits && !mask;   // only what a rule names is touched
+    u16x8_any v[OCTETS];
+    uint32_t allowed[OCTETS];
+    if (!sparse)
+#pragma unroll
+        for (int o = 0; o < OCTETS; ++o) {
+            const int i = 8 * (tid + LOGIT_THREADS * o);
+            allowed[o] = mask && i < nt ? mask[i >> 3] : 0xffu;
+            if (i + 8 <= nt) v[o] = *reinterpret_cast<const u16x8_any *>(x + i);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[o][e] = i + e < nt ? x[i + e] : 0;
+        }
+    const int tables_n = r.n_bias ? 2 * SLICE : SLICE;
+    for (int i = 4 * tid; i < tables_n; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(tables + i) = i32x4{0, 0, 0, 0};
     __syncthreads();
-    if (h.tokens) {
-        const int n = min(max(h.len[row], 0), h.room), start = h.start[row];
-        const int *tok = h.tokens + (size_t)row * h.room;
-        for (int i = tid; i < n; i += 256) {
-            const unsigned t = (unsigned)(tok[i] - t0);
+    const int *tok = h.tokens ? h.tokens + (size_t)row * h.room : nullptr;
+    const int len = tok ? min(max(h.len[row], 0), h.room) : 0;
+    const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(r.bias_start[row + 1], r.n_bias) : 0;
+    if (len) {
+        const int start = h.start[row], last = r.ngram > 0 ? len - r.ngram : -1;   // n-grams that begin at 0 .. last
+        const int *tail = tok + len - (r.ngram - 1);
+        const int first = r.ngram > 1 && last >= 0 ? tail[0] : 0;
+        auto one = [&](int i, int w) {
+            const unsigned t = (unsigned)(w - t0);
             if (t < (unsigned)nt) {
                 if (i >= start) atomicAdd(&said[t], 1u);
                 else atomicOr(&said[t], SEEN);
             }
-        }
-        if (r.ngram > 0 && n >= r.ngram) {
-            const int *tail = tok + n - (r.ngram - 1);
-            for (int i = tid; i + r.ngram <= n; i += 256) {
-                const unsigned t = (unsigned)(tok[i + r.ngram - 1] - t0);
-                if (t >= (unsigned)nt) continue;
+            if (i <= last && (r.ngram == 1 || w == first)) {
                 bool same = true;
-                for (int j = 0; j < r.ngram - 1 && same; ++j) same = tok[i + j] == tail[j];
-                if (same) atomicOr(&said[t], BANNED);
+                for (int j = 1; j < r.ngram - 1 && same; ++j) same = tok[i + j] == tail[j];
+                const unsigned end = (unsigned)(tok[i + r.ngram - 1] - t0);
+                if (same && end < (unsigned)nt) atomicOr(&said[end], BANNED);
             }
+        };
+        for (int i = 4 * tid; i < len; i += 4 * LOGIT_THREADS) {
+            if (i + 4 <= len) {
+                const i32x4_any w = *reinterpret_cast<const i32x4_any *>(tok + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) one(i + e, w[e]);
+            } else
+                for (int e = i; e < len; ++e) one(e, tok[e]);
         }
     }
-    if (r.n_bias) {
-        const int a = min(max(r.bias_start[row], 0), r.n_bias), b = min(r.bias_start[row + 1], r.n_bias);
-        for (int i = a + tid; i < b; i += 256) {
-            const unsigned t = (unsigned)(r.bias_token[i] - t0);
-            if (t < (unsigned)nt) atomicMax(&bias_at[t], (unsigned)i + 1);
-        }
+    for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {
+        const unsigned t = (unsigned)(r.bias_token[i] - t0);
+        if (t < (unsigned)nt) atomicMax(&bias_at[t], (unsigned)i + 1);
     }
-    __syncthreads();
     const RowRules rules = {r.repetition ? r.repetition[row] : 1.f, r.frequency ? r.frequency[row] : 0.f, r.presence ? r.presence[row] : 0.f};
-    const uint32_t *mask = nullptr;
-    if (r.n_masks) {
-        const int m = r.mask_row ? r.mask_row[row] : row;
-        if ((unsigned)m < (unsigned)r.n_masks) mask = r.mask + (size_t)m * ((V + 31) >> 5);
+    __syncthreads();
+    auto bias_of = [&](uint32_t at) { return at ? r.bias_value[at - 1] : 0.f; };
+    if (sparse) {
+        // who takes a token's word first applies its rules: the history's tokens, then those that only have a bias
+        for (int i = tid; i < len; i += LOGIT_THREADS) {
+            const unsigned t = (unsigned)(tok[i] - t0);
+            if (t >= (unsigned)nt) continue;
+            const uint32_t w = atomicExch(&said[t], 0u);
+            if (w) y[t] = f2h(adjusted(h2f(x[t]), w, r.n_bias ? bias_of(atomicExch(&bias_at[t], 0u)) : 0.f, rules));
+        }
+        if (!r.n_bias) return;
+        __syncthreads();
+        for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {
+            const unsigned t = (unsigned)(r.bias_token[i] - t0);
+            if (t >= (unsigned)nt) continue;
+            const uint32_t at = atomicExch(&bias_at[t], 0u);
+            if (at) y[t] = f2h(h2f(x[t]) + bias_of(at));
+        }
+        return;
     }
-    for (int i = tid; i < nt; i += 256) {
-        float v = adjusted(h2f(x[i]), said[i], bias_at[i] ? r.bias_value[bias_at[i] - 1] : 0.f, rules);
-        const int t = t0 + i;
-        if (mask && !(mask[t >> 5] >> (t & 31) & 1)) v = -INFINITY;
-        y[i] = f2h(v);
+#pragma unroll
+    for (int o = 0; o < OCTETS; ++o) {
+        const int i = 8 * (tid + LOGIT_THREADS * o);
+        if (i >= nt) break;
+        uint32_t w[8], at[8], any = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<i32x4 *>(w + e) = *reinterpret_cast<const i32x4 *>(said + i + e);
+            *reinterpret_cast<i32x4 *>(at + e) = r.n_bias ? *reinterpret_cast<const i32x4 *>(bias_at + i + e) : i32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) any |= w[e] | at[e];
+        if (any)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (w[e] | at[e]) v[o][e] = f2h(adjusted(h2f(v[o][e]), w[e], bias_of(at[e]), rules));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!(allowed[o] >> e & 1)) v[o][e] = 0xfc00;
+        if (out == logits && !any && allowed[o] == 0xffu) continue;
+        if (i + 8 <= nt) *reinterpret_cast<u16x8_any *>(y + i) = v[o];
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e < nt) y[i + e] = v[o][e];
     }
 }
 
@@ -215,11 +293,14 @@ extern "C" void gpt2_history_step(GPT2History *h, const int *parent, const int *
         arg_fail("gpt2_history_step: bad rows");
         return;
     }
-    int width = 6;   // log2 of the columns that a work-group takes
+    const bool wide = h->room % 4 == 0 && aligned16(h->tokens);
+    const int w = wide ? 4 : 1;
+    int width = wide ? 4 : 6;   // log2 of the pieces of a row that a work-group takes: 256 bytes
     while ((h->nSeq << width) > HIST_THREADS * HIST_ITEMS) --width;
     int threads = 256;
     while (threads < HIST_THREADS && (h->nSeq << width) > threads) threads *= 2;
-    hipLaunchKernelGGL(k_history_step, dim3(cdiv(h->room, 1 << width)), dim3(threads), 0, stream(), *h, parent, rows, ids, nRows, prompt, width);
+    hipLaunchKernelGGL(wide ? k_history_step<4> : k_history_step<1>, dim3(cdiv(h->room, w << width)), dim3(threads), 0, stream(), *h, parent, rows, ids, nRows,
+                       prompt, width);
     check_launch("k_history_step");
 }
 
@@ -242,6 +323,6 @@ extern "C" void gpt2_logits_adjust(gpt2_half *out, const gpt2_half *logits, long
         arg_fail("gpt2_logits_adjust: bad rules");
         return;
     }
-    hipLaunchKernelGGL(k_logits_adjust, dim3(cdiv(V, SLICE), rows), dim3(256), 0, stream(), out, logits, ld, V, r, h);
+    hipLaunchKernelGGL(k_logits_adjust, dim3(cdiv(V, SLICE), rows), dim3(LOGIT_THREADS), SLICE * 4 * (r.n_bias ? 2 : 1), stream(), out, logits, ld, V, r, h);
     check_launch("k_logits_adjust");
 }
