@@ -126,9 +126,9 @@ static bool history_refused(const GPT2History *h, const char *what) {
 // ------------------------------------------------------------------ logits
 // A work-group has SLICE tokens of a row.  What the row's history says of each is counted in LDS: how often it was said since
 // `start`, whether it was said at all, whether it would end a known n-gram.  Of a bias list's entries for a token the last counts, by the largest
-// index, in a second table where there are biases.  Tokens go by octets: 16 bytes of logits, wherever a row begins, a byte of the mask.  The octets are
-// asked for first and the history is read meanwhile.
-constexpr int SLICE = 8192, LOGIT_THREADS = 512, OCTETS = SLICE / 8 / LOGIT_THREADS;
+// index, in a second table where there are biases.  The tokens that were said are listed as their first mention is counted; for those,
+// and the few that only have a bias, a thread each works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever the row begins, a byte of the mask.
+constexpr int SLICE = 4096, LOGIT_THREADS = 512, OCTETS = SLICE / 8 / LOGIT_THREADS;
 constexpr uint32_t SEEN = 1u << 31, BANNED = 1u << 30, COUNT = BANNED - 1;
 typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -147,18 +147,35 @@ __device__ __forceinline__ float adjusted(float x, uint32_t said, float bias, co
     return x;
 }
 
+constexpr int TABLES = SLICE * (4 + 2 + 2) + 16, BIAS_TABLE = SLICE * 4;   // bytes of LDS; the second where there are biases
+
 __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, const uint16_t *logits, long ld, int V, GPT2LogitsRules r, GPT2History h) {
     extern __shared__ __attribute__((aligned(16))) uint32_t tables[];
-    uint32_t *const said = tables, *const bias_at = tables + SLICE;   // the second only where there are biases
+    uint32_t *const said = tables, *const listed = tables + SLICE;
+    uint16_t *const list = reinterpret_cast<uint16_t *>(tables + SLICE + 4), *const value = list + SLICE;   // tokens that were said; the slice's logits
+    uint32_t *const bias_at = tables + TABLES / 4;
     const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SLICE, nt = min(SLICE, V - t0);
     const uint16_t *x = logits + (size_t)row * ld + t0;
     uint16_t *y = out + (size_t)row * ld + t0;
+    const int *tok = h.tokens ? h.tokens + (size_t)row * h.room : nullptr;
+    const int len = tok ? min(max(h.len[row], 0), h.room) : 0, start = tok ? h.start[row] : 0;
+    const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(r.bias_start[row + 1], r.n_bias) : 0;
     const uint8_t *mask = nullptr;
     if (r.n_masks) {
         const int m = r.mask_row ? r.mask_row[row] : row;
         if ((unsigned)m < (unsigned)r.n_masks) mask = reinterpret_cast<const uint8_t *>(r.mask + (size_t)m * ((V + 31) >> 5)) + (t0 >> 3);
     }
     const bool sparse = out == logits && !mask;   // only what a rule names is touched
+    const RowRules rules = {r.repetition ? r.repetition[row] : 1.f, r.frequency ? r.frequency[row] : 0.f, r.presence ? r.presence[row] : 0.f};
+    // the thread's first tokens, bias and octets are asked for together
+    i32x4_any w0 = {};
+    int bias_t0 = -1;
+    float bias_v0 = 0.f;
+    if (4 * tid + 4 <= len) w0 = *reinterpret_cast<const i32x4_any *>(tok + 4 * tid);
+    if (bias0 + tid < bias1) {
+        bias_t0 = r.bias_token[bias0 + tid];
+        bias_v0 = r.bias_value[bias0 + tid];
+    }
     u16x8_any v[OCTETS];
     uint32_t allowed[OCTETS];
     if (!sparse)
@@ -171,88 +188,101 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[o][e] = i + e < nt ? x[i + e] : 0;
         }
-    const int tables_n = r.n_bias ? 2 * SLICE : SLICE;
-    for (int i = 4 * tid; i < tables_n; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(tables + i) = i32x4{0, 0, 0, 0};
+    for (int i = 4 * tid; i < SLICE + 4; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(tables + i) = i32x4{0, 0, 0, 0};
+    if (r.n_bias)
+        for (int i = 4 * tid; i < SLICE; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(bias_at + i) = i32x4{0, 0, 0, 0};
     __syncthreads();
-    const int *tok = h.tokens ? h.tokens + (size_t)row * h.room : nullptr;
-    const int len = tok ? min(max(h.len[row], 0), h.room) : 0;
-    const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(r.bias_start[row + 1], r.n_bias) : 0;
     if (len) {
-        const int start = h.start[row], last = r.ngram > 0 ? len - r.ngram : -1;   // n-grams that begin at 0 .. last
+        const int last = r.ngram > 0 ? len - r.ngram : -1;   // n-grams begin at 0 .. last
         const int *tail = tok + len - (r.ngram - 1);
         const int first = r.ngram > 1 && last >= 0 ? tail[0] : 0;
-        auto one = [&](int i, int w) {
-            const unsigned t = (unsigned)(w - t0);
-            if (t < (unsigned)nt) {
-                if (i >= start) atomicAdd(&said[t], 1u);
-                else atomicOr(&said[t], SEEN);
+        auto ends = [&](int i, int w) {   // n-grams from i on that begin as the last n - 1 tokens
+            if (i > last || (r.ngram > 1 && w != first)) return;
+            bool same = true;
+            for (int j = 1; j < r.ngram - 1 && same; ++j) same = tok[i + j] == tail[j];
+            const unsigned end = (unsigned)(tok[i + r.ngram - 1] - t0);
+            if (same && end < (unsigned)nt) atomicOr(&said[end], BANNED);
+        };
+        // counts first, then the list of those that were new: one place of it for each of a wave's, by one addition
+        auto take = [&](int i, const i32x4_any &w, int n) {
+            uint32_t before[4];
+            uint64_t fresh[4];
+            int total = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned t = (unsigned)(w[e] - t0);
+                before[e] = SEEN;
+                if (e < n && t < (unsigned)nt) before[e] = i + e >= start ? atomicAdd(&said[t], 1u) : atomicOr(&said[t], SEEN);
             }
-            if (i <= last && (r.ngram == 1 || w == first)) {
-                bool same = true;
-                for (int j = 1; j < r.ngram - 1 && same; ++j) same = tok[i + j] == tail[j];
-                const unsigned end = (unsigned)(tok[i + r.ngram - 1] - t0);
-                if (same && end < (unsigned)nt) atomicOr(&said[end], BANNED);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                fresh[e] = __ballot(!(before[e] & (SEEN | COUNT)));
+                total += __popcll(fresh[e]);
             }
+            if (total) {
+                int at = 0;
+                const uint64_t here = __ballot(true);
+                if ((tid & 63) == __builtin_ctzll(here)) at = (int)atomicAdd(listed, (uint32_t)total);
+                at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (!(before[e] & (SEEN | COUNT)))
+                        list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(fresh[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)fresh[e], 0u))] = (uint16_t)(w[e] - t0);
+                    at += __popcll(fresh[e]);
+                }
+            }
+            if (r.ngram > 0)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < n) ends(i + e, w[e]);
         };
         for (int i = 4 * tid; i < len; i += 4 * LOGIT_THREADS) {
+            i32x4_any w = w0;
             if (i + 4 <= len) {
-                const i32x4_any w = *reinterpret_cast<const i32x4_any *>(tok + i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) one(i + e, w[e]);
+                if (i != 4 * tid) w = *reinterpret_cast<const i32x4_any *>(tok + i);
             } else
-                for (int e = i; e < len; ++e) one(e, tok[e]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = i + e < len ? tok[i + e] : 0;
+            take(i, w, min(4, len - i));
         }
     }
     for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {
-        const unsigned t = (unsigned)(r.bias_token[i] - t0);
+        const unsigned t = (unsigned)((i == bias0 + tid ? bias_t0 : r.bias_token[i]) - t0);
         if (t < (unsigned)nt) atomicMax(&bias_at[t], (unsigned)i + 1);
     }
-    const RowRules rules = {r.repetition ? r.repetition[row] : 1.f, r.frequency ? r.frequency[row] : 0.f, r.presence ? r.presence[row] : 0.f};
+    if (!sparse)
+#pragma unroll
+        for (int o = 0; o < OCTETS; ++o) *reinterpret_cast<i32x4 *>(value + 8 * (tid + LOGIT_THREADS * o)) = __builtin_bit_cast(i32x4, v[o]);
     __syncthreads();
-    auto bias_of = [&](uint32_t at) { return at ? r.bias_value[at - 1] : 0.f; };
-    if (sparse) {
-        // who takes a token's word first applies its rules: the history's tokens, then those that only have a bias
-        for (int i = tid; i < len; i += LOGIT_THREADS) {
-            const unsigned t = (unsigned)(tok[i] - t0);
-            if (t >= (unsigned)nt) continue;
-            const uint32_t w = atomicExch(&said[t], 0u);
-            if (w) y[t] = f2h(adjusted(h2f(x[t]), w, r.n_bias ? bias_of(atomicExch(&bias_at[t], 0u)) : 0.f, rules));
-        }
-        if (!r.n_bias) return;
-        __syncthreads();
-        for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {
-            const unsigned t = (unsigned)(r.bias_token[i] - t0);
-            if (t >= (unsigned)nt) continue;
-            const uint32_t at = atomicExch(&bias_at[t], 0u);
-            if (at) y[t] = f2h(h2f(x[t]) + bias_of(at));
-        }
-        return;
+    auto put = [&](unsigned t, float bias) {
+        const uint16_t to = f2h(adjusted(h2f(sparse ? x[t] : value[t]), said[t], bias, rules));
+        if (sparse) y[t] = to;
+        else value[t] = to;
+    };
+    for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {   // tokens that only have a bias
+        const bool is_first = i == bias0 + tid;
+        const unsigned t = (unsigned)((is_first ? bias_t0 : r.bias_token[i]) - t0);
+        if (t < (unsigned)nt && bias_at[t] == (unsigned)i + 1 && !said[t]) put(t, is_first ? bias_v0 : r.bias_value[i]);
     }
+    for (int i = tid, n = *listed; i < n; i += LOGIT_THREADS) {
+        const unsigned t = list[i], at = r.n_bias ? bias_at[t] : 0u;
+        put(t, at ? r.bias_value[at - 1] : 0.f);
+    }
+    if (sparse) return;
+    __syncthreads();
 #pragma unroll
     for (int o = 0; o < OCTETS; ++o) {
         const int i = 8 * (tid + LOGIT_THREADS * o);
         if (i >= nt) break;
-        uint32_t w[8], at[8], any = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<i32x4 *>(w + e) = *reinterpret_cast<const i32x4 *>(said + i + e);
-            *reinterpret_cast<i32x4 *>(at + e) = r.n_bias ? *reinterpret_cast<const i32x4 *>(bias_at + i + e) : i32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) any |= w[e] | at[e];
-        if (any)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (w[e] | at[e]) v[o][e] = f2h(adjusted(h2f(v[o][e]), w[e], bias_of(at[e]), rules));
+        u16x8_any to = __builtin_bit_cast(u16x8_any, *reinterpret_cast<const i32x4 *>(value + i));
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (!(allowed[o] >> e & 1)) v[o][e] = 0xfc00;
-        if (out == logits && !any && allowed[o] == 0xffu) continue;
-        if (i + 8 <= nt) *reinterpret_cast<u16x8_any *>(y + i) = v[o];
+            if (!(allowed[o] >> e & 1)) to[e] = 0xfc00;
+        if (i + 8 <= nt) *reinterpret_cast<u16x8_any *>(y + i) = to;
         else
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (i + e < nt) y[i + e] = v[o][e];
+                if (i + e < nt) y[i + e] = to[e];
     }
 }
 
@@ -323,6 +353,6 @@ extern "C" void gpt2_logits_adjust(gpt2_half *out, const gpt2_half *logits, long
         arg_fail("gpt2_logits_adjust: bad rules");
         return;
     }
-    hipLaunchKernelGGL(k_logits_adjust, dim3(cdiv(V, SLICE), rows), dim3(LOGIT_THREADS), SLICE * 4 * (r.n_bias ? 2 : 1), stream(), out, logits, ld, V, r, h);
+    hipLaunchKernelGGL(k_logits_adjust, dim3(cdiv(V, SLICE), rows), dim3(LOGIT_THREADS), TABLES + (r.n_bias ? BIAS_TABLE : 0), stream(), out, logits, ld, V, r, h);
     check_launch("k_logits_adjust");
 }
