@@ -10,9 +10,11 @@
 namespace g2 {
 
 // ------------------------------------------------------------------ histories
-// All sequences change at once, in place: a work-group has a few columns of every sequence's row in its registers before it writes
-// any.  The lengths, which every work-group reads, are written by the one that arrives last.
-constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 4096 sequences at one piece each
+// All sequences change at once, in place: a work-group has what it moves in its registers before it writes any.  Where parents lie in their
+// children's block of R sequences (9 to 16: one is a multiple of any number of beams up to 16), it moves such a block's rows by long pieces; else a few
+// columns of every sequence.  1024 sequences of 4000 tokens in groups of 8: TBD us by blocks, 18 by columns, whose rows, 16 KB apart, meet in few
+// channels.  The lengths, which every work-group reads, are written by the one that arrives last.
+constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 16 sequences of 256, or 4096 of one
 
 struct HistSeq {
     int from, past, after, row0;   // from: the sequence that it goes on as, or -1
@@ -38,55 +40,83 @@ template <int W>
 __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, const int *__restrict__ parent, const int *__restrict__ rows,
                                                                const int *__restrict__ ids, int nRows, int prompt, int width_log2) {
     typedef std::conditional_t<W == 4, i32x4, int> piece;
-    // neighbouring columns, which share cache lines, to one XCD: consecutive work-groups go round the eight
-    const int xcd = blockIdx.x & 7, slabs = gridDim.x, slab = xcd * (slabs >> 3) + min(xcd, slabs & 7) + (blockIdx.x >> 3);
-    const int tid = threadIdx.x, threads = blockDim.x, width = 1 << width_log2, c = W * ((slab << width_log2) + (tid & (width - 1)));
-    const int per = threads >> width_log2, s0 = tid >> width_log2;   // sequences at once; this thread's first
-    piece value[HIST_ITEMS];
-    uint32_t moved = 0, grown = 0;
-    int past[HIST_ITEMS], after[HIST_ITEMS];
+    const int tid = threadIdx.x;
+    // sequence s0 + i * per for i < HIST_ITEMS, where below `end`; pieces at column c
+    auto move = [&](int s0, int per, int end, int c) {
+        piece value[HIST_ITEMS];
+        uint32_t moved = 0, grown = 0;
+        int past[HIST_ITEMS], after[HIST_ITEMS];
 #pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i) {
-        const int s = s0 + i * per;
-        past[i] = after[i] = 0;
-        if (s < h.nSeq) {
-            const HistSeq q = hist_seq(h, parent, rows, nRows, s);
-            past[i] = q.past;
-            after[i] = q.after;
-            if (q.from != s && c < q.past) {
-                value[i] = *reinterpret_cast<const piece *>(h.tokens + (size_t)q.from * h.room + c);
-                moved |= 1u << i;
+        for (int i = 0; i < HIST_ITEMS; ++i) {
+            const int s = s0 + i * per;
+            past[i] = after[i] = 0;
+            if (s < end) {
+                const HistSeq q = hist_seq(h, parent, rows, nRows, s);
+                past[i] = q.past;
+                after[i] = q.after;
+                if (q.from != s && c < q.past) {
+                    value[i] = *reinterpret_cast<const piece *>(h.tokens + (size_t)q.from * h.room + c);
+                    moved |= 1u << i;
+                }
+                if (q.after > q.past && c < q.after && c + W > q.past) grown |= 1u << i;   // so there are rows and ids
             }
-            if (q.after > q.past && c < q.after && c + W > q.past) grown |= 1u << i;   // so there are rows and ids
         }
+        // every token and length has been read: passing through here waits for the loads
+#pragma unroll
+        for (int i = 0; i < HIST_ITEMS; ++i) asm volatile("" : "+v"(value[i]) : : "memory");
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HIST_ITEMS; ++i) {
+            int *to = h.tokens + (size_t)(s0 + i * per) * h.room + c;
+            if (moved >> i & 1) {
+                if (c + W <= past[i]) *reinterpret_cast<piece *>(to) = value[i];
+                else if constexpr (W == 4)
+#pragma unroll
+                    for (int e = 0; e < W; ++e)
+                        if (c + e < past[i]) to[e] = value[i][e];
+            }
+            if (grown >> i & 1) {   // few: tokens that are appended
+                const int row0 = rows[s0 + i * per];
+                for (int e = max(0, past[i] - c); e < W && c + e < after[i]; ++e) to[e] = ids[row0 + (c + e - past[i])];
+            }
+        }
+    };
+    int block = 16;
+    if (h.nSeq > 16) {
+        __shared__ uint32_t fit;   // bit k: blocks of 9 + k
+        if (tid == 0) fit = 0xff;
+        __syncthreads();
+        uint32_t mine = 0xff;
+        if (parent)
+            for (int s = tid; s < h.nSeq; s += HIST_THREADS) {
+                const unsigned p = (unsigned)parent[s];
+                if (p < (unsigned)h.nSeq && p != (unsigned)s)
+#pragma unroll
+                    for (unsigned k = 0; k < 8; ++k)
+                        if ((unsigned)s / (9 + k) != p / (9 + k)) mine &= ~(1u << k);
+            }
+        if (mine != 0xff) atomicAnd(&fit, mine);
+        __syncthreads();
+        block = fit ? 9 + 31 - __builtin_clz(fit) : 0;
     }
-    // every token and length has been read: passing through here waits for the loads
-#pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i) asm volatile("" : "+v"(value[i]) : : "memory");
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < HIST_ITEMS; ++i) {
-        int *to = h.tokens + (size_t)(s0 + i * per) * h.room + c;
-        if (moved >> i & 1) {
-            if (c + W <= past[i]) *reinterpret_cast<piece *>(to) = value[i];
-            else if constexpr (W == 4)
-#pragma unroll
-                for (int e = 0; e < W; ++e)
-                    if (c + e < past[i]) to[e] = value[i][e];
+    if (block) {
+        const int chunks = (h.room + 256 * W - 1) / (256 * W), units = (h.nSeq + block - 1) / block * chunks;
+        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+            const int first = u / chunks * block;
+            move(first + (tid >> 8), 4, min(first + block, h.nSeq), W * ((u % chunks << 8) + (tid & 255)));
         }
-        if (grown >> i & 1) {   // few: tokens that are appended
-            const int row0 = rows[s0 + i * per];
-            for (int e = max(0, past[i] - c); e < W && c + e < after[i]; ++e) to[e] = ids[row0 + (c + e - past[i])];
-        }
+    } else {
+        const int slabs = (h.room + (W << width_log2) - 1) / (W << width_log2), width = 1 << width_log2;
+        for (int u = blockIdx.x; u < slabs; u += gridDim.x) move(tid >> width_log2, HIST_THREADS >> width_log2, h.nSeq, W * ((u << width_log2) + (tid & (width - 1))));
     }
     __shared__ int last;
+    // No fence: every length has been read ahead of a barrier, and what was written is for later kernels (a fence writes the L2 back: 19 us for 1024 sequences).
     if (tid == 0) {
-        __threadfence();
         last = atomicAdd(h.arrived, 1) == (int)gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
-    constexpr int LENS = GPT2_PKV_MAX_SEQ / 256;   // at most 4096 sequences, 256 threads at least
+    constexpr int LENS = GPT2_PKV_MAX_SEQ / HIST_THREADS, threads = HIST_THREADS;
     int len[LENS], start[LENS];
 #pragma unroll
     for (int i = 0; i < LENS; ++i) {
@@ -327,10 +357,10 @@ extern "C" void gpt2_history_step(GPT2History *h, const int *parent, const int *
     const int w = wide ? 4 : 1;
     int width = wide ? 4 : 6;   // log2 of the pieces of a row that a work-group takes: 256 bytes
     while ((h->nSeq << width) > HIST_THREADS * HIST_ITEMS) --width;
-    int threads = 256;
-    while (threads < HIST_THREADS && (h->nSeq << width) > threads) threads *= 2;
-    hipLaunchKernelGGL(wide ? k_history_step<4> : k_history_step<1>, dim3(cdiv(h->room, w << width)), dim3(threads), 0, stream(), *h, parent, rows, ids, nRows,
-                       prompt, width);
+    const long blocks = (long)cdiv(h->nSeq, 16) * cdiv(h->room, 256 * w), slabs = h->nSeq > 16 ? cdiv(h->room, w << width) : 1;
+    const long most = blocks > slabs ? blocks : slabs;
+    hipLaunchKernelGGL(wide ? k_history_step<4> : k_history_step<1>, dim3((unsigned)(most < 512 ? most : 512)), dim3(HIST_THREADS), 0, stream(), *h, parent, rows, ids,
+                       nRows, prompt, width);
     check_launch("k_history_step");
 }
 
