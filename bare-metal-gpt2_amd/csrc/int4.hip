@@ -504,8 +504,9 @@ static void rows_form(const Q4 &q, Q4RowsFn &fn, int &nt, int &kw) {
 }
 
 // A form for more rows, and what it takes in us: a round of work-groups `start` and `step` for each 128 k of a group of waves; each further work-group on a CU
-// that has room for `room` at once `start2` and `step2`.  Fitted to the times of 132 products of 17 to 2000 rows by 768 x 768 to 8192 x 8192 and 50257 x 768; the
-// form with the smallest sum is within 1.6% of the fastest of twelve in the mean, 14% at most.
+// that has room for `room` at once `start2` and `step2`.  Fitted to the times of 154 products of 17 to 2000 rows by 768 x 768 to 8192 x 8192 and 50257 x 768; the
+// form with the smallest sum is within 0.7% of the fastest of the nine in the mean, 9% at most, and without any one of them products are up to 1.18 to 1.5
+// times as long (the least, 16 x 64: 1.09).
 struct Q4Form {
     int bm, bn, ks, threads, room;
     float start, step, start2, step2;
@@ -518,13 +519,15 @@ static Q4Form q4_form(int room, float start, float step, float start2, float ste
 template <int G>
 static const Q4Form &tile_form(int M, int N, int kb, bool direct) {
     static const Q4Form by_loads[] = {
-        q4_form<G, 16, 32, 1, 1, 8, 2, false, true>(1, 1.51f, 0.91f, 0.f, 0.f),   q4_form<G, 32, 32, 1, 2, 4, 3, false, true>(1, 1.50f, 0.73f, 0.f, 0.f),
-        q4_form<G, 32, 64, 1, 2, 6, 2, true, true>(1, 2.41f, 1.31f, 0.f, 0.f),    q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.28f, 0.65f, 0.48f, 0.26f),
-        q4_form<G, 48, 64, 1, 2, 4, 2, false, true>(1, 2.50f, 1.18f, 0.f, 0.f),   q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.12f, 0.89f, 0.72f, 0.47f),
-        q4_form<G, 64, 128, 1, 4, 1, 3, false, true>(2, 1.83f, 0.80f, 1.93f, 0.38f), q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 2.85f, 1.17f, 3.69f, 0.86f)};
+        q4_form<G, 16, 32, 1, 1, 8, 2, false, true>(1, 1.54f, 0.91f, 0.f, 0.f),    q4_form<G, 16, 64, 1, 4, 3, 3, false, true>(2, 1.40f, 0.62f, 0.46f, 0.33f),
+        q4_form<G, 32, 32, 1, 2, 4, 3, false, true>(1, 1.53f, 0.72f, 0.f, 0.f),    q4_form<G, 32, 64, 1, 4, 4, 2, true, true>(1, 1.73f, 0.90f, 0.f, 0.f),
+        q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.33f, 0.62f, 0.43f, 0.28f), q4_form<G, 48, 64, 1, 4, 4, 2, true, true>(1, 1.88f, 1.11f, 0.f, 0.f),
+        q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.15f, 0.87f, 0.63f, 0.47f),  q4_form<G, 64, 128, 1, 4, 1, 3, false, true>(2, 1.76f, 0.80f, 1.85f, 0.36f),
+        q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 2.45f, 1.16f, 3.64f, 0.82f)};
+    // rows that are not at 16 bytes
     static const Q4Form by_registers[] = {
-        q4_form<G, 32, 32, 1, 2, 4, 2, true, false>(1, 1.50f, 0.73f, 0.f, 0.f), q4_form<G, 32, 64, 1, 4, 2, 2, true, false>(2, 1.28f, 0.65f, 0.48f, 0.26f),
-        q4_form<G, 64, 128, 1, 4, 1, 2, true, false>(2, 1.83f, 0.80f, 1.93f, 0.38f)};
+        q4_form<G, 32, 32, 1, 2, 4, 2, true, false>(1, 1.53f, 0.72f, 0.f, 0.f), q4_form<G, 32, 64, 1, 4, 2, 2, true, false>(2, 1.33f, 0.62f, 0.43f, 0.28f),
+        q4_form<G, 64, 128, 1, 4, 1, 2, true, false>(2, 1.76f, 0.80f, 1.85f, 0.36f)};
     const Q4Form *const forms = direct ? by_loads : by_registers, *best = forms;
     float least = INFINITY;
     for (const Q4Form *f = forms, *end = forms + (direct ? sizeof by_loads : sizeof by_registers) / sizeof *forms; f < end; ++f) {
