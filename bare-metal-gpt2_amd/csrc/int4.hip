@@ -522,7 +522,7 @@ static const Q4Form &tile_form(int M, int N, int kb, bool direct) {
         q4_form<G, 16, 32, 1, 1, 8, 2, false, true>(1, 1.54f, 0.91f, 0.f, 0.f),    q4_form<G, 16, 64, 1, 4, 3, 3, false, true>(2, 1.40f, 0.62f, 0.46f, 0.33f),
         q4_form<G, 32, 32, 1, 2, 4, 3, false, true>(1, 1.53f, 0.72f, 0.f, 0.f),    q4_form<G, 32, 64, 1, 4, 4, 2, true, true>(1, 1.73f, 0.90f, 0.f, 0.f),
         q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.33f, 0.62f, 0.43f, 0.28f), q4_form<G, 48, 64, 1, 4, 4, 2, true, true>(1, 1.88f, 1.11f, 0.f, 0.f),
-        q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.15f, 0.87f, 0.63f, 0.47f),  q4_form<G, 64, 128, 1, 4, 1, 3, false, true>(2, 1.76f, 0.80f, 1.85f, 0.36f),
+        q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.15f, 0.87f, 0.63f, 0.47f),  q4_form<G, 64, 128, 1, 4, 1, 2, true, true>(3, 1.70f, 0.78f, 1.66f, 0.33f),
         q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 2.45f, 1.16f, 3.64f, 0.82f)};
     // rows that are not at 16 bytes
     static const Q4Form by_registers[] = {
