@@ -159,7 +159,10 @@ static bool history_refused(const GPT2History *h, const char *what) {
 // A work-group has SLICE tokens of a row.  What the row's history says of each is counted in LDS: how often it was said since
 // `start`, whether it was said at all, whether it would end a known n-gram.  Of a bias list's entries for a token the last counts, by the largest
 // index, in a second table where there are biases.  The tokens that were said are listed as their first mention is counted; for those,
-// and the few that only have a bias, a thread each works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever the row begins, a byte of the mask.
+// and the few that only have a bias, a thread each works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever
+// the row begins, a byte of the mask.  256 rows of 50257 with masks, 300 biases and histories of up to 4096 take 24.5 us (2.3 TB/s), without any of them 15: every slice
+// goes through the row's whole history, and a work-group is a chain of lengths, tokens, counts and barriers.  Slices of 2048 take 28, 256 threads 30, rules worked out
+// where the row is copied 25 to 29 (nearly every wave then goes through all of them), claims by a second pass over the history 31.
 constexpr int SLICE = 4096, LOGIT_THREADS = 512, OCTETS = SLICE / 8 / LOGIT_THREADS;
 constexpr uint32_t SEEN = 1u << 31, BANNED = 1u << 30, COUNT = BANNED - 1;
 typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));

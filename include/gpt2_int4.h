@@ -17,7 +17,8 @@
  *   scales, 16 * 128 / group a tile: [n % 16 / 4][k % 128 / group][n % 4].
  * Codes past K are 0 (held as 8) and their groups' scales finite; rows past N mean nothing, but are read.
  *
- * Calls enqueue kernels on the stream of gpt2_set_stream and do nothing else, so they can be captured; errors as in gpt2_kernels.h.
+ * Every call but alloc and free only enqueues kernels on the stream of gpt2_set_stream, so it can be captured; there is no workspace, and calls may overlap.  Errors
+ * as in gpt2_kernels.h.
  */
 #ifndef GPT2_INT4_H
 #define GPT2_INT4_H
@@ -50,8 +51,8 @@ void gpt2_dequantize_int4(gpt2_half *dst, const GPT2Int4W *w);
 #define GPT2_EPI_NONE 0
 #define GPT2_EPI_GELU 1
 #define GPT2_EPI_ADD 2
-/* C[M][N] as above; bias [N] or NULL; resid [M][N], with GPT2_EPI_ADD only, may be C.  A, C, bias and resid need the alignment of
- * their type only; A with rows at 16 bytes (K % 8 == 0) is read by wider loads. */
+/* C[M][N] as above, M at most 2^21; bias [N] or NULL; resid [M][N], with GPT2_EPI_ADD only, may be C.  C overlaps neither A nor the weights.  A, C, bias and
+ * resid need the alignment of their type only; from 17 rows on, A with rows at 16 bytes (K % 8 == 0) is faster. */
 void gpt2_matmul_int4(gpt2_half *C, const gpt2_half *A, const GPT2Int4W *w, const gpt2_half *bias, int M, int epi,
                       const gpt2_half *resid);
 
