@@ -497,23 +497,23 @@ static void by_group(int group, F f) {
 typedef void (*Q4RowsFn)(uint16_t *, const uint16_t *, Q4, const uint16_t *, int, int, const uint16_t *, int);
 typedef void (*Q4TileFn)(uint16_t *, const uint16_t *, const uint32_t *, const uint16_t *, int, int, int, const uint16_t *, int, int, const uint16_t *, int, int, int, int);
 
-// The form for up to 16 rows: [one tile of outputs, two][waves].  us a call, one row unless said, NT x KW:
-//   few work-groups and long rows: 16 waves (2048 x 8192: 1 x 16 5.2, 1 x 8 6.5; 8192 x 8192: 2 x 16 8.8, 1 x 8 9.0, 1 x 16 9.6), up to eight rows, whose pieces leave
-//   room in the registers; else 8;
-//   four work-groups a CU and more: two tiles (50257 x 4096: 2 x 8 25.2, 1 x 8 26.7; 8 rows of 50257 x 768: 2 x 3 7.0, 1 x 3 7.2), one for up to four
-//   rows that are short (6.5, 6.7), and where a row is at most six tiles, three waves that have two each in flight (50257 x 768: 1 x 3 6.5, 1 x 8 8.1).
+// The form for up to 16 rows, NT tiles of outputs x KW waves.  us a call, one row unless said:
+//   768 tiles and more: 2 x 4 (16 rows of 16400 x 768 4.4, 1 x 8 for 16000 5.0; 50257 x 4096: 24.9, 2 x 8 25.2; x 1600, 16 rows: 16.4, 2 x 8 28.5, 1 x 4 with two tiles each under way 27.2), and for 5 to 8
+//   rows of at most six tiles, whose pieces leave room for two each, 2 x 3 (8 rows of 50257 x 768: 7.3, 2 x 4 8.1; one row 6.7 either way);
+//   fewer and long rows: 16 waves (2048 x 8192: 1 x 16 5.2, 1 x 8 6.5; 8192 x 8192: 2 x 16 8.8, 1 x 8 9.0, 1 x 16 9.6), 8 for more than eight rows, whose pieces
+//   would not leave the registers; else 1 x 8.
 template <int G, int RQ>
 static void rows_form(const Q4 &q, Q4RowsFn &fn, int &nt, int &kw) {
     const int tiles = cdiv(q.N, Q4_N);
     auto take = [&](Q4RowsFn f, int n, int k) { fn = f, nt = n, kw = k; };
-    if (tiles >= 1024 && q.kb <= 6) {
-        constexpr int NT = RQ == 1 ? 1 : 2;
-        return take(k_int4_rows<G, RQ, NT, 3, 2>, NT, 3);
+    if (tiles >= 768) {
+        if constexpr (RQ == 2)
+            if (q.kb <= 6) return take(k_int4_rows<G, RQ, 2, 3, 2>, 2, 3);
+        return take(k_int4_rows<G, RQ, 2, 4, 1>, 2, 4);
     }
-    const bool two = tiles >= 1024 || (tiles > 256 && q.kb >= 32);
-    if constexpr (RQ < 4)
-        if (tiles < 1024 && q.kb >= 32) return two ? take(k_int4_rows<G, RQ, 2, 16, 1>, 2, 16) : take(k_int4_rows<G, RQ, 1, 16, 1>, 1, 16);
-    return two ? take(k_int4_rows<G, RQ, 2, 8, 1>, 2, 8) : take(k_int4_rows<G, RQ, 1, 8, 1>, 1, 8);
+    if (q.kb < 32) return take(k_int4_rows<G, RQ, 1, 8, 1>, 1, 8);
+    if constexpr (RQ < 4) return tiles > 256 ? take(k_int4_rows<G, RQ, 2, 16, 1>, 2, 16) : take(k_int4_rows<G, RQ, 1, 16, 1>, 1, 16);
+    else return tiles > 256 ? take(k_int4_rows<G, RQ, 2, 8, 1>, 2, 8) : take(k_int4_rows<G, RQ, 1, 8, 1>, 1, 8);
 }
 
 // A form for more rows, and what it takes in us: a round of work-groups `start` and `step` for each 128 k of a group of waves; each further work-group on a CU
