@@ -156,42 +156,80 @@ static bool history_refused(const GPT2History *h, const char *what) {
 }
 
 // ------------------------------------------------------------------ logits
-// A work-group has SLICE tokens of a row.  What the row's history says of each is counted in LDS: how often it was said since
-// `start`, whether it was said at all, whether it would end a known n-gram.  Of a bias list's entries for a token the last counts, by the largest
-// index, in a second table where there are biases.  The tokens that were said are listed as their first mention is counted; for those,
-// and the few that only have a bias, a thread each works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever
-// the row begins, a byte of the mask.  256 rows of 50257 with masks, 300 biases and histories of up to 4096 take 24.5 us (2.3 TB/s), without any of them 15: every slice
-// goes through the row's whole history, and a work-group is a chain of lengths, tokens, counts and barriers.  Slices of 2048 take 28, 256 threads 30, rules worked out
-// where the row is copied 25 to 29 (nearly every wave then goes through all of them), claims by a second pass over the history 31.
-constexpr int SLICE = 4096, LOGIT_THREADS = 512, OCTETS = SLICE / 8 / LOGIT_THREADS;
-constexpr uint32_t SEEN = 1u << 31, BANNED = 1u << 30, COUNT = BANNED - 1;
+// A work-group has SLICE tokens of a row.  What the row's history says of each is counted in LDS: how often it was said since `start`, whether it was said at
+// all, whether it would end a known n-gram.  The tokens that were said are listed as their first mention is counted; for those, and those with a bias, a thread each
+// works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever the row begins, a byte of the mask.  An entry of the bias list marks
+// its token; only where a list is longer than the work-group, or a token has two, are entries compared for the last.
+// 256 rows of 50257 with masks, 300 biases and histories of up to 4096 take 20.0 us (2.8 TB/s), without any of them 14: every slice goes through the row's whole
+// history, and a work-group is a chain of lengths, tokens, counts and barriers.  Slices of 4096 with counts of 32 bits and a table for the biases' indexes took 24.4;
+// rules worked out where the row is copied, or claimed by a second pass over the history, 25 to 31 with either.
+// Counts have 16 bits where a history's room allows it.
+template <bool HALF>
+struct Said {
+    static constexpr uint32_t SEEN = HALF ? 0x8000u : 1u << 31, BANNED = SEEN >> 1, BIASED = SEEN >> 2, COUNT = BIASED - 1;
+    static constexpr int BYTES = HALF ? 2 : 4;
+    uint32_t *words;
+    __device__ __forceinline__ uint32_t add(unsigned t, uint32_t v) const {   // what it was before
+        if constexpr (HALF) return atomicAdd(&words[t >> 1], v << (16 * (t & 1))) >> (16 * (t & 1)) & 0xffffu;
+        else return atomicAdd(&words[t], v);
+    }
+    __device__ __forceinline__ uint32_t mark(unsigned t, uint32_t v) const {
+        if constexpr (HALF) return atomicOr(&words[t >> 1], v << (16 * (t & 1))) >> (16 * (t & 1)) & 0xffffu;
+        else return atomicOr(&words[t], v);
+    }
+    __device__ __forceinline__ void clear(unsigned t, uint32_t v) const {
+        if constexpr (HALF) atomicAnd(&words[t >> 1], ~(v << (16 * (t & 1))));
+        else atomicAnd(&words[t], ~v);
+    }
+    __device__ __forceinline__ uint32_t at(unsigned t) const {
+        if constexpr (HALF) return reinterpret_cast<const uint16_t *>(words)[t];
+        else return words[t];
+    }
+};
 typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 struct RowRules {
     float rep, freq, pres;
 };
+template <bool HALF>
 __device__ __forceinline__ float adjusted(float x, uint32_t said, float bias, const RowRules &r) {
     x += bias;
     if (said) {
         x = x > 0.f ? x / r.rep : x * r.rep;
-        const uint32_t n = said & COUNT;
+        const uint32_t n = said & Said<HALF>::COUNT;
         if (n) x -= __builtin_fmaf(r.freq, (float)n, r.pres);
-        if (said & BANNED) x = -INFINITY;
+        if (said & Said<HALF>::BANNED) x = -INFINITY;
     }
     return x;
 }
+// Bytes of LDS: what was said, counters, the list, the slice's logits, a piece of the bias list.
+template <int SLICE, int THREADS, bool HALF>
+constexpr int tables_bytes() { return SLICE * (Said<HALF>::BYTES + 2 + 2) + 16 + THREADS * 4; }
 
-constexpr int TABLES = SLICE * (4 + 2 + 2) + 16, BIAS_TABLE = SLICE * 4;   // bytes of LDS; the second where there are biases
-
-__global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, const uint16_t *logits, long ld, int V, GPT2LogitsRules r, GPT2History h) {
-    extern __shared__ __attribute__((aligned(16))) uint32_t tables[];
-    uint32_t *const said = tables, *const listed = tables + SLICE;
-    uint16_t *const list = reinterpret_cast<uint16_t *>(tables + SLICE + 4), *const value = list + SLICE;   // tokens that were said; the slice's logits
-    uint32_t *const bias_at = tables + TABLES / 4;
+template <int SLICE, int THREADS, bool HALF>
+__global__ __launch_bounds__(THREADS) void k_logits_adjust(uint16_t *out, const uint16_t *logits, long ld, int V, GPT2LogitsRules r, GPT2History h) {
+    __shared__ __attribute__((aligned(16))) uint32_t tables[tables_bytes<SLICE, THREADS, HALF>() / 4];
+    constexpr int OCTETS = SLICE / 8 / THREADS, WORDS = SLICE * Said<HALF>::BYTES / 4;
+    constexpr uint32_t SEEN = Said<HALF>::SEEN, COUNT = Said<HALF>::COUNT;
+    const Said<HALF> said = {tables};
+    uint32_t *const listed = tables + WORDS, *const biases = listed + 1, *const twice = listed + 2;   // how many are in the list, and in the piece; whether a token has two biases
+    uint16_t *const list = reinterpret_cast<uint16_t *>(tables + WORDS + 4), *const value = list + SLICE;   // tokens that were said; the slice's logits
+    uint32_t *const piece = tables + WORDS + 4 + SLICE;
     const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SLICE, nt = min(SLICE, V - t0);
     const uint16_t *x = logits + (size_t)row * ld + t0;
     uint16_t *y = out + (size_t)row * ld + t0;
+    // the octets, the thread's first tokens and its first bias are asked for together
+    u16x8_any v[OCTETS];
+    if (out != logits || r.n_masks)
+#pragma unroll
+        for (int o = 0; o < OCTETS; ++o) {
+            const int i = 8 * (tid + THREADS * o);
+            if (i + 8 <= nt) v[o] = *reinterpret_cast<const u16x8_any *>(x + i);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[o][e] = i + e < nt ? x[i + e] : 0;
+        }
     const int *tok = h.tokens ? h.tokens + (size_t)row * h.room : nullptr;
     const int len = tok ? min(max(h.len[row], 0), h.room) : 0, start = tok ? h.start[row] : 0;
     const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(r.bias_start[row + 1], r.n_bias) : 0;
@@ -202,30 +240,18 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
     }
     const bool sparse = out == logits && !mask;   // only what a rule names is touched
     const RowRules rules = {r.repetition ? r.repetition[row] : 1.f, r.frequency ? r.frequency[row] : 0.f, r.presence ? r.presence[row] : 0.f};
-    // the thread's first tokens, bias and octets are asked for together
     i32x4_any w0 = {};
     int bias_t0 = -1;
     float bias_v0 = 0.f;
     if (4 * tid + 4 <= len) w0 = *reinterpret_cast<const i32x4_any *>(tok + 4 * tid);
-    if (bias0 + tid < bias1) {
-        bias_t0 = r.bias_token[bias0 + tid];
-        bias_v0 = r.bias_value[bias0 + tid];
+    if (bias1 - 1 - tid >= bias0) {
+        bias_t0 = r.bias_token[bias1 - 1 - tid];
+        bias_v0 = r.bias_value[bias1 - 1 - tid];
     }
-    u16x8_any v[OCTETS];
     uint32_t allowed[OCTETS];
-    if (!sparse)
 #pragma unroll
-        for (int o = 0; o < OCTETS; ++o) {
-            const int i = 8 * (tid + LOGIT_THREADS * o);
-            allowed[o] = mask && i < nt ? mask[i >> 3] : 0xffu;
-            if (i + 8 <= nt) v[o] = *reinterpret_cast<const u16x8_any *>(x + i);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[o][e] = i + e < nt ? x[i + e] : 0;
-        }
-    for (int i = 4 * tid; i < SLICE + 4; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(tables + i) = i32x4{0, 0, 0, 0};
-    if (r.n_bias)
-        for (int i = 4 * tid; i < SLICE; i += 4 * LOGIT_THREADS) *reinterpret_cast<i32x4 *>(bias_at + i) = i32x4{0, 0, 0, 0};
+    for (int o = 0; o < OCTETS; ++o) allowed[o] = mask && 8 * (tid + THREADS * o) < nt ? mask[tid + THREADS * o] : 0xffu;
+    for (int i = 4 * tid; i < WORDS + 4; i += 4 * THREADS) *reinterpret_cast<i32x4 *>(tables + i) = i32x4{0, 0, 0, 0};
     __syncthreads();
     if (len) {
         const int last = r.ngram > 0 ? len - r.ngram : -1;   // n-grams begin at 0 .. last
@@ -236,7 +262,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
             bool same = true;
             for (int j = 1; j < r.ngram - 1 && same; ++j) same = tok[i + j] == tail[j];
             const unsigned end = (unsigned)(tok[i + r.ngram - 1] - t0);
-            if (same && end < (unsigned)nt) atomicOr(&said[end], BANNED);
+            if (same && end < (unsigned)nt) said.mark(end, Said<HALF>::BANNED);
         };
         // counts first, then the list of those that were new: one place of it for each of a wave's, by one addition
         auto take = [&](int i, const i32x4_any &w, int n) {
@@ -247,7 +273,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
             for (int e = 0; e < 4; ++e) {
                 const unsigned t = (unsigned)(w[e] - t0);
                 before[e] = SEEN;
-                if (e < n && t < (unsigned)nt) before[e] = i + e >= start ? atomicAdd(&said[t], 1u) : atomicOr(&said[t], SEEN);
+                if (e < n && t < (unsigned)nt) before[e] = i + e >= start ? said.add(t, 1u) : said.mark(t, SEEN);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -271,7 +297,7 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
                 for (int e = 0; e < 4; ++e)
                     if (e < n) ends(i + e, w[e]);
         };
-        for (int i = 4 * tid; i < len; i += 4 * LOGIT_THREADS) {
+        for (int i = 4 * tid; i < len; i += 4 * THREADS) {
             i32x4_any w = w0;
             if (i + 4 <= len) {
                 if (i != 4 * tid) w = *reinterpret_cast<const i32x4_any *>(tok + i);
@@ -281,33 +307,65 @@ __global__ __launch_bounds__(LOGIT_THREADS) void k_logits_adjust(uint16_t *out, 
             take(i, w, min(4, len - i));
         }
     }
-    for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {
-        const unsigned t = (unsigned)((i == bias0 + tid ? bias_t0 : r.bias_token[i]) - t0);
-        if (t < (unsigned)nt) atomicMax(&bias_at[t], (unsigned)i + 1);
-    }
+    // the thread's first bias takes the token with all its rules, and the list of what was said leaves it out; a second bias of a token is told
+    const unsigned bias_t = (unsigned)(bias_t0 - t0);
+    const bool biased = bias1 - 1 - tid >= bias0 && bias_t < (unsigned)nt;
+    if (biased && said.mark(bias_t, Said<HALF>::BIASED) & Said<HALF>::BIASED) *twice = 1;
     if (!sparse)
 #pragma unroll
-        for (int o = 0; o < OCTETS; ++o) *reinterpret_cast<i32x4 *>(value + 8 * (tid + LOGIT_THREADS * o)) = __builtin_bit_cast(i32x4, v[o]);
+        for (int o = 0; o < OCTETS; ++o) *reinterpret_cast<i32x4 *>(value + 8 * (tid + THREADS * o)) = __builtin_bit_cast(i32x4, v[o]);
     __syncthreads();
     auto put = [&](unsigned t, float bias) {
-        const uint16_t to = f2h(adjusted(h2f(sparse ? x[t] : value[t]), said[t], bias, rules));
+        const uint16_t to = f2h(adjusted<HALF>(h2f(sparse ? x[t] : value[t]), said.at(t) & ~Said<HALF>::BIASED, bias, rules));
         if (sparse) y[t] = to;
         else value[t] = to;
     };
-    for (int i = bias0 + tid; i < bias1; i += LOGIT_THREADS) {   // tokens that only have a bias
-        const bool is_first = i == bias0 + tid;
-        const unsigned t = (unsigned)((is_first ? bias_t0 : r.bias_token[i]) - t0);
-        if (t < (unsigned)nt && bias_at[t] == (unsigned)i + 1 && !said[t]) put(t, is_first ? bias_v0 : r.bias_value[i]);
+    if (bias1 - bias0 <= THREADS && !*twice) {
+        if (biased) put(bias_t, bias_v0);
+    } else {
+        // A long list, or a token with two biases: the list from its end, a piece of THREADS entries at a time; an entry counts if no later one of its piece, and none of a
+        // later piece, has its token.
+        if (biased) said.clear(bias_t, Said<HALF>::BIASED);
+        __syncthreads();
+        for (int end = bias1; end > bias0; end -= THREADS) {
+            const bool is_first = end == bias1;
+            const int i = end - 1 - tid;   // thread 0 has the last
+            unsigned t = ~0u;
+            float bias = 0.f;
+            if (i >= bias0) {
+                t = (unsigned)((is_first ? bias_t0 : r.bias_token[i]) - t0);
+                bias = is_first ? bias_v0 : r.bias_value[i];
+            }
+            const bool mine = t < (unsigned)nt && !(said.at(t) & Said<HALF>::BIASED);
+            if (mine) piece[atomicAdd(biases, 1u)] = t << 16 | (uint32_t)tid;
+            __syncthreads();
+            if (mine) {
+                bool counts = true;
+                for (int k = 0, n = (int)*biases; k < n; k += 8) {
+                    const i32x4 a = *reinterpret_cast<const i32x4 *>(piece + k), b = *reinterpret_cast<const i32x4 *>(piece + k + 4);   // what is past n is not looked at
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t other = (uint32_t)(e < 4 ? a[e & 3] : b[e & 3]);
+                        counts &= k + e >= n || (other >> 16) != t || (int)(other & 0xffffu) >= tid;
+                    }
+                }
+                if (counts) {
+                    put(t, bias);
+                    said.mark(t, Said<HALF>::BIASED);
+                }
+            }
+            __syncthreads();
+            if (tid == 0) *biases = 0;
+            if (end - THREADS > bias0) __syncthreads();
+        }
     }
-    for (int i = tid, n = *listed; i < n; i += LOGIT_THREADS) {
-        const unsigned t = list[i], at = r.n_bias ? bias_at[t] : 0u;
-        put(t, at ? r.bias_value[at - 1] : 0.f);
-    }
+    for (int i = tid, n = (int)*listed; i < n; i += THREADS)
+        if (!(said.at(list[i]) & Said<HALF>::BIASED)) put(list[i], 0.f);
     if (sparse) return;
     __syncthreads();
 #pragma unroll
     for (int o = 0; o < OCTETS; ++o) {
-        const int i = 8 * (tid + LOGIT_THREADS * o);
+        const int i = 8 * (tid + THREADS * o);
         if (i >= nt) break;
         u16x8_any to = __builtin_bit_cast(u16x8_any, *reinterpret_cast<const i32x4 *>(value + i));
 #pragma unroll
@@ -388,6 +446,11 @@ extern "C" void gpt2_logits_adjust(gpt2_half *out, const gpt2_half *logits, long
         arg_fail("gpt2_logits_adjust: bad rules");
         return;
     }
-    hipLaunchKernelGGL(k_logits_adjust, dim3(cdiv(V, SLICE), rows), dim3(LOGIT_THREADS), TABLES + (r.n_bias ? BIAS_TABLE : 0), stream(), out, logits, ld, V, r, h);
+    // 16-bit counts where a count cannot pass them, and slices of twice the length where there is a work-group of them for every CU (256 rows, histories of up to 600: 16.0 us
+    // for 19.5; 8 rows 5.1 for 4.8)
+    const bool half = !h.tokens || h.room <= (int)Said<true>::COUNT;
+    if (half && (long)rows * cdiv(V, 8192) >= 256)
+        hipLaunchKernelGGL((k_logits_adjust<8192, 512, true>), dim3(cdiv(V, 8192), rows), dim3(512), 0, stream(), out, logits, ld, V, r, h);
+    else hipLaunchKernelGGL((k_logits_adjust<4096, 512, false>), dim3(cdiv(V, 4096), rows), dim3(512), 0, stream(), out, logits, ld, V, r, h);
     check_launch("k_logits_adjust");
 }

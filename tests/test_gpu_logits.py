@@ -237,6 +237,35 @@ def test_counts_past_16_bits(pkg, L):
     assert got[0, 0] < -690
 
 
+@pytest.mark.parametrize("V,biases", [(900, 513), (9000, 1500), (9000, 9000), (20, 3000)])
+@pytest.mark.parametrize("rows", [3, 200])
+def test_long_bias_lists(pkg, L, V, biases, rows):
+    """Lists of more entries than a work-group has threads, of the whole vocabulary, of many entries for each token."""
+    rng = np.random.default_rng([V, biases, rows])
+    rules = Rules(pkg, rng, rows, V, [int(v) for v in rng.integers(0, 400, rows)], 2, biases if rows < 10 else biases // 5, rows // 2)
+    check(pkg, L, some_logits(rng, rows, V), rules, out_shift=0)
+    check(pkg, L, some_logits(rng, rows, V), rules)
+    rules.r.mask = None
+    rules.masks = [None] * rows
+    check(pkg, L, some_logits(rng, rows, V), rules)
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+def test_each_token_once(pkg, L, rows):
+    """Bias lists without a token twice, some of its tokens in the history and some not, as programs make them."""
+    rng = np.random.default_rng(rows)
+    V = 20000
+    rules = Rules(pkg, rng, rows, V, [150] * rows, 3, 0, 3, words=600)
+    dev = lambda a, t: rules.keep.append(pkg.Dev.from_numpy(np.asarray(a, t))) or rules.keep[-1].ptr  # noqa: E731
+    rules.biases = [list(zip([int(t) for t in np.concatenate([rng.permutation(V)[:250], sorted(set(s))[::3]])], rng.standard_normal(400).astype(np.float32).tolist())) for s in rules.seqs]
+    rules.biases = [list({t: v for t, v in b}.items()) for b in rules.biases]
+    flat = sum(rules.biases, [])
+    rules.r.n_bias, rules.r.bias_start = len(flat), dev(np.cumsum([0] + [len(b) for b in rules.biases]), np.int32)
+    rules.r.bias_token, rules.r.bias_value = dev([t for t, _ in flat], np.int32), dev([v for _, v in flat], np.float32)
+    check(pkg, L, some_logits(rng, rows, V), rules, out_shift=1)
+    check(pkg, L, some_logits(rng, rows, V), rules)
+
+
 # ----------------------------------------------------------------------------- histories
 class Pair:
     """Histories on the host and on the device."""
