@@ -12,7 +12,8 @@ namespace g2 {
 // ------------------------------------------------------------------ histories
 // All sequences change at once, in place: a work-group has what it moves in its registers before it writes any.  Where parents lie in their
 // children's block of R sequences (9 to 16: one is a multiple of any number of beams up to 16), it moves such a block's rows by long pieces; else a few
-// columns of every sequence.  1024 sequences of up to 4000 tokens in groups of 8: 8.6 us by blocks, 12.6 by columns, whose rows are 64 bytes each, 16 KB apart.  The lengths, which every work-group reads, are written by the one that arrives last.
+// columns of every sequence.  1024 sequences of up to 4000 tokens, with a copy of the lengths ahead: 12.3 us by blocks, in
+// groups of 8; 16.1 by columns, any sequence from any, whose rows are 64 bytes each, 16 KB apart.  The lengths, which every work-group reads, are written by the one that arrives last.
 constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 16 sequences of 256, or 4096 of one
 
 struct HistSeq {
