@@ -209,3 +209,22 @@ def test_same_bits_again(pkg, L):
         np.testing.assert_array_equal(a, run(pkg, L, c, weights=w))
         c.x[:m - 1] = 3
         np.testing.assert_array_equal(a[m - 1], run(pkg, L, c, weights=w)[m - 1])
+
+
+def test_outputs_past_4_gib(pkg, L):
+    """More than 2^32 bytes of results, from rows at 16 bytes and from others: the first and the last rows."""
+    for k in (32, 30):
+        m, n = 43000, 50257
+        c = Case(4, n, k, 32, bias=False)
+        rows = np.zeros((m, k), np.float16)
+        rows[:2], rows[-2:] = c.x[:2], c.x[2:]
+        w = Weights(pkg, c.codes, c.scales, 32)
+        d_a, d_c = pkg.Dev.from_numpy(rows), pkg.Dev(m * n * 2)
+        L.gpt2_matmul_int4(d_c.ptr, d_a.ptr, w.ref, None, m, 0, None)
+        L.gpt2_sync()
+        pkg.check("gpt2_matmul_int4")
+        got = np.empty((4, n), np.float16)
+        assert L.gpt2_d2h(got.ctypes.data, d_c.ptr, 4 * n) == 0 and L.gpt2_d2h(got[2:].ctypes.data, d_c.at((m - 2) * n * 2), 4 * n) == 0
+        want, tol = product(c.x, c.codes, c.scales, 32, None, 0, None)
+        assert (np.abs(got - want) <= tol).all()
+        d_c.free()

@@ -266,6 +266,26 @@ def test_each_token_once(pkg, L, rows):
     check(pkg, L, some_logits(rng, rows, V), rules)
 
 
+def test_logits_past_4_gib(pkg, L):
+    """Rows so far apart that the last begins past 2^32 bytes."""
+    rng = np.random.default_rng(3)
+    V, ld = 5000, 1 << 29
+    for masks in (0, 2):
+        rules = Rules(pkg, rng, 6, V, [30, 200, 0, 7, 90, 400], 2, 30, masks)
+        x = some_logits(rng, 6, V)
+        d = pkg.Dev((5 * ld + V) * 2)
+        for r in range(6):
+            assert L.gpt2_h2d(d.at(r * ld * 2), x[r].ctypes.data, V * 2) == 0
+        L.gpt2_logits_adjust(d.ptr, d.ptr, ld, 6, V, C.byref(rules.r))
+        L.gpt2_sync()
+        pkg.check("gpt2_logits_adjust")
+        got = np.empty((6, V), np.float16)
+        for r in range(6):
+            assert L.gpt2_d2h(got[r].ctypes.data, d.at(r * ld * 2), V * 2) == 0
+        same(got, *rules.want(x))
+        d.free()
+
+
 # ----------------------------------------------------------------------------- histories
 class Pair:
     """Histories on the host and on the device."""
@@ -318,6 +338,28 @@ def test_history(pkg, L, n, room):
     p.ref = Histories(n, room)
     p.check()
     p.dev.free()
+
+
+def test_history_past_4_gib(pkg, L):
+    """Rows past 2^32 bytes, by blocks and by columns, from others so far."""
+    rng = np.random.default_rng(12)
+    n, room = 80, 1 << 24
+    p = pkg.History(n, room)
+    oracle = Histories(n, room)
+    for t, parent in enumerate((None, np.arange(n) // 8 * 8, rng.permutation(n), None)):
+        counts = rng.integers(0, 300, n)
+        rows = np.cumsum([0] + counts.tolist())
+        ids = rng.integers(0, 50257, rows[-1])
+        d = [None if a is None else pkg.Dev.from_numpy(np.asarray(a, np.int32)) for a in (parent, rows, ids)]
+        L.gpt2_history_step(C.byref(p.h), *[v.ptr if v else None for v in d], len(ids), 0)
+        L.gpt2_sync()
+        pkg.check("gpt2_history_step")
+        oracle.step(parent, rows, ids, 0)
+        for s in range(n):
+            got = np.empty(len(oracle.seq[s]), np.int32)
+            assert L.gpt2_d2h(got.ctypes.data, p.h.tokens + 4 * s * room, got.nbytes) == 0
+            assert got.tolist() == oracle.seq[s]
+    p.free()
 
 
 def test_history_bad_offsets(pkg, L):
