@@ -102,15 +102,27 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
         __syncthreads();
         block = fit ? 9 + 31 - __builtin_clz(fit) : 0;
     }
-    if (block) {
-        const int chunks = (h.room + 256 * W - 1) / (256 * W), units = (h.nSeq + block - 1) / block * chunks;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int width = 1 << width_log2, blocks = block ? (h.nSeq + block - 1) / block : 0;
+    auto units = [&](int columns) { return block ? blocks * ((columns + 256 * W - 1) / (256 * W)) : (columns + (W << width_log2) - 1) / (W << width_log2); };
+    int longest = h.room;
+    if (units(h.room) > (int)gridDim.x) {   // room for far more than there may be: as far as the longest goes
+        __shared__ int most;
+        if (tid == 0) most = 0;
+        __syncthreads();
+        int mine = 0;
+        for (int s = tid; s < h.nSeq; s += HIST_THREADS) mine = max(mine, hist_seq(h, parent, rows, nRows, s).after);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) mine = max(mine, __shfl_xor(mine, o, 64));
+        if ((tid & 63) == 0) atomicMax(&most, mine);
+        __syncthreads();
+        longest = most;
+    }
+    const int n = units(longest), chunks = block ? max(1, n / blocks) : 1;
+    for (int u = blockIdx.x; u < n; u += gridDim.x) {
+        if (block) {
             const int first = u / chunks * block;
             move(first + (tid >> 8), 4, min(first + block, h.nSeq), W * ((u % chunks << 8) + (tid & 255)));
-        }
-    } else {
-        const int slabs = (h.room + (W << width_log2) - 1) / (W << width_log2), width = 1 << width_log2;
-        for (int u = blockIdx.x; u < slabs; u += gridDim.x) move(tid >> width_log2, HIST_THREADS >> width_log2, h.nSeq, W * ((u << width_log2) + (tid & (width - 1))));
+        } else move(tid >> width_log2, HIST_THREADS >> width_log2, h.nSeq, W * ((u << width_log2) + (tid & (width - 1))));
     }
     __shared__ int last;
     // No fence: every length has been read ahead of a barrier, and what was written is for later kernels (a fence writes the L2 back: 19 us for 1024 sequences).

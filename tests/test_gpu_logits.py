@@ -313,13 +313,13 @@ class Pair:
         np.testing.assert_array_equal(tokens, self.mem)
 
 
-@pytest.mark.parametrize("n,room", [(1, 1), (1, 64), (8, 1024), (7, 333), (64, 100), (255, 70), (257, 129), (1000, 17), (1025, 80), (4096, 33)])
+@pytest.mark.parametrize("n,room", [(5, 300000), (300, 20000), (100, 50001), (1, 1), (1, 64), (8, 1024), (7, 333), (64, 100), (255, 70), (257, 129), (1000, 17), (1025, 80), (4096, 33)])
 def test_history(pkg, L, n, room):
     rng = np.random.default_rng(n)
     p = Pair(pkg, L, n, room)
     p.check()
     for t in range(7):
-        counts = rng.integers(0, max(2, room // 2), n) * (rng.random(n) < 0.7) if t in (0, 3) else np.ones(n, int)
+        counts = rng.integers(0, max(2, min(room // 2, 1500)), n) * (rng.random(n) < 0.7) if t in (0, 3) else np.ones(n, int)
         rows = np.cumsum([0] + counts.tolist())
         ids = rng.integers(0, 50257, rows[-1])
         parent = None if t in (0, 4) else rng.integers(0, n, n)
