@@ -47,14 +47,24 @@ __device__ __forceinline__ f16x8 q4_values(uint32_t w, const Q4Bits &k) {
 
 // Eight consecutive halves of a row of K from k on, 0 past its end; rows at any alignment.
 typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint16_t u16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ f16x8 q4_eight(const uint16_t *at) { return __builtin_bit_cast(f16x8, *reinterpret_cast<const u16x8_any *>(at)); }
+// Where the row ends inside the octet, its last eight are loaded and moved down.
 __device__ __forceinline__ f16x8 q4_octet(const uint16_t *row, int k, int K) {
     f16x8 v = {};
-    if (k + 8 <= K) v = q4_eight(row + k);
-    else
+    if (K >= 8) {
+        const int past = k + 8 - K;   // halves past the end
+        const i32x4 w = __builtin_bit_cast(i32x4, q4_eight(row + min(k, K - 8)));
+        if (past <= 0) return __builtin_bit_cast(f16x8, w);
+        if (past >= 8) return v;
+        const uint64_t lo = (uint64_t)(uint32_t)w[1] << 32 | (uint32_t)w[0], hi = (uint64_t)(uint32_t)w[3] << 32 | (uint32_t)w[2];
+        const int bits = 16 * past;
+        const uint64_t a = bits < 64 ? lo >> bits | hi << (64 - bits) : hi >> (bits - 64), b = bits < 64 ? hi >> bits : 0;
+        return __builtin_bit_cast(f16x8, i32x4{(int)a, (int)(a >> 32), (int)b, (int)(b >> 32)});
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (k + e < K) v[e] = __builtin_bit_cast(f16, row[k + e]);
+    for (int e = 0; e < 8; ++e)
+        if (k + e < K) v[e] = __builtin_bit_cast(f16, row[k + e]);
     return v;
 }
 
@@ -150,30 +160,28 @@ __device__ __forceinline__ uint16_t q4_round(float v) {
 }
 
 // A lane's four outputs n .. n + 3 of row m: bias, what follows in fp32 (gelu_new as v / (1 + 2^(K (v + 0.044715 v^3))), K = -2 sqrt(2 / pi) log2(e);
-// or the residual), one rounding.  vec_c: C's rows, and the residual's, are at 8 bytes and N is a multiple of 4.
+// or the residual), one rounding.  Four halves go as one piece wherever a row begins (by halves 1059 rows of 10543 x 139 and a residual took 104 us).
 template <int EPI>
-__device__ __forceinline__ void q4_store(uint16_t *C, f32x4 v, int n, int m, int M, int N, const uint16_t *bias, const uint16_t *resid, int vec_c) {
+__device__ __forceinline__ void q4_store(uint16_t *C, f32x4 v, int n, int m, int M, int N, const uint16_t *bias, const uint16_t *resid) {
     if (m >= M || n >= N) return;
     const size_t at = (size_t)m * N + n;
-    uint16_t o[4];
-    if (vec_c) {
-        uint2 r = {};
-        if constexpr (EPI == GPT2_EPI_ADD) r = *reinterpret_cast<const uint2 *>(resid + at);
+    if (n + 4 <= N) {
+        u16x4_any b = {}, r = {}, o;
+        if (bias) b = *reinterpret_cast<const u16x4_any *>(bias + n);
+        if constexpr (EPI == GPT2_EPI_ADD) r = *reinterpret_cast<const u16x4_any *>(resid + at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float y = v[i] + (bias ? h2f(bias[n + i]) : 0.f);
-            if constexpr (EPI == GPT2_EPI_ADD) y = h2f((uint16_t)((i < 2 ? r.x : r.y) >> (16 * (i & 1)))) + y;
+            float y = v[i] + h2f(b[i]);
+            if constexpr (EPI == GPT2_EPI_ADD) y = h2f(r[i]) + y;
             o[i] = q4_round<EPI>(y);
         }
-        *reinterpret_cast<uint2 *>(C + at) = uint2{(uint32_t)o[0] | (uint32_t)o[1] << 16, (uint32_t)o[2] | (uint32_t)o[3] << 16};
+        *reinterpret_cast<u16x4_any *>(C + at) = o;
     } else
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) {
-                float y = v[i] + (bias ? h2f(bias[n + i]) : 0.f);
-                if constexpr (EPI == GPT2_EPI_ADD) y = h2f(resid[at + i]) + y;
-                C[at + i] = q4_round<EPI>(y);
-            }
+        for (int i = 0; n + i < N; ++i) {
+            float y = (i == 0 ? v[0] : i == 1 ? v[1] : v[2]) + (bias ? h2f(bias[n + i]) : 0.f);
+            if constexpr (EPI == GPT2_EPI_ADD) y = h2f(resid[at + i]) + y;
+            C[at + i] = q4_round<EPI>(y);
+        }
 }
 // f(epilogue as a constant)
 template <class F>
@@ -195,7 +203,7 @@ __device__ __forceinline__ void by_epilogue(int epi, F f) {
 // round of loads.  A tile of codes takes 36 vector instructions to become fp16 (with both masks as literals 52: 9.2 us for 8.9).
 template <int G, int RQ, int NT, int KW, int U>
 __global__ __launch_bounds__(64 * KW) void k_int4_rows(uint16_t *C, const uint16_t *__restrict__ A, Q4 w, const uint16_t *__restrict__ bias, int M, int epi,
-                                                       const uint16_t *resid, int vec_c) {
+                                                       const uint16_t *resid) {
     constexpr int PER = Q4_K / G, ROWS = 4 * RQ, STAGE = ROWS * 256, SUMS = KW * NT * 1024;
     static_assert(ROWS <= 16, "rows of one tile");
     __shared__ __attribute__((aligned(1024))) char lds[KW * STAGE > SUMS ? KW * STAGE : SUMS];
@@ -276,7 +284,7 @@ __global__ __launch_bounds__(64 * KW) void k_int4_rows(uint16_t *C, const uint16
         f32x4 v = sums[a * KW * 64 + lane];
 #pragma unroll
         for (int i = 1; i < KW; ++i) v += sums[(a * KW + i) * 64 + lane];
-        by_epilogue(epi, [&](auto k) { q4_store<k.value>(C, v, (tn0 + a) * Q4_N + 4 * g, l16, M, w.N, bias, resid, vec_c); });
+        by_epilogue(epi, [&](auto k) { q4_store<k.value>(C, v, (tn0 + a) * Q4_N + 4 * g, l16, M, w.N, bias, resid); });
     }
 }
 
@@ -292,7 +300,7 @@ __device__ __attribute__((aligned(16))) uint32_t g_q4_zero[4] = {};   // what is
 
 template <int G, int BM, int BN, int WM, int WN, int KS, int S, bool SREG, bool DIRECT>
 __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restrict__ A, const uint32_t *__restrict__ codes, const uint16_t *__restrict__ scales,
-                                          int N, int K, int kb, const uint16_t *__restrict__ bias, int M, int epi, const uint16_t *resid, int vec_c, int tiles_m,
+                                          int N, int K, int kb, const uint16_t *__restrict__ bias, int M, int epi, const uint16_t *resid, int tiles_m,
                                           int tiles, int along_n) {
 #if defined(__HIP_DEVICE_COMPILE__)   // LDS address-space pointers exist only in the device pass
     constexpr int PER = Q4_K / G, NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -466,15 +474,15 @@ __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restric
 #pragma unroll
         for (int a = 0; a < TN; ++a)
 #pragma unroll
-            for (int b = 0; b < TM; ++b) q4_store<e.value>(C, acc[a][b], (tn0 + wn0 + a) * Q4_N + 4 * g, m0 + wm0 + 16 * b + l16, M, N, bias, resid, vec_c);
+            for (int b = 0; b < TM; ++b) q4_store<e.value>(C, acc[a][b], (tn0 + wn0 + a) * Q4_N + 4 * g, m0 + wm0 + 16 * b + l16, M, N, bias, resid);
     });
 #endif
 }
 template <int G, int BM, int BN, int WM, int WN, int KS, int S, bool SREG, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN * KS) void k_int4_tile(uint16_t *C, const uint16_t *__restrict__ A, const uint32_t *__restrict__ codes, const uint16_t *__restrict__ scales,
-                                          int N, int K, int kb, const uint16_t *__restrict__ bias, int M, int epi, const uint16_t *resid, int vec_c, int tiles_m,
+                                          int N, int K, int kb, const uint16_t *__restrict__ bias, int M, int epi, const uint16_t *resid, int tiles_m,
                                           int tiles, int along_n) {
-    int4_tile<G, BM, BN, WM, WN, KS, S, SREG, DIRECT>(C, A, codes, scales, N, K, kb, bias, M, epi, resid, vec_c, tiles_m, tiles, along_n);
+    int4_tile<G, BM, BN, WM, WN, KS, S, SREG, DIRECT>(C, A, codes, scales, N, K, kb, bias, M, epi, resid, tiles_m, tiles, along_n);
 }
 
 static bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
@@ -494,8 +502,8 @@ static void by_group(int group, F f) {
     else f(std::integral_constant<int, 128>{});
 }
 
-typedef void (*Q4RowsFn)(uint16_t *, const uint16_t *, Q4, const uint16_t *, int, int, const uint16_t *, int);
-typedef void (*Q4TileFn)(uint16_t *, const uint16_t *, const uint32_t *, const uint16_t *, int, int, int, const uint16_t *, int, int, const uint16_t *, int, int, int, int);
+typedef void (*Q4RowsFn)(uint16_t *, const uint16_t *, Q4, const uint16_t *, int, int, const uint16_t *);
+typedef void (*Q4TileFn)(uint16_t *, const uint16_t *, const uint32_t *, const uint16_t *, int, int, int, const uint16_t *, int, int, const uint16_t *, int, int, int);
 
 // The form for up to 16 rows, NT tiles of outputs x KW waves.  us a call, one row unless said:
 //   768 tiles and more: 2 x 4 (16 rows of 16400 x 768 4.4, 1 x 8 for 16000 5.0; 50257 x 4096: 24.9, 2 x 8 25.2; x 1600, 16 rows: 16.4, 2 x 8 28.5, 1 x 4 with two tiles each under way 27.2), and for 5 to 8
@@ -611,7 +619,6 @@ extern "C" void gpt2_matmul_int4(gpt2_half *C, const gpt2_half *A, const GPT2Int
         return;
     }
     const Q4 q = {(const uint32_t *)w->codes, w->scales, w->N, w->K, cdiv(w->K, Q4_K)};
-    const int vec_c = w->N % 4 == 0 && !(((uintptr_t)C | (uintptr_t)resid) & 7);
     by_group(w->group, [&](auto group) {
         constexpr int G = group.value;
         if (M <= 16) {
@@ -620,7 +627,7 @@ extern "C" void gpt2_matmul_int4(gpt2_half *C, const gpt2_half *A, const GPT2Int
             if (M <= 4) rows_form<G, 1>(q, fn, nt, kw);
             else if (M <= 8) rows_form<G, 2>(q, fn, nt, kw);
             else rows_form<G, 4>(q, fn, nt, kw);
-            hipLaunchKernelGGL(fn, dim3(cdiv(cdiv(q.N, Q4_N), nt)), dim3(64 * kw), 0, stream(), C, A, q, bias, M, epi, resid, vec_c);
+            hipLaunchKernelGGL(fn, dim3(cdiv(cdiv(q.N, Q4_N), nt)), dim3(64 * kw), 0, stream(), C, A, q, bias, M, epi, resid);
             return;
         }
         const Q4Form &f = tile_form<G>(M, q.N, q.kb, w->K % 8 == 0 && aligned16(A));
@@ -629,7 +636,7 @@ extern "C" void gpt2_matmul_int4(gpt2_half *C, const gpt2_half *A, const GPT2Int
         // an XCD's run of tiles goes along n where the eight of them then read less: all codes once for each of up to eight rows of tiles, or all of A once for
         // each of up to eight columns (2000 x 4096 x 4096: 64 x 128 tiles 89.3 -> 84.7 us)
         const int along_n = 2.0 * M + 0.5 * q.N * (tm < 8 ? tm : 8) < 0.5 * q.N + 2.0 * M * (tn < 8 ? tn : 8);
-        hipLaunchKernelGGL(f.fn, dim3(tm * tn), dim3(f.threads), 0, stream(), C, A, q.codes, q.scales, q.N, q.K, q.kb, bias, M, epi, resid, vec_c, tm, tm * tn, along_n);
+        hipLaunchKernelGGL(f.fn, dim3(tm * tn), dim3(f.threads), 0, stream(), C, A, q.codes, q.scales, q.N, q.K, q.kb, bias, M, epi, resid, tm, tm * tn, along_n);
     });
     check_launch("gpt2_matmul_int4");
 }
