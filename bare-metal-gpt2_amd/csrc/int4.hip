@@ -361,13 +361,13 @@ __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restric
     const Q4Bits bits;
     f32x4 acc[TN][TM] = {};
     f16x4 s_now[SREG ? TN : 1][PER], s_next[SREG ? TN : 1][PER];
-    auto load_scales = [&](int t) {   // into s_next, ahead of a stage's other loads
+    auto load_scales = [&](f16x4 (&to)[SREG ? TN : 1][PER], int t) {
         const int tk = min(k_first + t, kb - 1);
 #pragma unroll
         for (int a = 0; a < TN; ++a)
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                s_next[a][j] = *reinterpret_cast<const f16x4 *>(scales + ((size_t)min(tn0 + wn0 + a, tns - 1) * kb + tk) * (16 * PER) + (g * PER + j) * 4);
+                to[a][j] = *reinterpret_cast<const f16x4 *>(scales + ((size_t)min(tn0 + wn0 + a, tns - 1) * kb + tk) * (16 * PER) + (g * PER + j) * 4);
     };
     auto compute = [&](int t) {
         const char *const st = ring + (t % S) * STAGE;
@@ -410,11 +410,11 @@ __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restric
             for (int a = 0; a < TN; ++a)
 #pragma unroll
                 for (int j = 0; j < PER; ++j) s_now[a][j] = s_next[a][j];
-            load_scales(t);
+            load_scales(s_next, t);   // ahead of a stage's other loads
         }
     };
-    if constexpr (SREG) load_scales(0);
     if constexpr (DIRECT) {
+        if constexpr (SREG) load_scales(s_next, 0);
 #pragma unroll
         for (int t = 0; t < S - 1; ++t)
             if (t < steps) issue(t);
@@ -447,7 +447,7 @@ __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restric
         put(0);
         for (int t = 0; t < steps; ++t) {
             __syncthreads();
-            next_scales(t + 1);
+            load_scales(s_now, t);   // needed behind the products
             if (t + 1 < steps) fetch(t + 1);
             if (KS == 1 || k_first + t < kb) compute(t);
             if (t + 1 < steps) put(t + 1);
@@ -478,8 +478,9 @@ __device__ __forceinline__ void int4_tile(uint16_t *C, const uint16_t *__restric
     });
 #endif
 }
+// Two waves a SIMD for the form through registers with four waves, which the compiler would give up for earlier loads (1272 rows of 4742 x 517, groups of 32: 33 us for 23).
 template <int G, int BM, int BN, int WM, int WN, int KS, int S, bool SREG, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN * KS) void k_int4_tile(uint16_t *C, const uint16_t *__restrict__ A, const uint32_t *__restrict__ codes, const uint16_t *__restrict__ scales,
+__global__ __launch_bounds__(64 * WM * WN * KS, !DIRECT && WM * WN * KS == 4 ? 2 : 1) void k_int4_tile(uint16_t *C, const uint16_t *__restrict__ A, const uint32_t *__restrict__ codes, const uint16_t *__restrict__ scales,
                                           int N, int K, int kb, const uint16_t *__restrict__ bias, int M, int epi, const uint16_t *resid, int tiles_m,
                                           int tiles, int along_n) {
     int4_tile<G, BM, BN, WM, WN, KS, S, SREG, DIRECT>(C, A, codes, scales, N, K, kb, bias, M, epi, resid, tiles_m, tiles, along_n);
