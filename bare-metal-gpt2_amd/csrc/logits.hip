@@ -245,7 +245,7 @@ __global__ __launch_bounds__(THREADS) void k_logits_adjust(uint16_t *out, const 
         }
     const int *tok = h.tokens ? h.tokens + (size_t)row * h.room : nullptr;
     const int len = tok ? min(max(h.len[row], 0), h.room) : 0, start = tok ? h.start[row] : 0;
-    const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(r.bias_start[row + 1], r.n_bias) : 0;
+    const int bias0 = r.n_bias ? min(max(r.bias_start[row], 0), r.n_bias) : 0, bias1 = r.n_bias ? min(max(r.bias_start[row + 1], 0), r.n_bias) : 0;
     const uint8_t *mask = nullptr;
     if (r.n_masks) {
         const int m = r.mask_row ? r.mask_row[row] : row;
