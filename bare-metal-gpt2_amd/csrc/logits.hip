@@ -35,6 +35,9 @@ __device__ __forceinline__ HistSeq hist_seq(const GPT2History &h, const int *__r
     return q;
 }
 
+// Waits for the wave's loads.  A barrier alone waits for nothing but LDS, and a load whose value is used behind it may still be under way.
+__device__ __forceinline__ void all_loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // A thread's pieces are W consecutive tokens (4 where rows lie at 16 bytes, else 1).
 template <int W>
 __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, const int *__restrict__ parent, const int *__restrict__ rows,
@@ -61,9 +64,7 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
                 if (q.after > q.past && c < q.after && c + W > q.past) grown |= 1u << i;   // so there are rows and ids
             }
         }
-        // every token and length has been read: passing through here waits for the loads
-#pragma unroll
-        for (int i = 0; i < HIST_ITEMS; ++i) asm volatile("" : "+v"(value[i]) : : "memory");
+        all_loaded();   // every token that is moved over, and every length that the last work-group writes over
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < HIST_ITEMS; ++i) {
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
         } else move(tid >> width_log2, HIST_THREADS >> width_log2, h.nSeq, W * ((u << width_log2) + (tid & (width - 1))));
     }
     __shared__ int last;
-    // No fence: every length has been read ahead of a barrier, and what was written is for later kernels (a fence writes the L2 back: 19 us for 1024 sequences).
+    // No fence: every length has been read ahead of a barrier (move, or the exchange of the longest), and what was written is for later kernels (a fence writes the L2 back: 19 us for 1024 sequences).
     if (tid == 0) {
         last = atomicAdd(h.arrived, 1) == (int)gridDim.x - 1;
     }
@@ -143,6 +144,7 @@ __global__ __launch_bounds__(HIST_THREADS) void k_history_step(GPT2History h, co
             start[i] = prompt && q.after > q.past ? q.after : q.from < 0 ? 0 : h.start[q.from];
         }
     }
+    all_loaded();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < LENS; ++i) {
