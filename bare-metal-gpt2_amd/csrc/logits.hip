@@ -17,7 +17,7 @@ namespace g2 {
 constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 16 sequences of 256, or 4096 of one
 
 struct HistSeq {
-    int from, past, after, row0;   // from: the sequence that it goes on as, or -1
+    int from, past, after;   // from: the sequence that it goes on as, or -1
 };
 __device__ __forceinline__ HistSeq hist_seq(const GPT2History &h, const int *__restrict__ parent, const int *__restrict__ rows, int nRows, int s) {
     HistSeq q;
@@ -30,7 +30,6 @@ __device__ __forceinline__ HistSeq hist_seq(const GPT2History &h, const int *__r
         b = rows[s + 1];
         if (a < 0 || b < a || b > nRows) a = b = 0;
     }
-    q.row0 = a;
     q.after = q.past + min(b - a, h.room - q.past);
     return q;
 }
