@@ -508,7 +508,9 @@ typedef void (*Q4TileFn)(uint16_t *, const uint16_t *, const uint32_t *, const u
 
 // The form for up to 16 rows, NT tiles of outputs x KW waves.  us a call, one row unless said:
 //   768 tiles and more: 2 x 4 (16 rows of 16400 x 768 4.4, 1 x 8 for 16000 5.0; 50257 x 4096: 24.9, 2 x 8 25.2; x 1600, 16 rows: 16.4, 2 x 8 28.5, 1 x 4 with two tiles each under way 27.2), and for 5 to 8
-//   rows of at most six tiles, whose pieces leave room for two each, 2 x 3 (8 rows of 50257 x 768: 7.3, 2 x 4 8.1; one row 6.7 either way);
+//   rows of five or six tiles along k, which three waves take in one round of two and four in two rounds, 2 x 3 (8 rows of 50257 x 768, groups of 128: 7.1, 2 x 4 7.7; x 640 6.7 and 7.3;
+//   100000 x 768 10.5 and 11.5).  Not of four tiles or fewer (50257 x 512: 6.4, 2 x 4 5.7; x 256 5.2 and 4.5), and not in groups of 32, whose scales leave its registers two
+//   work-groups a CU (50257 x 768: 8.4, 2 x 4 8.2; x 510 10.2 and 6.7);
 //   fewer and long rows: 16 waves (2048 x 8192: 1 x 16 5.2, 1 x 8 6.5; 8192 x 8192: 2 x 16 8.8, 1 x 8 9.0, 1 x 16 9.6), 8 for more than eight rows, whose pieces
 //   would not leave the registers; else 1 x 8.
 template <int G, int RQ>
@@ -516,8 +518,8 @@ static void rows_form(const Q4 &q, Q4RowsFn &fn, int &nt, int &kw) {
     const int tiles = cdiv(q.N, Q4_N);
     auto take = [&](Q4RowsFn f, int n, int k) { fn = f, nt = n, kw = k; };
     if (tiles >= 768) {
-        if constexpr (RQ == 2)
-            if (q.kb <= 6) return take(k_int4_rows<G, RQ, 2, 3, 2>, 2, 3);
+        if constexpr (RQ == 2 && G > 32)
+            if (q.kb == 5 || q.kb == 6) return take(k_int4_rows<G, RQ, 2, 3, 2>, 2, 3);
         return take(k_int4_rows<G, RQ, 2, 4, 1>, 2, 4);
     }
     if (q.kb < 32) return take(k_int4_rows<G, RQ, 1, 8, 1>, 1, 8);
