@@ -548,12 +548,13 @@ static const Q4Form &tile_form(int M, int N, int kb, bool direct) {
         q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.33f, 0.62f, 0.43f, 0.28f), q4_form<G, 48, 64, 1, 4, 4, 2, true, true>(1, 1.88f, 1.11f, 0.f, 0.f),
         q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.15f, 0.87f, 0.63f, 0.47f),  q4_form<G, 64, 128, 1, 4, 1, 2, true, true>(3, 1.70f, 0.78f, 1.66f, 0.33f),
         q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 2.45f, 1.16f, 3.64f, 0.82f)};
-    // Rows that are not at 16 bytes: fitted to 126 products alike, K from 300 to 8190; within 0.6% in the mean.  Without 16 x 64 products are up to 1.46 times as
-    // long, without the others 1.2 to 1.5; by three of these forms with the figures above 777 rows of 768 x 3070 took 17.7 us for 15.2, 64 of 3072 x 770 7.2 for 5.3.
+    // Rows that are not at 16 bytes: fitted to the times of 580 products, 17 to 2000 rows, N from 66 to 50257, K from 139 to 8175, each in groups of 32, 64 and 128: within 0.2% of the fastest of the six in the
+    // mean, 13% at most; fitted to the first 460, 0.4% and 11% on the others.  Without any one of them products are up to 1.17 to 1.9 times as long.  How many
+    // work-groups of 32 x 64 and 64 x 128 a CU has room for goes by the registers that a group size takes.
     static const Q4Form by_registers[] = {
-        q4_form<G, 16, 32, 1, 1, 8, 2, true, false>(1, 2.53f, 1.44f, 0.f, 0.f), q4_form<G, 16, 64, 1, 4, 3, 2, true, false>(2, 1.66f, 0.68f, 0.39f, 0.40f),
-        q4_form<G, 32, 64, 1, 4, 4, 2, true, false>(1, 2.69f, 1.16f, 0.f, 0.f), q4_form<G, 32, 64, 1, 4, 2, 2, true, false>(2, 2.11f, 0.69f, 0.f, 0.24f),
-        q4_form<G, 48, 64, 1, 4, 4, 2, true, false>(1, 3.41f, 1.53f, 0.f, 0.f), q4_form<G, 64, 128, 1, 4, 1, 2, true, false>(3, 3.36f, 1.06f, 1.59f, 0.43f)};
+        q4_form<G, 16, 32, 1, 1, 8, 2, true, false>(1, 1.79f, 1.34f, 0.f, 0.f), q4_form<G, 16, 64, 1, 4, 3, 2, true, false>(2, 1.44f, 0.60f, 0.36f, 0.42f),
+        q4_form<G, 32, 64, 1, 4, 4, 2, true, false>(1, 1.56f, 1.24f, 0.f, 0.f), q4_form<G, 32, 64, 1, 4, 2, 2, true, false>(G == 64 ? 2 : 3, 1.32f, 0.75f, 0.22f, 0.35f),
+        q4_form<G, 48, 64, 1, 4, 4, 2, true, false>(1, 1.89f, 1.55f, 0.f, 0.f), q4_form<G, 64, 128, 1, 4, 1, 2, true, false>(G == 128 ? 3 : 2, 2.56f, 0.93f, 1.13f, 0.33f)};
     const Q4Form *const forms = direct ? by_loads : by_registers, *best = forms;
     float least = INFINITY;
     for (const Q4Form *f = forms, *end = forms + (direct ? sizeof by_loads : sizeof by_registers) / sizeof *forms; f < end; ++f) {
