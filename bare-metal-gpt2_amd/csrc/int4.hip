@@ -528,9 +528,9 @@ static void rows_form(const Q4 &q, Q4RowsFn &fn, int &nt, int &kw) {
 }
 
 // A form for more rows, and what it takes in us: a round of work-groups `start` and `step` for each 128 k of a group of waves; each further work-group on a CU
-// that has room for `room` at once `start2` and `step2`.  Fitted to the times of 154 products of 17 to 2000 rows by 768 x 768 to 8192 x 8192 and 50257 x 768; the
-// form with the smallest sum is within 0.7% of the fastest of the nine in the mean, 9% at most, and without any one of them products are up to 1.18 to 1.5
-// times as long (the least, 16 x 64: 1.09).
+// that has room for `room` at once `start2` and `step2`.  Fitted to the times of 580 products, 17 to 1990 rows, N from 65 to 50257, K from 136 to 8152, each in groups of 32, 64
+// and 128: the form with the smallest sum is within 0.3% of the fastest of the nine in the mean, 15% at most (fitted to the first 460, 0.5% and 12% on the others); without any one of them products
+// are up to 1.16 to 1.49 times as long (the least, 64 x 64: 1.11).
 struct Q4Form {
     int bm, bn, ks, threads, room;
     float start, step, start2, step2;
@@ -543,11 +543,11 @@ static Q4Form q4_form(int room, float start, float step, float start2, float ste
 template <int G>
 static const Q4Form &tile_form(int M, int N, int kb, bool direct) {
     static const Q4Form by_loads[] = {
-        q4_form<G, 16, 32, 1, 1, 8, 2, false, true>(1, 1.54f, 0.91f, 0.f, 0.f),    q4_form<G, 16, 64, 1, 4, 3, 3, false, true>(2, 1.40f, 0.62f, 0.46f, 0.33f),
-        q4_form<G, 32, 32, 1, 2, 4, 3, false, true>(1, 1.53f, 0.72f, 0.f, 0.f),    q4_form<G, 32, 64, 1, 4, 4, 2, true, true>(1, 1.73f, 0.90f, 0.f, 0.f),
-        q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.33f, 0.62f, 0.43f, 0.28f), q4_form<G, 48, 64, 1, 4, 4, 2, true, true>(1, 1.88f, 1.11f, 0.f, 0.f),
-        q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 2.15f, 0.87f, 0.63f, 0.47f),  q4_form<G, 64, 128, 1, 4, 1, 2, true, true>(3, 1.70f, 0.78f, 1.66f, 0.33f),
-        q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 2.45f, 1.16f, 3.64f, 0.82f)};
+        q4_form<G, 16, 32, 1, 1, 8, 2, false, true>(1, 2.07f, 0.75f, 0.f, 0.f),    q4_form<G, 16, 64, 1, 4, 3, 3, false, true>(2, 1.63f, 0.58f, 0.29f, 0.48f),
+        q4_form<G, 32, 32, 1, 2, 4, 3, false, true>(1, 1.70f, 0.66f, 0.f, 0.f),    q4_form<G, 32, 64, 1, 4, 4, 2, true, true>(1, 1.89f, 0.95f, 0.f, 0.f),
+        q4_form<G, 32, 64, 1, 4, 2, 3, false, true>(2, 1.50f, 0.66f, 0.27f, 0.30f), q4_form<G, 48, 64, 1, 4, 4, 2, true, true>(1, 1.75f, 1.24f, 0.f, 0.f),
+        q4_form<G, 64, 64, 1, 2, 2, 2, true, true>(2, 1.82f, 0.97f, 0.86f, 0.41f),  q4_form<G, 64, 128, 1, 4, 1, 2, true, true>(3, 1.81f, 0.76f, 0.98f, 0.37f),
+        q4_form<G, 128, 128, 1, 4, 1, 2, true, true>(2, 3.77f, 1.25f, 1.85f, 0.67f)};
     // Rows that are not at 16 bytes: fitted to the times of 580 products, 17 to 2000 rows, N from 66 to 50257, K from 139 to 8175, each in groups of 32, 64 and 128: within 0.2% of the fastest of the six in the
     // mean, 13% at most; fitted to the first 460, 0.4% and 11% on the others.  Without any one of them products are up to 1.17 to 1.9 times as long.  How many
     // work-groups of 32 x 64 and 64 x 128 a CU has room for goes by the registers that a group size takes.

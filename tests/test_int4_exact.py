@@ -12,7 +12,8 @@ from test_gpu_int4 import run
 from test_gpu_int4_forms import FEW, MANY, ODD
 
 SIZES = FEW + MANY + ODD + [(1, 300, 8192), (7, 48, 8200), (48, 48, 8200), (90, 48, 8200), (16, 600, 8190), (33, 200, 8190), (300, 130, 8191), (1, 17, 5), (20, 40, 3), (70, 33, 1000), (5, 70, 1022),
-                            (129, 257, 1022), (400, 300, 1016), (2, 3100, 896), (300, 9001, 130), (600, 4099, 261)]
+                            (129, 257, 1022), (400, 300, 1016), (2, 3100, 896), (300, 9001, 130), (600, 4099, 261), (867, 7343, 144),
+                            (444, 4669, 776), (801, 1283, 1728)]
 
 
 class Exact:
