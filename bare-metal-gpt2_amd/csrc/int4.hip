@@ -27,7 +27,8 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int q4_word(int n, int o) { return ((o & 3) * 16 + n) * 4 + (o >> 2); }
 
 // Eight codes as exact fp16 values, in order: a code under the exponent of 1024 is 1024 + u, or with its four bits one place
-// of four higher 1024 + 16 u; u = q + 8.  The masks come from registers, so that each pair takes one instruction for mask and exponent (a vector
+// of four higher 1024 + 16 u; u = q + 8 (codes made fp16 by their exponent: Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run: Bringing Large Scale MoE Models into
+// Cloud Scale Production", 2022).  The masks come from registers, so that each pair takes one instruction for mask and exponent (a vector
 // instruction has room for one literal): a kernel makes one Q4Bits and keeps it.
 struct Q4Bits {
     uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;

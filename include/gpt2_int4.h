@@ -51,7 +51,7 @@ void gpt2_dequantize_int4(gpt2_half *dst, const GPT2Int4W *w);
 #define GPT2_EPI_NONE 0
 #define GPT2_EPI_GELU 1
 #define GPT2_EPI_ADD 2
-/* C[M][N] as above, M at most 2^21; bias [N] or NULL; resid [M][N], with GPT2_EPI_ADD only, may be C.  C overlaps neither A nor the weights.  A, C, bias and
+/* C[M][N] as above, M at most 2^21, M * N below some 2^37 (what the work-groups of one launch can have; more is refused); bias [N] or NULL; resid [M][N], with GPT2_EPI_ADD only, may be C.  C overlaps neither A nor the weights.  A, C, bias and
  * resid need the alignment of their type only; from 17 rows on, A with rows at 16 bytes (K % 8 == 0) is faster. */
 void gpt2_matmul_int4(gpt2_half *C, const gpt2_half *A, const GPT2Int4W *w, const gpt2_half *bias, int M, int epi,
                       const gpt2_half *resid);

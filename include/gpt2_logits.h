@@ -66,6 +66,8 @@ typedef struct GPT2LogitsRules {
  *     c > 0 times from `start` on:  x = x - (frequency * c + presence)
  *     -inf where the mask has no bit, or t would complete an n-gram (`ngram` tokens) that the history has
  * in fp32, rounded to fp16 once.  A NaN stays one unless it is masked or banned; a mask of nothing leaves a row of -inf.  repetition > 0.
+ * An n-gram of the history that begins as its last n - 1 tokens do is compared with them token by token, so a long history of one token, over and over, costs its
+ * length times n comparisons.
  * Without a history (NULL) there are no penalties and no n-grams.  With out == logits, rows without a mask are touched
  * only where a token is penalised, banned or biased. */
 void gpt2_logits_adjust(gpt2_half *out, const gpt2_half *logits, long ld, int rows, int V, const GPT2LogitsRules *rules);
