@@ -200,7 +200,7 @@ __device__ __forceinline__ void by_epilogue(int epi, F f) {
 // next U on the way.  A wave's piece of A goes through LDS of its own, 4 RQ rows of 256 bytes (16-byte octet o of row r at o ^ (r & 15), so that rows
 // read together lie in different banks), so nothing is waited for but the wave's own loads; where there are fewer than 16 rows the matrix unit's other
 // columns compute what nobody stores.  The waves' sums are added in wave order.
-// Bound by the stream: one row of 8192 x 8192, 34.6 MB, 8.2 us (4.2 TB/s, where a copy has 5.1), of 2304 x 768 3.0 under the tracer, the latency of a launch and one
+// Bound by the stream: one row of 8192 x 8192, 34.6 MB, 8.3 us (4.2 TB/s, where a copy has 5.1), of 2304 x 768 2.9 under the tracer, the latency of a launch and one
 // round of loads.  A tile of codes takes 36 vector instructions to become fp16 (with both masks as literals 52: 9.2 us for 8.9).
 template <int G, int RQ, int NT, int KW, int U>
 __global__ __launch_bounds__(64 * KW) void k_int4_rows(uint16_t *C, const uint16_t *__restrict__ A, Q4 w, const uint16_t *__restrict__ bias, int M, int epi,
@@ -293,8 +293,8 @@ __global__ __launch_bounds__(64 * KW) void k_int4_rows(uint16_t *C, const uint16
 // scales go to LDS by direct loads into a ring of S stages; a wave reads its fragments, makes the codes fp16 and multiplies.  WM x WN waves share a
 // stage, each with 16 TM rows and 16 TN outputs; KS such groups split K and meet in LDS.  SREG: scales in registers instead, which lets one more work-group on a
 // CU (two of 128 x 128: 2 x 80 KB); !DIRECT: everything through registers, for rows that are not at 16 bytes.
-// 2000 x 4096 x 4096 takes 71 us (0.94 PFLOP/s): with 256 x 128 tiles on eight waves (77 for 72 in one process) the matrix units had 46% of the cycles, vector
-// instructions 31 and LDS reads 26, so what is left is how they overlap; hints to the compiler's scheduling gave nothing.  A wave takes 128 rows by 32 outputs rather
+// 2000 x 4096 x 4096 takes 67 to 76 us by the card (0.88 to 1.0 PFLOP/s): by the counters of its 128 x 128 form the matrix units have 48% of the cycles, other vector
+// instructions 32 and LDS reads 25, without a bank conflict, so what is left is how they overlap; hints to the compiler's scheduling gave nothing, 256 x 128 tiles on eight waves took 77 for 72.  A wave takes 128 rows by 32 outputs rather
 // than 64 by 64, since each wave makes its codes fp16 for itself (70 us for 76).  Products of a few hundred rows are chains of short steps: 777 rows of 768
 // x 3072, six steps of 1.1 us and the launch.
 __device__ __attribute__((aligned(16))) uint32_t g_q4_zero[4] = {};   // what is multiplied past K

@@ -12,8 +12,8 @@ namespace g2 {
 // ------------------------------------------------------------------ histories
 // All sequences change at once, in place: a work-group has what it moves in its registers before it writes any.  Where parents lie in their
 // children's block of R sequences (9 to 16: one is a multiple of any number of beams up to 16), it moves such a block's rows by long pieces; else a few
-// columns of every sequence.  1024 sequences of up to 4000 tokens, with a copy of the lengths ahead: 12.3 us by blocks, in
-// groups of 8; 16.1 by columns, any sequence from any, whose rows are 64 bytes each, 16 KB apart.  The lengths, which every work-group reads, are written by the one that arrives last.
+// columns of every sequence.  1024 sequences of up to 4000 tokens, with a copy of the lengths ahead: 12.7 us by blocks, in
+// groups of 8; 14.9 by columns, any sequence from any, whose rows are 64 bytes each, 16 KB apart.  The lengths, which every work-group reads, are written by the one that arrives last.
 constexpr int HIST_THREADS = 1024, HIST_ITEMS = 4;   // pieces a thread holds: 16 sequences of 256, or 4096 of one
 
 struct HistSeq {
@@ -174,7 +174,7 @@ static bool history_refused(const GPT2History *h, const char *what) {
 // all, whether it would end a known n-gram.  The tokens that were said are listed as their first mention is counted; for those, and those with a bias, a thread each
 // works out the logit, in LDS, through which the slice goes by octets: 16 bytes of logits, wherever the row begins, a byte of the mask.  An entry of the bias list marks
 // its token; only where a list is longer than the work-group, or a token has two, are entries compared for the last.
-// 256 rows of 50257 with masks, 300 biases and histories of up to 4096 take 20.0 us (2.8 TB/s), without any of them 14: every slice goes through the row's whole
+// 256 rows of 50257 with masks, 300 biases and histories of up to 4096 take 20.1 us (2.8 TB/s), without any of them 14: every slice goes through the row's whole
 // history, and a work-group is a chain of lengths, tokens, counts and barriers.  Slices of 4096 with counts of 32 bits and a table for the biases' indexes took 24.4;
 // rules worked out where the row is copied, or claimed by a second pass over the history, 25 to 31 with either.
 // Counts have 16 bits where a history's room allows it.
